@@ -11,7 +11,7 @@ FLAGS := --offload-arch=$(ARCH) -O3 -fPIC -std=c++17 -Wall -Wno-unused-function 
 
 all: $(LIB)
 
-$(CSRC)/%.o: $(CSRC)/%.hip $(CSRC)/common.h
+$(CSRC)/%.o: $(CSRC)/%.hip $(wildcard $(CSRC)/*.h)
 	$(HIPCC) $(FLAGS) -c $< -o $@
 
 # one typed thunk per stream-taking entry point, generated from the header's declarations

@@ -15,7 +15,7 @@
  *     VQA_WALK_REV, VQA_NT_MIN_MB, VQA_CONV_PAIR, VQA_WGRAD_COF4 - they change the order in which a kernel walks its
  *     tiles, how many images share a tile, the size of a persistent grid or the cache policy of its accesses, never
  *     what is computed (outputs identical; partial-sum rows may be cut differently: fp32 summation order);
- *   - dtype codes: 0 = f32, 1 = bf16, 2 = f16 (image input only).  "T" below = the activation / MFMA dtype;
+ *   - dtype codes: 0 = f32, 1 = bf16, 2 = f16 (image input and the sequence operators).  "T" below = the activation / MFMA dtype;
  *   - activations are NHWC; matrices are row-major with an explicit leading dimension in elements.
  */
 #ifndef VQA_HIP_H
@@ -341,6 +341,61 @@ int vqa_soft_accuracy_sum_sparse(void* stream, const float* logits, const long* 
 int vqa_clip_adamax(void* stream, float* p, const float* g, float* m, float* u, long n, float max_norm, float lr,
                     float b1, float b2, float eps, int step, double* part, float* sq, float* coef,
                     float* total_norm);
+
+/* ---------------------------------------------------------------- sequence operators (vqa_amd/sequence.py)
+ * NO COUNTERPART IN THE REFERENCE: a norm, a short convolution and a linear recurrence over tokens, beside its BatchNorm,
+ * convolutions and GRU.  dtype 0, 1 or 2 (f16 as well) for the rows; parameters, states of the scan, statistics and every
+ * sum are f32.  Strides are in elements, the last axis is contiguous; 16-byte accesses are used where pointers, strides
+ * and widths allow them, element accesses elsewhere.  lengths (int32 [B], may be NULL): tokens at or past lengths[b] are
+ * padding - zero rows out, zero gradients, no part in any sum or state, whatever they hold. */
+
+/* y = (x - mean) rstd weight + bias over the last axis; x [rows] with stride ldx, y contiguous; width <= 8192; weight /
+ * bias may be NULL (1 / 0); mean, rstd [rows] (both or neither) are what the backward needs. */
+int vqa_layer_norm_fwd(void* stream, int dtype, const void* x, long ldx, const float* weight, const float* bias, long rows,
+                       int width, float eps, void* y, float* mean, float* rstd);
+int vqa_layer_norm_bwd_part(long rows, int width);      /* partial rows: part is [that][2][width] f32 */
+int vqa_layer_norm_bwd(void* stream, int dtype, const void* dy, long lddy, const void* x, long ldx, const float* weight,
+                       const float* mean, const float* rstd, long rows, int width, void* dx, float* dweight, float* dbias,
+                       float* part);
+
+/* y_t = act(bias + sum_k weight[:, k] x_{t - taps + 1 + k}), act = silu or none; x [B][L][D], weight [D][taps], taps 2..4.
+ * state [B][taps - 1][D] (dtype, may be NULL = zeros): the rows before the first; last (may be NULL): the rows that a
+ * continuation needs, from before each sequence's length.  y, dx [B][L][D], last, dlast, dstate contiguous. */
+int vqa_causal_conv_fwd(void* stream, int dtype, const void* x, long x_batch, long x_row, const float* weight,
+                        const float* bias, const void* state, const int* lengths, int B, int L, int D, int taps, int silu,
+                        void* y, void* last);
+int vqa_causal_conv_bwd_part(int B, int L, int D);      /* partial rows: part is [that][taps + 1][D] f32 */
+int vqa_causal_conv_bwd(void* stream, int dtype, const void* dy, long dy_batch, long dy_row, const void* dlast,
+                        const void* x, long x_batch, long x_row, const float* weight, const float* bias, const void* state,
+                        const int* lengths, int B, int L, int D, int taps, int silu, void* dx, float* dweight,
+                        float* dbias, void* dstate, float* part);
+/* One token per sequence: state [B][taps - 1][D] (strides given) is shifted in place. */
+int vqa_causal_conv_token(void* stream, int dtype, const void* x, long x_batch, void* state, long state_batch,
+                          long state_row, const float* weight, const float* bias, int B, int D, int taps, int silu,
+                          void* y);
+
+/* dt = softplus(dt + dt_bias) (softplus = 0: dt + dt_bias), h_t = exp(dt_t a) h_{t-1} + (dt_t x_t) b_t,
+ * y_t = (sum_n c_t h_t + skip x_t) silu(gate_t); x, dt, gate [B][L][D], a [D][N], b, c [B][L][G][N] (the last two axes
+ * contiguous), N <= 64, D % G == 0; gate, skip, dt_bias, state, lengths, last may be NULL.  state, last, dlast, dstate f32
+ * [B][D][N].  keep: what the backward needs of the forward (NULL without one); sizes (host, 3 longs) = bytes of the
+ * forward's ws, of keep, of the backward's ws; all 16-byte aligned. */
+int vqa_scan_ws_bytes(int dtype, int B, int L, int D, int N, int G, long* sizes);
+int vqa_scan_fwd(void* stream, int dtype, const void* x, long x_batch, long x_row, const void* dt, long dt_batch,
+                 long dt_row, const void* gate, long gate_batch, long gate_row, const float* a, const void* b, long b_batch,
+                 long b_row, const void* c, long c_batch, long c_row, const float* skip, const float* dt_bias, int softplus,
+                 const float* state, const int* lengths, int B, int L, int D, int N, int G, void* y, float* last,
+                 float* keep, float* ws);
+int vqa_scan_bwd(void* stream, int dtype, const void* dy, long dy_batch, long dy_row, const float* dlast, const void* x,
+                 long x_batch, long x_row, const void* dt, long dt_batch, long dt_row, const void* gate, long gate_batch,
+                 long gate_row, const float* a, const void* b, long b_batch, long b_row, const void* c, long c_batch,
+                 long c_row, const float* skip, const float* dt_bias, int softplus, const int* lengths, int B, int L, int D,
+                 int N, int G, const float* keep, void* dx, void* ddt, void* dgate, float* da, void* db, void* dc,
+                 float* dskip, float* ddt_bias, float* dstate, float* ws);
+/* One token per sequence: x, dt, gate [B][D], b, c [B][G][N]; state [B][D][N] (batch stride given) in place. */
+int vqa_scan_token(void* stream, int dtype, const void* x, long x_batch, float* state, long state_batch, const void* dt,
+                   long dt_batch, const void* gate, long gate_batch, const float* a, const void* b, long b_batch,
+                   const void* c, long c_batch, const float* skip, const float* dt_bias, int softplus, int B, int D, int N,
+                   int G, void* y);
 
 /* ---------------------------------------------------------------- one call for a recorded sequence of calls
  * NO COUNTERPART IN THE REFERENCE (its layers are one Python call each: cnn.py:49-54 `self.convolutions(x)`).

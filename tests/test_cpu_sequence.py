@@ -1,0 +1,70 @@
+"""CPU: the sequence operators' entry points refuse what their kernels do not take before anything is launched, and size
+their workspaces consistently."""
+import ctypes
+
+import pytest
+import torch
+
+
+def test_cpu_tensors_are_refused():
+    from vqa_amd import sequence as S
+    from vqa_amd._lib import VqaHipError
+    x = torch.zeros(2, 3, 8)
+    for f in (lambda: S.layer_norm(x), lambda: S.causal_conv(x, torch.zeros(8, 4)),
+              lambda: S.causal_conv_step(x[:, 0], x, torch.zeros(8, 4)),
+              lambda: S.selective_scan(x, x, torch.zeros(8, 4), x[..., :4], x[..., :4]),
+              lambda: S.selective_scan_step(x[:, 0], torch.zeros(2, 8, 4), x[:, 0], torch.zeros(8, 4), x[:, 0, :4], x[:, 0, :4])):
+        with pytest.raises(VqaHipError, match='GPU'):
+            f()
+
+
+P = ctypes.c_void_p(64)          # never dereferenced: every call below is refused by the host code
+
+
+def test_entry_points_refuse_bad_arguments():
+    from vqa_amd import _lib as L
+    lib = L.lib()
+    norm = lambda dtype=0, x=P, rows=4, width=8, y=P, mean=P, rstd=P: lib.vqa_layer_norm_fwd(      # noqa: E731
+        None, dtype, x, width, None, None, rows, width, 1e-5, y, mean, rstd)
+    assert all(rc == 1 for rc in (norm(dtype=3), norm(x=None), norm(rows=0), norm(width=0), norm(width=8193),
+                                  norm(y=None), norm(mean=None), norm(rows=1 << 31)))
+    assert lib.vqa_layer_norm_bwd(None, 0, P, 8, P, 8, None, P, P, 4, 8, P, None, None, None) == 1
+    assert lib.vqa_layer_norm_bwd(None, 0, P, 8, P, 8, None, None, P, 4, 8, P, None, None, P) == 1
+    assert lib.vqa_layer_norm_bwd_part(0, 8) == 0 and lib.vqa_layer_norm_bwd_part(4, 9000) == 0
+    conv = lambda dtype=0, B=1, T=4, D=8, taps=4, w=P: lib.vqa_causal_conv_fwd(                    # noqa: E731
+        None, dtype, P, T * D, D, w, None, None, None, B, T, D, taps, 1, P, None)
+    assert all(rc == 1 for rc in (conv(dtype=-1), conv(B=0), conv(T=0), conv(D=0), conv(taps=1), conv(taps=5),
+                                  conv(w=None), conv(B=1 << 20, T=1 << 20)))
+    assert lib.vqa_causal_conv_bwd_part(0, 4, 8) == 0
+    assert lib.vqa_causal_conv_token(None, 0, P, 8, None, 24, 8, P, None, 1, 8, 4, 1, P) == 1
+    sizes = (ctypes.c_long * 3)()
+    at = ctypes.addressof(sizes)
+    for args in ((0, 0, 4, 8, 16, 1), (0, 1, 0, 8, 16, 1), (0, 1, 4, 8, 65, 1), (0, 1, 4, 8, 0, 1), (0, 1, 4, 9, 16, 2),
+                 (5, 1, 4, 8, 16, 1), (0, 1, 1 << 30, 8, 16, 1), (0, 1, 4, 8, 16, 0)):
+        assert lib.vqa_scan_ws_bytes(*args, at) == 1, args
+    assert lib.vqa_scan_ws_bytes(0, 1, 4, 8, 16, 1, None) == 1
+
+    def scan(B=1, T=1024, D=8, N=16, G=1, ws=P, keep=None, y=P):
+        return lib.vqa_scan_fwd(None, 0, P, T * D, D, P, T * D, D, None, 0, 0, P, P, T * N, N, P, T * N, N, None, None, 1,
+                                None, None, B, T, D, N, G, y, None, keep, ws)
+    assert all(rc == 1 for rc in (scan(ws=None), scan(ws=ctypes.c_void_p(68)), scan(keep=ctypes.c_void_p(72)), scan(N=65),
+                                  scan(G=3), scan(y=None), scan(B=0)))
+
+
+def test_scan_workspaces_hold_what_the_kernels_write():
+    """The forward's segments, the kept states and the backward's partial sums, from the sizes alone."""
+    from vqa_amd import _lib as L
+    lib = L.lib()
+    for B, T, D, N, G in ((1, 1, 1, 1, 1), (256, 14, 2048, 16, 1), (1, 16383, 2048, 16, 1), (3, 577, 600, 16, 2),
+                          (4, 2048, 2048, 16, 1), (2, 100, 64, 64, 4), (7, 700, 33, 20, 1)):
+        sizes = (ctypes.c_long * 3)()
+        assert lib.vqa_scan_ws_bytes(1, B, T, D, N, G, ctypes.addressof(sizes)) == 0
+        fwd, keep, bwd = sizes
+        channels = 64 if N <= 16 else 32 if N <= 32 else 16
+        waves = G * -(-(D // G) // channels)
+        assert keep == 4 * 1024 * B * waves * -(-T // 8)
+        assert bwd >= fwd + 4 * (waves // G) * B * T * G * 2 * N + 4 * waves * 1024
+        assert all(s % 16 == 0 for s in (fwd, keep)) and fwd >= 0
+        if fwd:
+            segments = fwd // (4 * B * waves * (1024 + channels))
+            assert fwd == 4 * B * waves * (1024 + channels) * segments and 1 < segments <= max(1, T // 64)

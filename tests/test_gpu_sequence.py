@@ -1,0 +1,637 @@
+"""GPU: the sequence operators (vqa_amd.sequence) against the same formulas token by token in 64 bits: outputs, gradients,
+padded batches, carried states, single tokens, strides, types, streams, graphs, refusals.
+
+Roundings counted in a tolerance (sequence_ref.close): layer norm and the convolution chain a few operations per value plus
+their sums' partial chains (rows / 16 rows side by side); a scan's state takes 3 roundings a token and its decay's error is
+that of dt (about 16: softplus by exponential, reciprocal and a series of 7 terms) times dt a e^{dt a} <= 1/e."""
+import pytest
+import torch
+
+from tests import sequence_ref as R
+
+pytestmark = pytest.mark.gpu
+
+DT = {'f32': torch.float32, 'bf16': torch.bfloat16, 'f16': torch.float16}
+
+
+def S():
+    from vqa_amd import sequence
+    return sequence
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _leaf(t, dtype=torch.float32):
+    """(GPU leaf in dtype, CPU float64 leaf of the same values)"""
+    if t is None:
+        return None, None
+    t = t.to(dtype)
+    return t.cuda().requires_grad_(True), t.double().requires_grad_(True)
+
+
+def _grads(outs, seeds, leaves):
+    names = [k for k, v in leaves.items() if v is not None]
+    got = torch.autograd.grad([o for o in outs if o is not None], [leaves[k] for k in names],
+                              [s for o, s in zip(outs, seeds) if o is not None])
+    return dict(zip(names, got))
+
+
+# ---------------------------------------------------------------------------------------------------------- layer norm
+
+@pytest.mark.parametrize('rows,width,dtype', [
+    (1, 1, 'f32'), (3, 2, 'bf16'), (14, 300, 'f32'), (5, 300, 'bf16'), (7, 513, 'f16'), (65, 1024, 'bf16'),
+    (130, 64, 'f32'), (9, 1025, 'bf16'), (33, 2048, 'bf16'), (12, 2047, 'f32'), (6, 4096, 'f16'), (5, 4095, 'bf16'),
+    (4, 8192, 'f32'), (3, 8191, 'bf16'), (2100, 40, 'bf16')])
+def test_layer_norm(rows, width, dtype):
+    g = _gen(rows * 10007 + width)
+    x, xr = _leaf(torch.randn(rows, width, generator=g) * 2 + 0.5, DT[dtype])
+    w, wr = _leaf(1 + 0.1 * torch.randn(width, generator=g))
+    b, br = _leaf(0.1 * torch.randn(width, generator=g))
+    dy = torch.randn(rows, width, generator=g).to(DT[dtype])
+    y, yr = S().layer_norm(x, w, b), R.norm(xr, wr, br)
+    assert y.dtype == x.dtype
+    if width == 1:
+        # a row of one value: x - mean is 0, rstd is 1 / sqrt(eps) = 316 and no gradient reaches x
+        R.close('y', y, yr, 16)
+        (dx,) = torch.autograd.grad(y, [x], dy.cuda())
+        assert not dx.any()
+        return
+    R.close('y', y, yr, 32)
+    got = _grads([y], [dy.cuda()], dict(x=x, w=w, b=b))
+    want = _grads([yr], [dy.double()], dict(x=xr, w=wr, b=br))
+    # dx = rstd (g - mean(g) - xh mean(g xh)), g = dy w: each of the three terms is at most rstd max|g| sqrt(width) and
+    # rounded a few times, while their sum may cancel altogether (two values a row: xh = +-1, the sum is 0 but for eps),
+    # so dx's rounding is counted at the terms' size.  max|xh| <= sqrt(width); mean(g xh) <= max|g|.
+    rstd = float(1 / torch.sqrt(xr.detach().var(-1, unbiased=False) + 1e-5).max())
+    terms = rstd * float((dy.double() * wr).abs().max()) * float(((xr - xr.mean(-1, keepdim=True)).abs().amax(-1) /
+                                                                  xr.std(-1, unbiased=False)).max())
+    R.close('dx', got['x'], want['x'], 64, scale=terms)
+    R.close('dw', got['w'], want['w'], 64 + rows)
+    R.close('db', got['b'], want['b'], 64 + rows)
+
+
+@pytest.mark.parametrize('weight,bias', [(False, False), (True, False), (False, True)])
+def test_layer_norm_without_parameters_and_in_three_axes(weight, bias):
+    g = _gen(3)
+    x, xr = _leaf(torch.randn(4, 5, 72, generator=g), torch.bfloat16)
+    w, wr = _leaf(torch.randn(72, generator=g)) if weight else (None, None)
+    b, br = _leaf(torch.randn(72, generator=g)) if bias else (None, None)
+    dy = torch.randn(4, 5, 72, generator=g).bfloat16()
+    y, yr = S().layer_norm(x, w, b, eps=1e-3), R.norm(xr, wr, br, 1e-3)
+    R.close('y', y, yr, 32)
+    got, want = _grads([y], [dy.cuda()], dict(x=x, w=w, b=b)), _grads([yr], [dy.double()], dict(x=xr, w=wr, b=br))
+    for k in got:
+        R.close(k, got[k], want[k], 128)
+
+
+@pytest.mark.parametrize('width,dtype', [(48, 'bf16'), (47, 'f32'), (2048, 'bf16')])
+def test_layer_norm_of_strided_rows(width, dtype):
+    """Rows of a wider matrix (aligned and not), every other row, a transposed matrix, a broadcast row, a broadcast dy."""
+    g = _gen(5)
+    base = torch.randn(10, 2 * width + 8, generator=g).to(DT[dtype])
+    w = torch.randn(width, generator=g)
+    dev = base.cuda()
+    for name, f in {'aligned': lambda m: m[:, 8:8 + width], 'odd': lambda m: m[:, 3:3 + width],
+                    'alternate': lambda m: m[::2, :width], 'transposed': lambda m: m[:, :10].t()[:, :7],
+                    'broadcast': lambda m: m[:1, :width].expand(6, width)}.items():
+        x, xr = f(dev), f(base).double()
+        ww = w[:x.shape[1]]
+        y = S().layer_norm(x, ww.cuda(), None)
+        R.close(name, y, R.norm(xr, ww.double(), None), 32)
+        assert y.is_contiguous()
+    x, xr = _leaf(base[:, :width], DT[dtype])
+    y, yr = S().layer_norm(x), R.norm(xr, None, None)
+    y.sum().backward()                                       # dy with strides 0
+    # xhat sums to 0 over a row, so the exact gradient of the sum is 0: what is left is rounding of terms of size rstd
+    assert float(x.grad.abs().max()) <= 64 * 2.0 ** -24 * float(1 / xr.std(1, unbiased=False).min())
+
+
+def test_layer_norm_extremes():
+    """A constant row (variance 0), a row far from 0, rows with NaN and infinity: each row by itself."""
+    g = _gen(6)
+    x = torch.randn(6, 384, generator=g)
+    x[0] = 3.25
+    x[1] += 4096
+    x[2, 5] = float('nan')
+    x[3, 7] = float('inf')
+    y = S().layer_norm(x.cuda()).cpu()
+    assert not y[0].any()
+    # the mean of values near 4096 is off by a few of its half steps, 2^-12 each; y has the scale 1
+    assert float((y[1].double() - R.norm(x[1:2].double(), None, None)[0]).abs().max()) <= 8 * 2.0 ** -12
+    assert torch.isnan(y[2]).all() and torch.isnan(y[3]).all()
+    R.close('rest', y[4:], R.norm(x[4:].double(), None, None), 32)
+    w = torch.ones(384, device='cuda', requires_grad=True)
+    assert S().layer_norm(torch.empty(0, 384, device='cuda'), w).shape == (0, 384)
+    S().layer_norm(torch.empty(0, 384, device='cuda'), w).sum().backward()
+    assert not w.grad.any()
+
+
+# --------------------------------------------------------------------------------------------------- causal convolution
+
+def _conv_case(B, T, D, taps, dtype, act, lengths, carry, seed=0, bias=True):
+    g = _gen(seed + B * 1000 + T * 10 + D)
+    t = DT[dtype]
+    raw = torch.randn(B, T, D, generator=g)
+    w = torch.randn(D, taps, generator=g) / taps ** 0.5
+    lens = torch.tensor(lengths, dtype=torch.int32) if lengths is not None else None
+    dy, dlast = torch.randn(B, T, D, generator=g).to(t), torch.randn(B, taps - 1, D, generator=g).to(t)
+    leaves = dict(x=_leaf(raw, t), w=_leaf(w), b=_leaf(0.2 * torch.randn(D, generator=g)) if bias else (None, None),
+                  state=_leaf(torch.randn(B, taps - 1, D, generator=g), t) if carry else (None, None))
+    return leaves, lens, dy, dlast
+
+
+@pytest.mark.parametrize('B,T,D,taps,dtype,act,lengths,carry', [
+    (1, 1, 1, 4, 'f32', 'silu', None, False), (2, 1, 8, 3, 'bf16', 'silu', None, True),
+    (3, 2, 7, 4, 'f32', None, None, True), (4, 14, 64, 4, 'bf16', 'silu', [14, 0, 1, 9], True),
+    (2, 33, 300, 2, 'f16', 'silu', [2, 33], False), (3, 65, 96, 3, 'bf16', None, [64, 3, 70], True),
+    (1, 200, 2048, 4, 'bf16', 'silu', None, True), (5, 71, 515, 4, 'f32', 'silu', [71, 70, -3, 2, 3], True),
+    (70, 9, 24, 4, 'bf16', 'silu', None, False)])
+def test_causal_conv(B, T, D, taps, dtype, act, lengths, carry):
+    leaves, lens, dy, dlast = _conv_case(B, T, D, taps, dtype, act, lengths, carry)
+    (x, xr), (w, wr), (b, br), (st, sr) = (leaves[k] for k in ('x', 'w', 'b', 'state'))
+    dlen = lens.cuda() if lens is not None else None
+    y, last = S().causal_conv(x, w, b, act, state=st, lengths=dlen, return_state=True)
+    yr, lastr = R.conv(xr, wr, br, act, sr, lens)
+    R.close('y', y, yr, 32)
+    assert torch.equal(last.detach().cpu().double(), lastr.detach())          # copies of rows
+    got = _grads([y, last], [dy.cuda(), dlast.cuda()], dict(x=x, w=w, b=b, state=st))
+    want = _grads([yr, lastr], [dy.double(), dlast.double()], dict(x=xr, w=wr, b=br, state=sr))
+    for k in got:
+        R.close('d' + k, got[k], want[k], 64 if k in ('x', 'state') else 64 + B * T)
+    if lens is not None:                                     # padding may hold anything, in x and in dy
+        bad, bady = x.detach().clone(), dy.cuda()
+        for i, n in enumerate(lengths):
+            bad[i, max(0, n):], bady[i, max(0, n):] = float('nan'), float('inf')
+        bad.requires_grad_(True)
+        y2, last2 = S().causal_conv(bad, w, b, act, state=st, lengths=dlen, return_state=True)
+        assert torch.equal(y2, y) and torch.equal(last2, last)
+        again = _grads([y2, last2], [bady, dlast.cuda()], dict(x=bad, w=w, b=b, state=st))
+        for k in again:
+            assert torch.equal(again[k], got[k]), k
+
+
+def test_causal_conv_parts_of_outputs():
+    """Only y, only the state, no bias; a state that nothing needs."""
+    leaves, _, dy, dlast = _conv_case(2, 6, 16, 4, 'f32', 'silu', None, True, bias=False)
+    (x, xr), (w, wr), (st, sr) = (leaves[k] for k in ('x', 'w', 'state'))
+    y = S().causal_conv(x, w, state=st)
+    yr, lastr = R.conv(xr, wr, None, 'silu', sr, None)
+    got, want = (_grads([o], [d], l) for o, d, l in ((y, dy.cuda(), dict(x=x, w=w, s=st)),
+                                                     (yr, dy.double(), dict(x=xr, w=wr, s=sr))))
+    for k in got:
+        R.close(k, got[k], want[k], 128)
+    _, last = S().causal_conv(x, w, state=st, return_state=True)
+    gx, gw = torch.autograd.grad(last, [x, w], dlast.cuda())
+    assert torch.equal(gx[:, 3:], dlast.cuda()) and not gx[:, :3].any() and not gw.any()
+    y0, last0 = S().causal_conv(x[:, :0], w, state=st, return_state=True)
+    assert y0.shape == (2, 0, 16) and torch.equal(last0, st)
+    assert torch.autograd.grad(last0, st, dlast.cuda())[0].equal(dlast.cuda())
+
+
+@pytest.mark.parametrize('dtype,D', [('bf16', 64), ('f32', 33)])
+def test_causal_conv_strided_and_broadcast(dtype, D):
+    """x as half of a projection's output, time-major x, one sequence broadcast over the batch (gradient summed)."""
+    g = _gen(11)
+    t = DT[dtype]
+    w = torch.randn(D, 4, generator=g)
+    wide = torch.randn(3, 10, 2 * D, generator=g).to(t)
+    for f in (lambda m: m[..., :D], lambda m: m[..., D:], lambda m: m[..., 1:D + 1], lambda m: m.transpose(0, 1)[..., :D],
+              lambda m: m[:, ::2, :D], lambda m: m[..., ::2]):
+        x = f(wide.cuda())
+        y = S().causal_conv(x, w.cuda())
+        R.close('y', y, R.conv(f(wide).double(), w.double(), None, 'silu', None, None)[0], 32)
+    one, oner = _leaf(wide[:1, :, :D], t)
+    dy = torch.randn(4, 10, D, generator=g).to(t)
+    (gx,) = torch.autograd.grad(S().causal_conv(one.expand(4, -1, -1), w.cuda()), one, dy.cuda())
+    (want,) = torch.autograd.grad(R.conv(oner.expand(4, -1, -1), w.double(), None, 'silu', None, None)[0], oner, dy.double())
+    # four rounded rows are summed by autograd in x's type: 4 half steps of the terms, 3 of the partial sums
+    tol = 8 * torch.finfo(t).eps * float(want.abs().max())
+    assert float((gx.cpu().double() - want).abs().max()) <= tol
+
+
+@pytest.mark.parametrize('B,D,taps,dtype', [(1, 1, 2, 'f32'), (3, 64, 4, 'bf16'), (5, 301, 3, 'f16'), (300, 24, 4, 'bf16')])
+def test_causal_conv_steps_continue_a_sequence(B, D, taps, dtype):
+    """A padded prompt, then tokens one at a time = the whole sequence at once, bit for bit (one order of sums)."""
+    g = _gen(12)
+    t = DT[dtype]
+    w, b = torch.randn(D, taps, generator=g).cuda(), torch.randn(D, generator=g).cuda()
+    x = torch.randn(B, 9, D, generator=g).to(t).cuda()
+    n = torch.randint(0, 6, (B,), generator=g, dtype=torch.int32)
+    whole = S().causal_conv(x, w, b)
+    _, state = S().causal_conv(x[:, :5], w, b, lengths=n.cuda(), return_state=True)
+    pool = torch.full((B, taps - 1, 2 * D), 7.0, device='cuda', dtype=t)        # a state kept as part of something wider
+    pool[..., :D] = state
+    for k in range(3):
+        at = (n.long() + k).cuda().clamp(max=8)
+        tok = x[torch.arange(B, device='cuda'), at]
+        y = S().causal_conv_step(tok, state, w, b)
+        assert torch.equal(S().causal_conv_step(tok, pool[..., :D], w, b), y)
+        assert torch.equal(y, whole[torch.arange(B, device='cuda'), at])
+    assert torch.equal(pool[..., :D], state) and (pool[..., D:] == 7).all()
+
+
+# ------------------------------------------------------------------------------------------------- selective state space
+
+SCAN = ('x', 'dt', 'a', 'b', 'c', 'skip', 'gate', 'dt_bias', 'state')
+
+
+def _scan_case(B, T, D, N, G, dtype, seed=0, carry=True, without=()):
+    g = _gen(seed + B * 1000 + T * 10 + D + N)
+    t = DT[dtype]
+    rn = lambda *s: torch.randn(*s, generator=g)                                # noqa: E731
+    v = dict(x=rn(B, T, D), dt=0.5 * rn(B, T, D), a=-(0.2 + 4 * torch.rand(D, N, generator=g)), b=rn(B, T, G, N),
+             c=rn(B, T, G, N), skip=rn(D), gate=rn(B, T, D), dt_bias=rn(D) - 2, state=rn(B, D, N) if carry else None)
+    leaves = {k: (None, None) if v[k] is None or k in without else
+              _leaf(v[k], torch.float32 if k in ('a', 'skip', 'dt_bias', 'state') else t) for k in SCAN}
+    return leaves, rn(B, T, D).to(t), rn(B, D, N)
+
+
+def _scan_check(leaves, dy, dlast, lens, softplus=True):
+    B, T, D = dy.shape
+    G = {k: v[0] for k, v in leaves.items()}
+    C = {k: v[1] for k, v in leaves.items()}
+    dlen = lens.cuda() if lens is not None else None
+    y, last = S().selective_scan(*(G[k] for k in SCAN[:8]), softplus=softplus, state=G['state'], lengths=dlen,
+                                 return_state=True)
+    yr, lastr = R.scan(*(C[k] for k in SCAN[:8]), softplus, C['state'], lens)
+    n = 128 + 8 * T
+    R.close('y', y, yr, n)
+    R.close('last', last, lastr, n)
+    got = _grads([y, last], [dy.cuda(), dlast.cuda()], G)
+    want = _grads([yr, lastr], [dy.double(), dlast.double()], C)
+    for k in got:
+        # db, dc sum over the channels of a group; parameter gradients over all tokens
+        R.close('d' + k, got[k], want[k], 2 * n + {'b': D, 'c': D}.get(k, B * T if k in ('a', 'skip', 'dt_bias') else 0))
+    return G, y, last, got
+
+
+@pytest.mark.parametrize('B,T,D,N,G,dtype,lengths', [
+    (1, 1, 1, 1, 1, 'f32', None), (2, 3, 5, 3, 1, 'bf16', None), (1, 7, 64, 16, 1, 'bf16', None),
+    (2, 8, 65, 16, 1, 'f32', None), (3, 9, 128, 16, 2, 'bf16', [9, 0, 5]), (2, 17, 48, 8, 1, 'f16', [1, 17]),
+    (2, 14, 33, 17, 1, 'f32', None), (1, 23, 64, 32, 2, 'bf16', None), (2, 19, 40, 64, 1, 'bf16', [18, 30]),
+    (2, 12, 36, 33, 4, 'f32', [-1, 12]), (9, 5, 16, 16, 1, 'f32', None)])
+def test_selective_scan(B, T, D, N, G, dtype, lengths):
+    lens = torch.tensor(lengths, dtype=torch.int32) if lengths is not None else None
+    leaves, dy, dlast = _scan_case(B, T, D, N, G, dtype)
+    ins, y, last, got = _scan_check(leaves, dy, dlast, lens)
+    if lens is not None:                                     # padding may hold anything
+        bad, bady = {k: v.detach().clone() for k, v in ins.items()}, dy.cuda()
+        for i, n in enumerate(lengths):
+            for j, k in enumerate(('x', 'dt', 'b', 'c', 'gate')):
+                bad[k][i, max(0, n):] = (float('nan'), float('inf'), float('-inf'))[j % 3]
+            bady[i, max(0, n):] = float('nan')
+        bad = {k: v.requires_grad_(True) for k, v in bad.items()}
+        y2, last2 = S().selective_scan(*(bad[k] for k in SCAN[:8]), state=bad['state'], lengths=lens.cuda(),
+                                       return_state=True)
+        assert torch.equal(y2, y) and torch.equal(last2, last)
+        again = _grads([y2, last2], [bady, dlast.cuda()], bad)
+        for k in again:
+            assert torch.equal(again[k], got[k]), k
+
+
+@pytest.mark.parametrize('B,T,D,N,G,dtype,lengths', [
+    (1, 600, 32, 16, 1, 'f32', None), (2, 333, 72, 16, 1, 'bf16', [200, 333]), (1, 257, 24, 40, 2, 'f32', [256]),
+    (2, 130, 17, 20, 1, 'bf16', [0, 64])])
+def test_selective_scan_in_segments(B, T, D, N, G, dtype, lengths):
+    """Few rows and a long axis: the tokens are cut into segments that are joined again."""
+    lens = torch.tensor(lengths, dtype=torch.int32) if lengths is not None else None
+    leaves, dy, dlast = _scan_case(B, T, D, N, G, dtype, seed=1)
+    _scan_check(leaves, dy, dlast, lens)
+
+
+@pytest.mark.parametrize('without,softplus,carry', [(('gate',), True, False), (('skip', 'dt_bias'), True, True),
+                                                    (('gate', 'skip', 'dt_bias'), False, False)])
+def test_selective_scan_options(without, softplus, carry):
+    leaves, dy, dlast = _scan_case(2, 21, 40, 16, 1, 'f32', seed=2, carry=carry, without=without)
+    if not softplus:                                         # dt as it is: positive, so that the states stay bounded
+        dt = 0.1 * torch.rand(2, 21, 40, generator=_gen(9))
+        leaves['dt'] = _leaf(dt)
+    _scan_check(leaves, dy, dlast, None, softplus)
+
+
+def test_selective_scan_many_sequences_in_one_wave():
+    """More batch rows than waves are wanted for: a wave takes several, its parameter sums run on."""
+    B, T, D, N = 300, 3, 1024, 16
+    leaves, dy, _ = _scan_case(B, T, D, N, 1, 'f32', seed=3, carry=False)
+    G = {k: v[0] for k, v in leaves.items()}
+    y = S().selective_scan(*(G[k] for k in SCAN[:8]))
+    got = _grads([y], [dy.cuda()], G)
+    half = {k: 0 for k in ('a', 'skip', 'dt_bias')}
+    for lo in range(0, B, 100):                              # the same sums, from three calls that take one row a wave
+        part = {k: (v.detach()[lo:lo + 100] if k in ('x', 'dt', 'b', 'c', 'gate') else v.detach()).requires_grad_(True)
+                for k, v in G.items() if v is not None}
+        p = S().selective_scan(*(part[k] for k in SCAN[:8]))
+        assert torch.equal(p, y[lo:lo + 100])
+        gp = _grads([p], [dy.cuda()[lo:lo + 100]], part)
+        for k in ('x', 'dt', 'b', 'c', 'gate'):
+            assert torch.equal(gp[k], got[k][lo:lo + 100]), k
+        for k in half:
+            half[k] = half[k] + gp[k].double()
+    for k in half:
+        R.close(k, got[k], half[k].cpu(), 2 * B * T)
+
+
+@pytest.mark.parametrize('dtype,D', [('bf16', 64), ('f32', 20)])
+def test_selective_scan_strided_and_shared(dtype, D):
+    """Rows as slices of projections' outputs, b and c as one slice [B, L, N] each, one sequence's b broadcast."""
+    g = _gen(14)
+    t, N = DT[dtype], 16
+    rn = lambda *s: torch.randn(*s, generator=g)                                # noqa: E731
+    proj, small = rn(3, 11, 3 * D).to(t), rn(3, 11, 5 + 2 * N).to(t)
+    a, bias = -(0.2 + 3 * torch.rand(D, N, generator=g)), rn(D) - 2
+    args = lambda p, s: (p[..., :D], p[..., D:2 * D], s[..., 5:5 + N], s[..., 5 + N:], p[..., 2 * D:])  # noqa: E731
+    x, dt, b, c, gate = args(proj.cuda(), small.cuda())
+    y = S().selective_scan(x, dt, a.cuda(), b, c, None, gate, bias.cuda())
+    x, dt, b, c, gate = args(proj.double(), small.double())
+    yr, _ = R.scan(x, dt, a.double(), b[:, :, None], c[:, :, None], None, gate, bias.double(), True, None, None)
+    R.close('y', y, yr, 256)
+    p, s = proj.cuda(), small.cuda().requires_grad_(True)
+    x, dt, b, c, gate = args(p, s)
+    tm = [v.transpose(0, 1).contiguous().transpose(0, 1) for v in (x, dt, gate)]          # time-major rows
+    y2 = S().selective_scan(tm[0], tm[1], a.cuda(), b, c, None, tm[2], bias.cuda())
+    assert torch.equal(y2, y)
+    one = b[:1].detach().requires_grad_(True)
+    cc = c.detach()
+    (gb,) = torch.autograd.grad(S().selective_scan(x, dt, a.cuda(), one.expand(3, -1, -1), cc, None, gate, bias.cuda()),
+                                one, torch.ones_like(y))
+    full = one.expand(3, -1, -1).detach().clone().requires_grad_(True)
+    (gf,) = torch.autograd.grad(S().selective_scan(x, dt, a.cuda(), full, cc, None, gate, bias.cuda()), full,
+                                torch.ones_like(y))
+    assert float((gb.double() - gf.double().sum(0, keepdim=True)).abs().max()) <= 4 * torch.finfo(t).eps * float(
+        gf.double().abs().sum(0).max())
+
+
+def test_selective_scan_of_nothing():
+    leaves, _, dlast = _scan_case(2, 3, 16, 16, 1, 'f32')
+    G = {k: v[0] for k, v in leaves.items()}
+    cut = {k: v[:, :0] if k in ('x', 'dt', 'b', 'c', 'gate') else v for k, v in G.items()}
+    y, last = S().selective_scan(*(cut[k] for k in SCAN[:8]), state=G['state'], return_state=True)
+    assert y.shape == (2, 0, 16) and torch.equal(last, G['state'])
+    gs, ga = torch.autograd.grad(last, [G['state'], G['a']], dlast.cuda())
+    assert torch.equal(gs, dlast.cuda()) and not ga.any()
+
+
+@pytest.mark.parametrize('B,D,N,G,dtype', [(1, 1, 1, 1, 'f32'), (3, 64, 16, 1, 'bf16'), (2, 40, 5, 2, 'f32'),
+                                           (4, 48, 8, 1, 'f16'), (2, 24, 33, 1, 'bf16'), (3, 32, 64, 4, 'f32')])
+def test_selective_scan_steps_continue_a_sequence(B, D, N, G, dtype):
+    """A padded prompt, then tokens one at a time, against the whole sequences in 64 bits; the state in a wider pool."""
+    T, steps = 6, 3
+    leaves, _, _ = _scan_case(B, T + steps, D, N, G, dtype, seed=4, carry=False)
+    g = {k: v[0].detach() if v[0] is not None else None for k, v in leaves.items()}
+    n = torch.randint(0, T + 1, (B,), generator=_gen(5), dtype=torch.int32)
+    _, state = S().selective_scan(*(g[k][:, :T] if k in ('x', 'dt', 'b', 'c', 'gate') else g[k] for k in SCAN[:8]),
+                                  lengths=n.cuda(), return_state=True)
+    pool = torch.full((B, 2, D, N), 5.0, device='cuda')
+    pool[:, 1] = state
+    rows = torch.arange(B, device='cuda')
+    yr, hr = R.scan(*(leaves[k][1] for k in SCAN[:8]), True, None, n + steps)
+    for k in range(steps):
+        at = n.long().cuda() + k
+        tok = {q: g[q][rows, at] for q in ('x', 'dt', 'b', 'c', 'gate')}
+        args = (tok['dt'], g['a'], tok['b'], tok['c'], g['skip'], tok['gate'], g['dt_bias'])
+        y = S().selective_scan_step(tok['x'], state, *args)
+        assert torch.equal(S().selective_scan_step(tok['x'], pool[:, 1], *args), y)
+        R.close('y', y, yr[torch.arange(B), n.long() + k], 128 + 8 * (T + steps))
+    R.close('state', state, hr, 128 + 8 * (T + steps))
+    assert torch.equal(pool[:, 1], state) and (pool[:, 0] == 5).all()
+
+
+# ------------------------------------------------------------------------------------------------------------- together
+
+def _block(P, x, lengths=None, states=None, keep=False):
+    """One token-mixing block: norm, projection, convolution, projections of dt / b / c, scan, projection."""
+    s = S()
+    D, N = P['a'].shape
+    h = s.layer_norm(x, P['nw'], P['nb'])
+    xz = h @ P['win']
+    u = s.causal_conv(xz[..., :D], P['wc'], P['bc'], state=states and states[0], lengths=lengths, return_state=True)
+    dbc = u[0] @ P['wx']
+    y = s.selective_scan(u[0], dbc[..., :D], P['a'], dbc[..., D:D + N], dbc[..., D + N:], P['skip'], xz[..., D:],
+                         P['dtb'], state=states and states[1], lengths=lengths, return_state=True)
+    out = x + y[0] @ P['wout']
+    return (out, (u[1], y[1])) if keep else out
+
+
+def _block_ref(P, x, lengths):
+    D, N = P['a'].shape
+    xz = R.norm(x, P['nw'], P['nb']) @ P['win']
+    u, _ = R.conv(xz[..., :D], P['wc'], P['bc'], 'silu', None, lengths)
+    dbc = u @ P['wx']
+    y, _ = R.scan(u, dbc[..., :D], P['a'], dbc[..., None, D:D + N], dbc[..., None, D + N:], P['skip'], xz[..., D:],
+                  P['dtb'], True, None, lengths)
+    return x + y @ P['wout']
+
+
+def _block_params(C, D, N):
+    g = _gen(21)
+    rn = lambda *s: torch.randn(*s, generator=g)                                # noqa: E731
+    p = dict(nw=1 + 0.1 * rn(C), nb=0.1 * rn(C), win=rn(C, 2 * D) / C ** 0.5, wc=rn(D, 4) / 2, bc=0.1 * rn(D),
+             wx=rn(D, D + 2 * N) / D ** 0.5, a=-(0.2 + 3 * torch.rand(D, N, generator=g)), skip=rn(D), dtb=rn(D) - 2,
+             wout=rn(D, C) / D ** 0.5)
+    return {k: v.cuda().requires_grad_(True) for k, v in p.items()}, {k: v.double().requires_grad_(True) for k, v in p.items()}
+
+
+def test_block_trains():
+    """All operators in one float32 block over a padded batch: the loss's gradient for every parameter and the input."""
+    P, Pr = _block_params(24, 48, 16)
+    x, xr = _leaf(torch.randn(3, 14, 24, generator=_gen(22)))
+    lens = torch.tensor([14, 5, 9], dtype=torch.int32)
+    out, ref = _block(P, x, lens.cuda()), _block_ref(Pr, xr, lens)
+    dy = torch.randn(3, 14, 24, generator=_gen(23))
+    # the chain of all operators: the scan's 128 + 8 T, the products' sums of at most 96 terms, amplified by each other
+    R.close('out', out, ref, 2048)
+    got, want = _grads([out], [dy.cuda()], dict(P, x=x)), _grads([ref], [dy.double()], dict(Pr, x=xr))
+    for k in got:
+        R.close('d' + k, got[k], want[k], 8192)
+
+
+def test_block_reads_a_padded_prompt_and_then_single_tokens():
+    P, Pr = _block_params(16, 32, 16)
+    s = S()
+    x = torch.randn(3, 9, 16, generator=_gen(24))
+    n = torch.tensor([4, 1, 6], dtype=torch.int32)
+    with torch.no_grad():
+        _, (cs, hs) = _block(P, x[:, :6].cuda(), n.cuda(), keep=True)
+        ref = _block_ref(Pr, x.double(), None)
+        D, N = P['a'].shape
+        for k in range(3):
+            at = n.long() + k
+            tok = x[torch.arange(3), at].cuda()
+            xz = s.layer_norm(tok, P['nw'], P['nb']) @ P['win']
+            u = s.causal_conv_step(xz[:, :D], cs, P['wc'], P['bc'])
+            dbc = u @ P['wx']
+            y = s.selective_scan_step(u, hs, dbc[:, :D], P['a'], dbc[:, D:D + N], dbc[:, D + N:], P['skip'], xz[:, D:],
+                                      P['dtb'])
+            R.close('token', tok + y @ P['wout'], ref[torch.arange(3), at], 2048)
+
+
+def test_gradients_against_differences():
+    """d/de of <out, dy> along a random direction, from the kernels' own forward at +-e (float32, so e = 2^-6: the
+    difference is off by e^2 of a third derivative of the order of the value and by 2^-24 / e)."""
+    P, _ = _block_params(16, 32, 16)
+    x = torch.randn(2, 20, 16, generator=_gen(31)).cuda().requires_grad_(True)
+    dy = torch.randn(2, 20, 16, generator=_gen(32)).cuda()
+    leaves = dict(P, x=x)
+    grads = _grads([_block(P, x)], [dy], leaves)
+    g = _gen(33)
+    for k, v in leaves.items():
+        way = torch.randn(v.shape, generator=g).cuda()
+        way = way / way.norm()
+        vals = []
+        with torch.no_grad():
+            for e in (2.0 ** -6, -2.0 ** -6):
+                Q = {q: w.detach() + (e * way if q == k else 0) for q, w in leaves.items()}
+                vals.append((_block(Q, Q['x']).double() * dy.double()).sum())
+        slope = float((vals[0] - vals[1]) * 32)
+        want = float((grads[k].double() * way.double()).sum())
+        assert abs(slope - want) <= 2e-3 * max(float(grads[k].double().norm()), 1e-3), k
+
+
+# ---------------------------------------------------------------------------------------------- streams, graphs, devices
+
+def test_same_bits_every_time_and_on_another_stream():
+    P, _ = _block_params(64, 128, 16)
+    x = torch.randn(4, 130, 64, generator=_gen(41)).cuda().requires_grad_(True)
+    lens = torch.tensor([130, 64, 1, 100], dtype=torch.int32, device='cuda')
+    dy = torch.randn(4, 130, 64, generator=_gen(42)).cuda()
+
+    def once():
+        out = _block(P, x, lens)
+        return [out.detach()] + list(_grads([out], [dy], dict(P, x=x)).values())
+    first = once()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = once()
+    torch.cuda.current_stream().wait_stream(side)
+    for u, v in zip(first, second):
+        assert torch.equal(u, v)
+
+
+def test_captured_graphs_replay():
+    """Forward and backward captured (two graphs of different sizes, replayed in turn with eager work between), every
+    replay against the eager result on the inputs of that replay."""
+    s = S()
+
+    def make(B, T, D, N):
+        leaves, dy, _ = _scan_case(B, T, D, N, 1, 'bf16', seed=B)
+        ins = {k: v[0] for k, v in leaves.items()}
+        w = torch.randn(D, 4, generator=_gen(1)).cuda().requires_grad_(True)
+        nw = torch.randn(D, generator=_gen(2)).cuda().requires_grad_(True)
+
+        def step(ins, w, nw, dy):
+            u = s.causal_conv(s.layer_norm(ins['x'], nw), w)
+            y, last = s.selective_scan(u, *(ins[k] for k in SCAN[1:8]), state=ins['state'], return_state=True)
+            return [y, last] + list(torch.autograd.grad(y, [*ins.values(), w, nw], dy))
+        return ins, w, nw, dy.cuda(), step
+
+    graphs = []
+    for shape in ((2, 9, 64, 16), (1, 200, 40, 16)):
+        ins, w, nw, dy, step = make(*shape)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(ins, w, nw, dy)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step(ins, w, nw, dy)
+        graphs.append((graph, ins, w, nw, dy, step, outs))
+    for k in range(3):
+        for graph, ins, w, nw, dy, step, outs in graphs:
+            with torch.no_grad():
+                ins['x'].copy_(torch.randn(ins['x'].shape, generator=_gen(50 + k)))
+                dy.copy_(torch.randn(dy.shape, generator=_gen(60 + k)))
+            graph.replay()
+            fresh = {q: v.detach().clone().requires_grad_(True) for q, v in ins.items()}
+            want = step(fresh, w.detach().clone().requires_grad_(True), nw.detach().clone().requires_grad_(True), dy)
+            torch.cuda.synchronize()
+            for u, v in zip(outs, want):
+                assert torch.equal(u, v)
+
+
+def test_captured_steps_replay():
+    """Serving: one token's two steps captured, the states living outside the graph."""
+    s = S()
+    B, D, N = 4, 64, 16
+    leaves, _, _ = _scan_case(B, 8, D, N, 1, 'bf16', seed=7, carry=False)
+    g = {k: v[0].detach() if v[0] is not None else None for k, v in leaves.items()}
+    w = torch.randn(D, 4, generator=_gen(3)).cuda()
+    tok = {k: torch.zeros_like(g[k][:, 0]) for k in ('x', 'dt', 'b', 'c', 'gate')}
+    cs, hs = torch.zeros(B, 3, D, device='cuda', dtype=torch.bfloat16), torch.zeros(B, D, N, device='cuda')
+
+    def step():
+        u = s.causal_conv_step(tok['x'], cs, w)
+        return s.selective_scan_step(u, hs, tok['dt'], g['a'], tok['b'], tok['c'], g['skip'], tok['gate'], g['dt_bias'])
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    cs.zero_(), hs.zero_()
+    want = s.selective_scan(s.causal_conv(g['x'], w), *(g[k] for k in SCAN[1:8]))
+    for k in range(8):
+        for q in tok:
+            tok[q].copy_(g[q][:, k])
+        graph.replay()
+        torch.cuda.synchronize()
+        R.close('y', out, want[:, k].double().cpu(), 256 + 2.0 ** 17)           # (both sides are rounded to bf16)
+
+
+def test_versions_and_second_derivatives():
+    s = S()
+    x = torch.randn(2, 8, device='cuda')
+    state = torch.zeros(2, 3, 8, device='cuda')
+    w = torch.randn(8, 4, device='cuda', requires_grad=True)
+    y = s.causal_conv(x[:, None], w, state=state)
+    with torch.no_grad():
+        s.causal_conv_step(x, state, w)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
+    z = torch.randn(3, 8, device='cuda', requires_grad=True)
+    (g,) = torch.autograd.grad(s.layer_norm(z).square().sum(), z, create_graph=True)
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        g.sum().backward()
+
+
+def test_refusals():
+    s = S()
+    from vqa_amd._lib import VqaHipError
+    x = torch.zeros(2, 4, 8, device='cuda')
+    w = torch.zeros(8, 4, device='cuda')
+    state = torch.zeros(2, 3, 8, device='cuda')
+    a = -torch.ones(8, 16, device='cuda')
+    b = torch.zeros(2, 4, 16, device='cuda')
+    h = torch.zeros(2, 8, 16, device='cuda')
+    lens = torch.tensor([4, 2], dtype=torch.int32, device='cuda')
+    bad = [
+        lambda: s.layer_norm(x.cpu()), lambda: s.layer_norm(x.double()), lambda: s.layer_norm(x, torch.ones(7, device='cuda')),
+        lambda: s.layer_norm(x, torch.ones(8, device='cuda').bfloat16()), lambda: s.layer_norm(x, torch.ones(8)),
+        lambda: s.layer_norm(torch.zeros(2, 8193, device='cuda')), lambda: s.layer_norm(torch.zeros((), device='cuda')),
+        lambda: s.causal_conv(x[0], w), lambda: s.causal_conv(x, w[:, :1]), lambda: s.causal_conv(x, w[:7]),
+        lambda: s.causal_conv(x, torch.zeros(8, 5, device='cuda')), lambda: s.causal_conv(x, w, activation='relu'),
+        lambda: s.causal_conv(x, w, state=state[:, :2]), lambda: s.causal_conv(x, w, state=state.bfloat16()),
+        lambda: s.causal_conv(x, w, lengths=lens.long()), lambda: s.causal_conv(x, w, lengths=lens.cpu()),
+        lambda: s.causal_conv(x, w, lengths=lens[:1]),
+        lambda: s.causal_conv_step(x, state, w), lambda: s.causal_conv_step(x[:, 0], state[:1].expand(2, 3, 8), w),
+        lambda: s.causal_conv_step(x[:, 0], state[:, :1].expand(2, 3, 8), w),
+        lambda: s.causal_conv_step(x[:, 0], state.transpose(1, 2).contiguous().transpose(1, 2), w),
+        lambda: s.causal_conv_step(x[:, 0], state, w.clone().requires_grad_(True)),
+        lambda: s.selective_scan(x, x[:, :3], a, b, b), lambda: s.selective_scan(x, x.bfloat16(), a, b, b),
+        lambda: s.selective_scan(x, x, a[:, :8], b, b), lambda: s.selective_scan(x, x, a.bfloat16(), b, b),
+        lambda: s.selective_scan(x, x, a, b, b[..., :8]), lambda: s.selective_scan(x, x, a, b[:1], b[:1]),
+        lambda: s.selective_scan(x, x, a, b[:, :, None].expand(2, 4, 3, 16), b[:, :, None].expand(2, 4, 3, 16)),
+        lambda: s.selective_scan(x, x, torch.zeros(8, 65, device='cuda'), *(torch.zeros(2, 4, 65, device='cuda'),) * 2),
+        lambda: s.selective_scan(x, x, a, b, b, gate=x[..., :4]), lambda: s.selective_scan(x, x, a, b, b, state=h[:1]),
+        lambda: s.selective_scan(x, x, a, b, b, lengths=lens.float()),
+        lambda: s.selective_scan_step(x[:, 0], h[:1].expand(2, 8, 16), x[:, 0], a, b[:, 0], b[:, 0]),
+        lambda: s.selective_scan_step(x[:, 0], h.transpose(1, 2).contiguous().transpose(1, 2), x[:, 0], a, b[:, 0], b[:, 0]),
+        lambda: s.selective_scan_step(x[:, 0], h.bfloat16(), x[:, 0], a, b[:, 0], b[:, 0]),
+        lambda: s.selective_scan_step(x[:, 0], h, x[:, 0], a.clone().requires_grad_(True), b[:, 0], b[:, 0]),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(VqaHipError):
+            f()
+            pytest.fail(f'call {i} was not refused')

@@ -1,0 +1,276 @@
+// Layer norm over the last axis, forward and backward.
+//   y = (x - mean) rstd w + b;   with g = dy w and xh = (x - mean) rstd:
+//   dx = rstd (g - mean(g) - xh mean(g xh)),  dw = sum over rows of dy xh,  db = sum over rows of dy
+// Both directions are bound by HBM: a row is read once into registers (E elements per lane of its team of 64, 256 or 512
+// lanes), the mean and then the mean square of the CENTRED values are taken from there - no cancellation between large
+// sums - and the result is written from there.  The backward's workgroups walk over rows and keep their share of dw / db
+// in registers; one partial row per workgroup is written and summed in a fixed order (no atomics: the same bits every
+// time).
+#include "seq.h"
+
+namespace {
+
+// Sums of a and b over the team.  The waves of a larger team meet at ONE barrier: two successive sums use the two halves
+// of sh, and a wave that writes a half again has passed the barrier behind which the other waves had read it.
+template <int TEAM> __device__ __forceinline__ void team_sum2(float& a, float& b, float2 (*sh)[TEAM / 64], int& half) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if constexpr (TEAM > 64) {
+        float2* s = sh[half];
+        half ^= 1;
+        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = make_float2(a, b);
+        __syncthreads();
+        a = b = 0.f;
+#pragma unroll
+        for (int i = 0; i < TEAM / 64; ++i) { a += s[i].x; b += s[i].y; }
+    }
+}
+
+template <typename T, int V, int TEAM, int NV>
+__global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_fwd(const T* __restrict__ x, long ldx,
+                                                                  const float* __restrict__ w,
+                                                                  const float* __restrict__ bias, long rows, int width,
+                                                                  float eps, T* __restrict__ y,
+                                                                  float* __restrict__ mean, float* __restrict__ rstd) {
+    __shared__ float2 sh[2][TEAM / 64];
+    int half = 0;
+    const int lane = threadIdx.x % TEAM;
+    const long row = (long)blockIdx.x * (TEAM == 64 ? 4 : 1) + (TEAM == 64 ? threadIdx.x / 64 : 0);
+    if (row >= rows) return;                               // (whole waves; only where a team is one wave)
+    Raw<T, V> r[NV];
+    float sum = 0.f, zero = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * TEAM + lane) * V;
+        if (c < width) r[i].load(x + row * ldx + c); else r[i].zero();
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) sum += r[i].get(k);
+    team_sum2<TEAM>(sum, zero, sh, half);
+    const float mu = sum / width;
+    float sq = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if ((i * TEAM + lane) * V < width) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) { const float d = r[i].get(k) - mu; sq += d * d; }
+        }
+    team_sum2<TEAM>(sq, zero, sh, half);
+    const float rs = 1.f / sqrtf(sq / width + eps);
+    if (lane == 0 && mean) { mean[row] = mu; rstd[row] = rs; }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * TEAM + lane) * V;
+        if (c < width) {
+            Raw<float, V> wv, bv;
+            if (w) wv.load(w + c);
+            if (bias) bv.load(bias + c);
+            Raw<T, V> o;
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                float v = (r[i].get(k) - mu) * rs;
+                if (w) v *= wv.get(k);
+                if (bias) v += bv.get(k);
+                o.set(k, v);
+            }
+            o.store(y + row * width + c);
+        }
+    }
+}
+
+template <typename T, int V, int TEAM, int NV>
+__global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_bwd(const T* __restrict__ dy, long lddy,
+                                                                  const T* __restrict__ x, long ldx,
+                                                                  const float* __restrict__ w,
+                                                                  const float* __restrict__ mean,
+                                                                  const float* __restrict__ rstd, long rows, int width,
+                                                                  T* __restrict__ dx, float* __restrict__ part) {
+    constexpr int TEAMS = TEAM == 64 ? 4 : 1;
+    __shared__ float2 sh[2][TEAM / 64];
+    int half = 0;
+    const int lane = threadIdx.x % TEAM, team = TEAM == 64 ? threadIdx.x / 64 : 0;
+    float wv[NV][V], aw[NV][V], ab[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = (i * TEAM + lane) * V + k;
+            wv[i][k] = c < width ? (w ? w[c] : 1.f) : 0.f;
+            aw[i][k] = ab[i][k] = 0.f;
+        }
+    const float inv = 1.f / width;
+    const long step = (long)gridDim.x * TEAMS;
+    long row = (long)blockIdx.x * TEAMS + team;
+    Raw<T, V> xr[NV], gr[NV], xn[NV], gn[NV];
+    float mu = 0.f, rs = 0.f, mun = 0.f, rsn = 0.f;
+    auto fetch = [&](long at) {                            // the next row is in flight while this one is worked on
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * TEAM + lane) * V;
+            xn[i].zero();
+            gn[i].zero();
+            if (at < rows && c < width) { xn[i].load(x + at * ldx + c); gn[i].load(dy + at * lddy + c); }
+        }
+        if (at < rows) { mun = mean[at]; rsn = rstd[at]; }
+    };
+    fetch(row);
+    for (; row < rows; row += step) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) { xr[i] = xn[i]; gr[i] = gn[i]; }
+        mu = mun;
+        rs = rsn;
+        fetch(row + step);
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float xh = (xr[i].get(k) - mu) * rs, d = gr[i].get(k), g = d * wv[i][k];
+                s1 += g;
+                s2 += g * xh;
+                aw[i][k] += d * xh;
+                ab[i][k] += d;
+            }
+        team_sum2<TEAM>(s1, s2, sh, half);
+        s1 *= inv;
+        s2 *= inv;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * TEAM + lane) * V;
+            if (c < width) {
+                Raw<T, V> o;
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const float xh = (xr[i].get(k) - mu) * rs;
+                    o.set(k, rs * (gr[i].get(k) * wv[i][k] - s1 - xh * s2));
+                }
+                o.store(dx + row * width + c);
+            }
+        }
+    }
+    // the workgroup's share of dw and db: part[blockIdx][2][width]; the four one-wave teams are joined through LDS
+    float* out = part + (long)blockIdx.x * 2 * width;
+    if constexpr (TEAMS == 1) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const int c = (i * TEAM + lane) * V + k;
+                if (c < width) { out[c] = aw[i][k]; out[width + c] = ab[i][k]; }
+            }
+    } else {
+        constexpr int E = NV * V;
+        __shared__ float acc[2 * E * 64];
+        for (int t = 0; t < TEAMS; ++t) {
+            if (team == t) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int k = 0; k < V; ++k) {
+                        float* a = acc + (i * V + k) * 64 + lane;
+                        a[0] = (t ? a[0] : 0.f) + aw[i][k];
+                        a[E * 64] = (t ? a[E * 64] : 0.f) + ab[i][k];
+                    }
+            }
+            __syncthreads();
+        }
+        for (int j = threadIdx.x; j < 2 * E * 64; j += 256) {
+            const int half = j / (E * 64), e = (j / 64) % E, l = j & 63, c = ((e / V) * 64 + l) * V + e % V;
+            if (c < width) out[half * width + c] = acc[j];
+        }
+    }
+}
+
+// Lanes per row and elements per lane.
+struct Shape { int team, e; };
+Shape shape_of(int width) {
+    if (width <= 512) return {64, 8};
+    if (width <= 1024) return {64, 16};
+    if (width <= 2048) return {64, 32};
+    if (width <= 4096) return {256, 16};
+    return {512, 16};
+}
+constexpr int MAX_WIDTH = 8192;
+
+int bwd_groups(long rows, int width) {
+    const Shape s = shape_of(width);
+    const long per = s.team == 64 ? 4 : 1;
+    long g = (rows + per * 4 - 1) / (per * 4);             // four rows a team, so that the partial rows stay few
+    return (int)(g < 1 ? 1 : g > 512 ? 512 : g);
+}
+
+template <typename T, int V, typename F> int by_shape(int width, F f) {
+    const Shape s = shape_of(width);
+    if (s.team == 64 && s.e == 8) return f.template operator()<T, V, 64, 8 / V>();
+    if (s.team == 64 && s.e == 16) return f.template operator()<T, V, 64, 16 / V>();
+    if (s.team == 64) return f.template operator()<T, V, 64, 32 / V>();
+    if (s.team == 256) return f.template operator()<T, V, 256, 16 / V>();
+    return f.template operator()<T, V, 512, 16 / V>();
+}
+template <typename F> int by_type(int dtype, bool vec, int width, F f) {
+    if (dtype == VQA_F32) return vec ? by_shape<float, 4>(width, f) : by_shape<float, 1>(width, f);
+    if (dtype == VQA_BF16) return vec ? by_shape<bf16, 8>(width, f) : by_shape<bf16, 1>(width, f);
+    return vec ? by_shape<_Float16, 8>(width, f) : by_shape<_Float16, 1>(width, f);
+}
+
+struct Fwd {
+    hipStream_t st; const void* x; long ldx; const float *w, *b; long rows; int width; float eps; void* y; float *mean, *rstd;
+    template <typename T, int V, int TEAM, int NV> int operator()() const {
+        const long grid = TEAM == 64 ? (rows + 3) / 4 : rows;
+        ln_fwd<T, V, TEAM, NV><<<(unsigned)grid, TEAM == 64 ? 256 : TEAM, 0, st>>>(
+            static_cast<const T*>(x), ldx, w, b, rows, width, eps, static_cast<T*>(y), mean, rstd);
+        CHECK_LAUNCH();
+        return VQA_OK;
+    }
+};
+struct Bwd {
+    hipStream_t st; const void* dy; long lddy; const void* x; long ldx; const float *w, *mean, *rstd; long rows; int width;
+    void* dx; float* part;
+    template <typename T, int V, int TEAM, int NV> int operator()() const {
+        ln_bwd<T, V, TEAM, NV><<<bwd_groups(rows, width), TEAM == 64 ? 256 : TEAM, 0, st>>>(
+            static_cast<const T*>(dy), lddy, static_cast<const T*>(x), ldx, w, mean, rstd, rows, width,
+            static_cast<T*>(dx), part);
+        CHECK_LAUNCH();
+        return VQA_OK;
+    }
+};
+
+bool bad_shape(int dtype, long rows, int width) {
+    return !vqa_dtype_ok(dtype) || rows < 1 || rows > 0x7fffffffL || width < 1 || width > MAX_WIDTH;
+}
+bool param_vec(const float* p) { return ((uintptr_t)p & 15) == 0; }      // (NULL is aligned)
+
+}  // namespace
+
+extern "C" int vqa_layer_norm_fwd(void* stream, int dtype, const void* x, long ldx, const float* weight,
+                                  const float* bias, long rows, int width, float eps, void* y, float* mean,
+                                  float* rstd) {
+    if (bad_shape(dtype, rows, width) || !x || !y || (mean == nullptr) != (rstd == nullptr)) return VQA_ERR_ARG;
+    const int e = vqa_elem_bytes(dtype);
+    const bool vec = width % (16 / e) == 0 && vqa_vec_ok(x, ldx, e) && vqa_vec_ok(y, width, e) && param_vec(weight) &&
+                     param_vec(bias);
+    return by_type(dtype, vec, width,
+                   Fwd{static_cast<hipStream_t>(stream), x, ldx, weight, bias, rows, width, eps, y, mean, rstd});
+}
+
+extern "C" int vqa_layer_norm_bwd_part(long rows, int width) {
+    return rows < 1 || width < 1 || width > MAX_WIDTH ? 0 : bwd_groups(rows, width);
+}
+
+extern "C" int vqa_layer_norm_bwd(void* stream, int dtype, const void* dy, long lddy, const void* x, long ldx,
+                                  const float* weight, const float* mean, const float* rstd, long rows, int width,
+                                  void* dx, float* dweight, float* dbias, float* part) {
+    if (bad_shape(dtype, rows, width) || !dy || !x || !mean || !rstd || !dx || !part) return VQA_ERR_ARG;
+    const int e = vqa_elem_bytes(dtype);
+    const bool vec = width % (16 / e) == 0 && vqa_vec_ok(x, ldx, e) && vqa_vec_ok(dy, lddy, e) && vqa_vec_ok(dx, width, e);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const int rc = by_type(dtype, vec, width, Bwd{st, dy, lddy, x, ldx, weight, mean, rstd, rows, width, dx, part});
+    if (rc != VQA_OK) return rc;
+    if (dweight || dbias) {
+        seq_sum_columns(st, part, bwd_groups(rows, width), 2L * width, dweight, width, dbias);
+        CHECK_LAUNCH();
+    }
+    return VQA_OK;
+}

@@ -33,7 +33,7 @@ struct PlanEntry {
 constexpr long PLAN_MAGIC = 0x56514150314cL;      // "VQAP1L"
 enum { K_INT = 0, K_F32 = 1, K_F64 = 2, K_PTR = 3, K_NULL = 4, K_PTRARR = 5, K_INTARR = 6 };
 constexpr long OP_SYNC = -1;                      // [OP_SYNC, waiter stream, 1, K_INT, signalling stream]
-constexpr int MAX_SLOTS = 32, MAX_PTRS = 256, MAX_INTS = 1024;
+constexpr int MAX_SLOTS = 64, MAX_PTRS = 256, MAX_INTS = 1024;
 
 inline void* resolve(long ref, void* const* bases, int n_bases, bool& ok) {
     if (ref == -1) return nullptr;

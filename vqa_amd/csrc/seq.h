@@ -1,0 +1,80 @@
+// Device helpers of the sequence operators (layer_norm.hip, causal_conv.hip, scan.hip): rows of float, bf16 or f16
+// elements are moved V at a time (16 bytes where base, strides and width allow it, else one element), the arithmetic is
+// f32, and each result is rounded once, to nearest even, when it is stored.
+#pragma once
+#include "common.h"
+
+template <> __device__ __forceinline__ _Float16 from_f32<_Float16>(float x) { return (_Float16)x; }
+
+template <typename T, int V> struct RowVec { typedef T type __attribute__((ext_vector_type(V))); };
+template <typename T> struct RowVec<T, 1> { typedef T type; };
+
+// V consecutive elements as they lie in memory (p is aligned to V * sizeof(T))
+template <typename T, int V> struct Raw {
+    typename RowVec<T, V>::type v;
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const typename RowVec<T, V>::type*>(p); }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (V == 1) return to_f32(v); else return to_f32((T)v[i]);
+    }
+    __device__ __forceinline__ void zero() {
+        if constexpr (V == 1) v = from_f32<T>(0.f);
+        else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = from_f32<T>(0.f);
+        }
+    }
+    __device__ __forceinline__ void set(int i, float x) {
+        if constexpr (V == 1) v = from_f32<T>(x); else v[i] = from_f32<T>(x);
+    }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<typename RowVec<T, V>::type*>(p) = v; }
+};
+
+// exp through the hardware's base-2 exponential (1 ulp; results under 2^-126 become 0)
+__device__ __forceinline__ float exp_f(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+__device__ __forceinline__ float sigmoid_f(float x) { return __builtin_amdgcn_rcpf(1.f + exp_f(-x)); }
+// x * sigmoid(x): exp(-x) may overflow to infinity, whose reciprocal is the 0 that is meant
+__device__ __forceinline__ float silu_f(float x) { return x * sigmoid_f(x); }
+__device__ __forceinline__ float dsilu_f(float x) {
+    const float s = sigmoid_f(x);
+    return s * (1.f + x * (1.f - s));
+}
+
+static inline int vqa_elem_bytes(int dtype) { return dtype == VQA_F32 ? 4 : 2; }
+static inline bool vqa_dtype_ok(int dtype) { return dtype == VQA_F32 || dtype == VQA_BF16 || dtype == VQA_F16; }
+// a pointer whose rows start `stride` elements apart can be read 16 bytes at a time
+static inline bool vqa_vec_ok(const void* p, long stride, int elem) {
+    return ((uintptr_t)p & 15) == 0 && (stride * elem) % 16 == 0;
+}
+
+// Column sums of part[rows][cols] (f32) in a fixed order: 64 columns x 16 row lanes per workgroup, eight rows of each lane
+// in flight, the lanes joined through LDS.  Column c of the first `n0` goes to out0[c], the rest to out1[c - n0].
+__global__ __launch_bounds__(1024) static void seq_column_sums(const float* __restrict__ part, int rows, long cols,
+                                                               float* __restrict__ out0, long n0,
+                                                               float* __restrict__ out1) {
+    const long c = (long)blockIdx.x * 64 + (threadIdx.x & 63);
+    const int lane_row = threadIdx.x >> 6;
+    float acc[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) acc[u] = 0.f;
+    if (c < cols) {
+        for (int r = lane_row; r < rows; r += 128) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (r + 16 * u < rows) acc[u] += part[(long)(r + 16 * u) * cols + c];
+        }
+    }
+    __shared__ float s[16][64];
+    s[lane_row][threadIdx.x & 63] = ((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7]));
+    __syncthreads();
+    if (lane_row == 0 && c < cols) {
+        float t = 0.f;
+#pragma unroll
+        for (int u = 0; u < 16; ++u) t += s[u][threadIdx.x];
+        if (c < n0) { if (out0) out0[c] = t; }
+        else if (out1) out1[c - n0] = t;
+    }
+}
+static inline void seq_sum_columns(hipStream_t st, const float* part, int rows, long cols, float* out0, long n0,
+                                   float* out1) {
+    seq_column_sums<<<(unsigned)((cols + 63) / 64), 1024, 0, st>>>(part, rows, cols, out0, n0, out1);
+}

@@ -1,0 +1,424 @@
+"""Sequence operators beside the GRU and BatchNorm, HIP-backed: layer norm over the last axis, the short causal convolution
+and the selective state space scan over tokens - whole sequences with their gradients, and one token at a time against a
+state that the caller keeps.
+
+    h = layer_norm(x, w, b)                                          # [..., C]
+    u, conv_state = causal_conv(h, wc, bc, return_state=True)        # [B, L, D]
+    y, state = selective_scan(u, dt, a, b, c, skip, gate, dt_bias, return_state=True)
+    ... the next token:  u = causal_conv_step(h1, conv_state, wc, bc);  y = selective_scan_step(u, state, dt1, a, b1, c1, ...)
+
+Rows (x, dt, b, c, gate, the convolution's state) are float32, bfloat16 or float16, all of one type; parameters (weight,
+bias, a, skip, dt_bias) and the scan's state are float32, as are all sums.  The last axis of a row must be contiguous (it
+is copied otherwise), the other axes may have any stride.  `lengths` (int32 [B], on the GPU) marks a padded batch: tokens at
+or past lengths[b] give zero rows and zero gradients, take no part in any sum or state, and may hold anything; values are
+taken between 0 and L.  `state` continues a sequence and `return_state` returns what its continuation needs; gradients pass
+through both.  Everything runs on torch's current stream of the tensors' device; workspaces are torch allocations of the
+call, so captured graphs share nothing.  A backward that is to be captured into a graph needs leaves that no live eager
+graph uses (torch ties a leaf's gradient accumulation to the stream of its first use); the *_step functions are forward
+only.  Errors of use raise VqaHipError (a RuntimeError) before anything is launched.
+"""
+import ctypes
+from functools import lru_cache
+
+import torch
+from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
+
+from . import _lib as L
+
+_ROW_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class _device_of:
+    """Makes x's device the current one for the call where it is not (the kernels go to the current device's stream)."""
+
+    def __init__(self, x):
+        self.want, self.had = x.device.index, None
+
+    def __enter__(self):
+        if torch._C._cuda_getDevice() != self.want:
+            self.had = torch._C._cuda_getDevice()
+            torch._C._cuda_setDevice(self.want)
+
+    def __exit__(self, *exc):
+        if self.had is not None:
+            torch._C._cuda_setDevice(self.had)
+
+
+def _fail(what):
+    raise L.VqaHipError(what)
+
+
+def _rows(name, x, shape=None, like=None):
+    """A row tensor: on the GPU, of a row type, of `like`'s type and device, of this shape."""
+    if not x.is_cuda:
+        _fail(f'{name} must be on the GPU (there is no CPU fallback)')
+    if like is None:
+        if x.dtype not in _ROW_TYPES:
+            _fail(f'{name} must be float32, bfloat16 or float16, not {x.dtype}')
+    elif x.dtype != like.dtype or x.device != like.device:
+        _fail(f'{name} is {x.dtype} on {x.device}: {like.dtype} on {like.device} is wanted')
+    if shape is not None and x.shape != shape:
+        _fail(f'{name} has shape {tuple(x.shape)}: {tuple(shape)} is wanted')
+
+
+def _param(name, p, shape, x):
+    """A float32 parameter or state of this shape on x's device, contiguous; None stays None."""
+    if p is None:
+        return None
+    if p.dtype != torch.float32 or p.device != x.device:
+        _fail(f'{name} is {p.dtype} on {p.device}: float32 on {x.device} is wanted')
+    if p.shape != shape:
+        _fail(f'{name} has shape {tuple(p.shape)}: {tuple(shape)} is wanted')
+    return p if p.is_contiguous() else p.contiguous()
+
+
+def _lengths(lengths, x):
+    if lengths is None:
+        return None
+    if lengths.dtype != torch.int32 or lengths.device != x.device or lengths.shape != x.shape[:1]:
+        _fail(f'lengths must be int32 [{x.shape[0]}] on {x.device}')
+    return lengths.contiguous()
+
+
+def _unit(x):
+    """x with a contiguous last axis"""
+    return x if x.stride(-1) == 1 else x.contiguous()
+
+
+def _tracked(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _no_tracking(what, *tensors):
+    if _tracked(*tensors):
+        _fail(f'{what} has no gradient: call it under torch.no_grad()')
+
+
+# ---------------------------------------------------------------------------------------------------------- layer norm
+
+def _as_matrix(x):
+    """[..., C] -> [rows, C] with a contiguous last axis and one row stride; a view where the strides allow it"""
+    return _unit(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
+
+
+def _norm_fwd(x2, weight, bias, eps, shape, stats):
+    rows, width = x2.shape
+    y = torch.empty(shape, device=x2.device, dtype=x2.dtype)
+    st = torch.empty(2, rows, device=x2.device, dtype=torch.float32) if stats else None
+    if rows:
+        L.call('vqa_layer_norm_fwd', L.dt(x2), x2, x2.stride(0), weight, bias, rows, width, eps, y,
+               st[0] if stats else None, st[1] if stats else None)
+    return y, st
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        x2 = _as_matrix(x)
+        with _device_of(x):
+            y, st = _norm_fwd(x2, weight, bias, eps, x.shape, True)
+        ctx.save_for_backward(x, weight, st)
+        ctx.has_bias = bias is not None
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, st = ctx.saved_tensors
+        x2, dy2 = _as_matrix(x), _as_matrix(dy)
+        rows, width = x2.shape
+        dev = x.device
+        with _device_of(x):
+            dx = torch.empty(x.shape, device=dev, dtype=x.dtype)
+            dw = torch.empty(width, device=dev, dtype=torch.float32) if weight is not None else None
+            db = torch.empty(width, device=dev, dtype=torch.float32) if ctx.has_bias else None
+            if rows:
+                part = torch.empty(L.lib().vqa_layer_norm_bwd_part(rows, width), 2, width, device=dev,
+                                   dtype=torch.float32)
+                L.call('vqa_layer_norm_bwd', L.dt(x), dy2, dy2.stride(0), x2, x2.stride(0), weight, st[0], st[1], rows,
+                       width, dx, dw, db, part)
+            else:
+                for g in (dw, db):
+                    if g is not None:
+                        g.zero_()
+        return dx, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis (biased variance), statistics in float32.
+    x [..., C] with C <= 8192; weight, bias float32 [C] or None."""
+    _rows('x', x)
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 8192:
+        _fail(f'x has shape {tuple(x.shape)}: a last axis of 1 to 8192 is wanted')
+    weight, bias = _param('weight', weight, x.shape[-1:], x), _param('bias', bias, x.shape[-1:], x)
+    if _tracked(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, eps)
+    with _device_of(x):
+        return _norm_fwd(_as_matrix(x), weight, bias, eps, x.shape, False)[0]
+
+
+# --------------------------------------------------------------------------------------------------- causal convolution
+
+def _silu_flag(activation):
+    if activation not in (None, 'silu'):
+        _fail(f"activation is {activation!r}: 'silu' or None is wanted")
+    return int(activation == 'silu')
+
+
+def _taps(weight, D):
+    if weight.dim() != 2 or weight.shape[0] != D or not 2 <= weight.shape[1] <= 4:
+        _fail(f'weight has shape {tuple(weight.shape)}: [{D}, 2 to 4] is wanted')
+    return weight.shape[1]
+
+
+def _conv_fwd(x, weight, bias, silu, state, lengths, want_last):
+    B, T, D = x.shape
+    taps = weight.shape[1]
+    y = torch.empty(B, T, D, device=x.device, dtype=x.dtype)
+    last = torch.empty(B, taps - 1, D, device=x.device, dtype=x.dtype) if want_last else None
+    if y.numel():
+        L.call('vqa_causal_conv_fwd', L.dt(x), x, x.stride(0), x.stride(1), weight, bias, state, lengths, B, T, D, taps,
+               silu, y, last)
+    elif want_last and last.numel():
+        last.zero_() if state is None else last.copy_(state)
+    return y, last
+
+
+class _CausalConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, silu, state, lengths, want_last):
+        with _device_of(x):
+            y, last = _conv_fwd(x, weight, bias, silu, state, lengths, want_last)
+        ctx.save_for_backward(x, weight, bias, state, lengths)
+        ctx.silu = silu
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dlast):
+        x, weight, bias, state, lengths = ctx.saved_tensors
+        B, T, D = x.shape
+        taps, dev = weight.shape[1], x.device
+        with _device_of(x):
+            dy = torch.zeros(B, T, D, device=dev, dtype=x.dtype) if dy is None else _unit(dy)
+            dlast = None if dlast is None else dlast.contiguous()
+            dx = torch.empty(B, T, D, device=dev, dtype=x.dtype)
+            dw = torch.empty(D, taps, device=dev, dtype=torch.float32)
+            db = torch.empty(D, device=dev, dtype=torch.float32) if bias is not None else None
+            dstate = torch.empty(B, taps - 1, D, device=dev, dtype=x.dtype) if state is not None else None
+            if dx.numel():
+                part = torch.empty(L.lib().vqa_causal_conv_bwd_part(B, T, D), taps + 1, D, device=dev,
+                                   dtype=torch.float32)
+                L.call('vqa_causal_conv_bwd', L.dt(x), dy, dy.stride(0), dy.stride(1), dlast, x, x.stride(0),
+                       x.stride(1), weight, bias, state, lengths, B, T, D, taps, ctx.silu, dx, dw, db, dstate, part)
+            else:
+                dw.zero_()
+                if db is not None:
+                    db.zero_()
+                if dstate is not None:
+                    dstate.zero_() if dlast is None else dstate.copy_(dlast)
+        return dx, dw, db, None, dstate, None, None
+
+
+def causal_conv(x, weight, bias=None, activation='silu', state=None, lengths=None, return_state=False):
+    """One filter of 2 to 4 taps per channel over the tokens of x [B, L, D], each token seeing itself and those before it:
+    y_t = act(bias + sum_k weight[:, k] x_{t - taps + 1 + k}), act = silu or (activation=None) nothing; weight float32
+    [D, taps], bias float32 [D].  state [B, taps - 1, D] (x's type): the rows before the first (None: zeros).  Returns y,
+    or with return_state (y, state after each sequence's last token)."""
+    _rows('x', x)
+    if x.dim() != 3:
+        _fail(f'x has shape {tuple(x.shape)}: [B, L, D] is wanted')
+    B, T, D = x.shape
+    taps = _taps(weight, D)
+    weight, bias = _param('weight', weight, (D, taps), x), _param('bias', bias, (D,), x)
+    silu = _silu_flag(activation)
+    if state is not None:
+        _rows('state', state, (B, taps - 1, D), x)
+        state = state.contiguous()
+    lengths = _lengths(lengths, x)
+    x = _unit(x)
+    if _tracked(x, weight, bias, state):
+        y, last = _CausalConv.apply(x, weight, bias, silu, state, lengths, return_state)
+    else:
+        with _device_of(x):
+            y, last = _conv_fwd(x, weight, bias, silu, state, lengths, return_state)
+    return (y, last) if return_state else y
+
+
+def causal_conv_step(x, state, weight, bias=None, activation='silu'):
+    """causal_conv for ONE new token per sequence: x [B, D]; state [B, taps - 1, D] (x's type; rows may be strided) is
+    shifted in place.  Returns y [B, D].  Forward only."""
+    _rows('x', x)
+    if x.dim() != 2:
+        _fail(f'x has shape {tuple(x.shape)}: [B, D] is wanted')
+    B, D = x.shape
+    taps = _taps(weight, D)
+    weight, bias = _param('weight', weight, (D, taps), x), _param('bias', bias, (D,), x)
+    silu = _silu_flag(activation)
+    _rows('state', state, (B, taps - 1, D), x)
+    _no_tracking('causal_conv_step', x, state, weight, bias)
+    y = torch.empty(B, D, device=x.device, dtype=x.dtype)
+    if not y.numel():
+        return y
+    s0, s1, s2 = state.stride()
+    if (s2 != 1 and D > 1) or not (s1 >= D or taps == 2) or not (
+            B == 1 or s0 >= (taps - 2) * s1 + D or (s0 >= D and s1 >= (B - 1) * s0 + D)):
+        _fail(f'state has strides {state.stride()}: it is updated in place, so rows must be contiguous and apart')
+    x = _unit(x)
+    with _device_of(x):
+        L.call('vqa_causal_conv_token', L.dt(x), x, x.stride(0), state, s0, s1, weight, bias, B, D, taps, silu, y)
+    increment_version(state)
+    return y
+
+
+# ------------------------------------------------------------------------------------------------- selective state space
+
+@lru_cache(maxsize=1024)
+def _scan_bytes(dtype, B, T, D, N, G):
+    sizes = (ctypes.c_long * 3)()
+    if L.lib().vqa_scan_ws_bytes(dtype, B, T, D, N, G, ctypes.addressof(sizes)) != 0:
+        _fail(f'selective_scan: batch {B}, length {T}, width {D}, {N} states in {G} groups is out of range')
+    return tuple(sizes)
+
+
+def _floats(nbytes, dev):
+    return torch.empty(nbytes // 4, device=dev, dtype=torch.float32) if nbytes else None
+
+
+def _strides(x, tokens):
+    """the leading strides of a row tensor, zeros for None"""
+    return (0, 0) if x is None else (x.stride(0), x.stride(1)) if tokens else (x.stride(0),)
+
+
+def _scan_fwd(x, dt, a, b, c, skip, gate, dt_bias, softplus, state, lengths, want_last, want_keep):
+    B, T, D = x.shape
+    G, N, dev, code = b.shape[2], b.shape[3], x.device, L.dt(x)
+    y = torch.empty(B, T, D, device=dev, dtype=x.dtype)
+    last = torch.empty(B, D, N, device=dev, dtype=torch.float32) if want_last else None
+    if not y.numel():
+        if want_last and last.numel():
+            last.zero_() if state is None else last.copy_(state)
+        return y, last, None
+    fwd, keep_bytes, _ = _scan_bytes(code, B, T, D, N, G)
+    ws = _floats(fwd, dev)
+    keep = _floats(keep_bytes, dev) if want_keep else None
+    L.call('vqa_scan_fwd', code, x, x.stride(0), x.stride(1), dt, dt.stride(0), dt.stride(1), gate,
+           *_strides(gate, True), a, b, b.stride(0), b.stride(1), c, c.stride(0), c.stride(1), skip, dt_bias, softplus,
+           state, lengths, B, T, D, N, G, y, last, keep, ws)
+    return y, last, keep
+
+
+class _SelectiveScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, dt, a, b, c, skip, gate, dt_bias, softplus, state, lengths, want_last):
+        with _device_of(x):
+            y, last, keep = _scan_fwd(x, dt, a, b, c, skip, gate, dt_bias, softplus, state, lengths, want_last, True)
+        ctx.save_for_backward(x, dt, a, b, c, skip, gate, dt_bias, lengths, keep)
+        ctx.softplus, ctx.has_state = softplus, state is not None
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dlast):
+        x, dt, a, b, c, skip, gate, dt_bias, lengths, keep = ctx.saved_tensors
+        B, T, D = x.shape
+        G, N, dev, code = b.shape[2], b.shape[3], x.device, L.dt(x)
+        f32 = lambda *s: torch.empty(*s, device=dev, dtype=torch.float32)       # noqa: E731
+        rows = lambda *s: torch.empty(*s, device=dev, dtype=x.dtype)            # noqa: E731
+        with _device_of(x):
+            dlast = None if dlast is None else dlast.contiguous()
+            dx, ddt, dgate = rows(B, T, D), rows(B, T, D), rows(B, T, D) if gate is not None else None
+            db, dc, da = rows(B, T, G, N), rows(B, T, G, N), f32(D, N)
+            dskip, dbias = f32(D) if skip is not None else None, f32(D) if dt_bias is not None else None
+            dstate = f32(B, D, N) if ctx.has_state else None
+            if not dx.numel():
+                for g in (da, dskip, dbias):
+                    if g is not None:
+                        g.zero_()
+                if dstate is not None:
+                    dstate.zero_() if dlast is None else dstate.copy_(dlast)
+            else:
+                dy = torch.zeros(B, T, D, device=dev, dtype=x.dtype) if dy is None else _unit(dy)
+                ws = _floats(_scan_bytes(code, B, T, D, N, G)[2], dev)
+                L.call('vqa_scan_bwd', code, dy, dy.stride(0), dy.stride(1), dlast, x, x.stride(0), x.stride(1), dt,
+                       dt.stride(0), dt.stride(1), gate, *_strides(gate, True), a, b, b.stride(0), b.stride(1), c,
+                       c.stride(0), c.stride(1), skip, dt_bias, ctx.softplus, lengths, B, T, D, N, G, keep, dx, ddt,
+                       dgate, da, db, dc, dskip, dbias, dstate, ws)
+        return dx, ddt, da, db, dc, dskip, dgate, dbias, None, dstate, None, None
+
+
+def _shared(name, b, lead, x):
+    """b or c as [*lead, G, N] with contiguous groups"""
+    _rows(name, b, None, x)
+    k = len(lead)
+    if b.dim() not in (k + 1, k + 2) or b.shape[:k] != lead:
+        _fail(f'{name} has shape {tuple(b.shape)}: [{", ".join(map(str, lead))}, N] or [.., G, N] is wanted')
+    if b.dim() == k + 1:
+        b = b.unsqueeze(k)
+    G, N = b.shape[k:]
+    return b if b.stride(-1) == 1 and (G == 1 or b.stride(-2) == N) else b.contiguous()
+
+
+def _scan_args(x, dt, a, b, c, skip, gate, dt_bias):
+    lead, D = x.shape[:-1], x.shape[-1]
+    _rows('dt', dt, x.shape, x)
+    if gate is not None:
+        _rows('gate', gate, x.shape, x)
+        gate = _unit(gate)
+    b, c = _shared('b', b, lead, x), _shared('c', c, lead, x)
+    G, N = b.shape[-2:]
+    if c.shape != b.shape:
+        _fail(f'b and c have shapes {tuple(b.shape)} and {tuple(c.shape)}: the same is wanted')
+    if not 1 <= N <= 64 or G < 1 or D % G:
+        _fail(f'{N} states in {G} groups over {D} channels: 1 to 64 states and a whole number of channels a group')
+    return (_unit(x), _unit(dt), _param('a', a, (D, N), x), b, c, _param('skip', skip, (D,), x), gate,
+            _param('dt_bias', dt_bias, (D,), x))
+
+
+def selective_scan(x, dt, a, b, c, skip=None, gate=None, dt_bias=None, softplus=True, state=None, lengths=None,
+                   return_state=False):
+    """The selective state space recurrence over x [B, L, D], token by token, per channel and its N <= 64 states:
+        dt_t = softplus(dt_t + dt_bias)                   (softplus=False: dt_t + dt_bias)
+        h_t = exp(dt_t a) h_{t-1} + (dt_t x_t) b_t,       y_t = (sum_n c_t h_t + skip x_t) * silu(gate_t)
+    dt, gate [B, L, D]; b, c [B, L, N], or [B, L, G, N] where each of G groups of D / G channels has its own; a float32
+    [D, N]; skip, dt_bias float32 [D]; state float32 [B, D, N] (None: zeros).  gate, skip, dt_bias may be None.
+    Returns y, or with return_state (y, state after each sequence's last token)."""
+    _rows('x', x)
+    if x.dim() != 3:
+        _fail(f'x has shape {tuple(x.shape)}: [B, L, D] is wanted')
+    args = x, dt, a, b, c, skip, gate, dt_bias = _scan_args(x, dt, a, b, c, skip, gate, dt_bias)
+    state = _param('state', state, (x.shape[0], *a.shape), x)
+    lengths = _lengths(lengths, x)
+    if _tracked(*args, state):
+        y, last = _SelectiveScan.apply(*args, int(softplus), state, lengths, return_state)
+    else:
+        with _device_of(x):
+            y, last, _ = _scan_fwd(*args, int(softplus), state, lengths, return_state, False)
+    return (y, last) if return_state else y
+
+
+def selective_scan_step(x, state, dt, a, b, c, skip=None, gate=None, dt_bias=None, softplus=True):
+    """selective_scan for ONE new token per sequence: x, dt, gate [B, D]; b, c [B, N] or [B, G, N]; state float32
+    [B, D, N] is updated in place (its batch axis may be strided).  Returns y [B, D].  Forward only."""
+    _rows('x', x)
+    if x.dim() != 2:
+        _fail(f'x has shape {tuple(x.shape)}: [B, D] is wanted')
+    x, dt, a, b, c, skip, gate, dt_bias = _scan_args(x, dt, a, b, c, skip, gate, dt_bias)
+    B, D = x.shape
+    G, N = b.shape[1:]
+    if state.dtype != torch.float32 or state.device != x.device or state.shape != (B, D, N):
+        _fail(f'state is {state.dtype} {tuple(state.shape)} on {state.device}: float32 {(B, D, N)} on {x.device} is wanted')
+    _no_tracking('selective_scan_step', x, state, dt, a, b, c, skip, gate, dt_bias)
+    y = torch.empty(B, D, device=x.device, dtype=x.dtype)
+    if not y.numel():
+        return y
+    if (state.stride(2) != 1 and N > 1) or (state.stride(1) != N and D > 1) or (B > 1 and state.stride(0) < D * N):
+        _fail(f'state has strides {state.stride()}: it is updated in place, so [D, N] must be contiguous and apart')
+    with _device_of(x):
+        L.call('vqa_scan_token', L.dt(x), x, x.stride(0), state, state.stride(0), dt, dt.stride(0), gate,
+               *_strides(gate, False)[:1], a, b, b.stride(0), c, c.stride(0), skip, dt_bias, int(softplus), B, D, N, G, y)
+    increment_version(state)
+    return y
