@@ -107,31 +107,34 @@ template <typename T, int CH, int NS, int VE> struct Wave {
     // staging: vector k of this lane is token trow(k) of the tile, channels c0 + tcol(k) ...
     __device__ __forceinline__ int trow(int k) const { return (k * 64 + lane) / (WC / VE); }
     __device__ __forceinline__ int tcol(int k) const { return (k * 64 + lane) % (WC / VE) * VE; }
-    __device__ __forceinline__ void fetch(const Rows& R, int b, int t0, int len, Raw<T, VE> (&v)[NV]) const {
-        const T* base = static_cast<const T*>(R.p) + b * R.batch;
+    // (a tile's base is uniform; 8 rows of any tensor span less than 2^31 bytes: the host sees to it)
+    __device__ __forceinline__ unsigned place(int k, int row, int t0, int te) const {
+        return t0 + trow(k) < te && c0 + tcol(k) < cend ? (trow(k) * row + tcol(k)) * (unsigned)sizeof(T) : BUF_OUT;
+    }
+    __device__ __forceinline__ bool staged(int k, int v, int t0, int te) const {
+        return t0 + trow(k) < te && c0 + tcol(k) + v < cend;
+    }
+    __device__ __forceinline__ void fetch(const Rows& R, int b, int t0, int te, Raw<T, VE> (&v)[NV]) const {
+        const auto rs = buffer_of(static_cast<const T*>(R.p) + b * R.batch + t0 * R.row + c0, BUF_BYTES);
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int t = t0 + trow(k), c = c0 + tcol(k);
-            v[k].zero();
-            if (t < len && c < cend) v[k].load(base + t * R.row + c);
-        }
+        for (int k = 0; k < NV; ++k) v[k] = buf_load<T, VE>(rs, place(k, (int)R.row, t0, te));
     }
     __device__ __forceinline__ void put(void* p, int b, int L, int D, int t0, int te, const Raw<T, VE> (&v)[NV]) const {
-        T* base = static_cast<T*>(p) + (long)b * L * D;
+        const auto rs = buffer_of(static_cast<T*>(p) + ((long)b * L + t0) * D + c0, BUF_BYTES);
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int t = t0 + trow(k), c = c0 + tcol(k);
-            if (t < te && c < cend) v[k].store(base + (long)t * D + c);
-        }
+        for (int k = 0; k < NV; ++k) buf_store<T, VE>(rs, place(k, D, t0, te), v[k]);
     }
-    __device__ __forceinline__ void fetch_bc(const Rows& R, int b, int t0, int len, int N, T (&v)[NBC]) const {
-        const T* base = static_cast<const T*>(R.p) + b * R.batch + (long)g * N;
+    __device__ __forceinline__ void fetch_bc(const Rows& R, int b, int t0, int te, int N, Raw<T, 1> (&v)[NBC]) const {
+        const auto rs = buffer_of(static_cast<const T*>(R.p) + b * R.batch + t0 * R.row + (long)g * N, BUF_BYTES);
 #pragma unroll
         for (int k = 0; k < NBC; ++k) {
-            const int t = t0 + (k * 64 + lane) / NP, n = (k * 64 + lane) % NP;
-            v[k] = from_f32<T>(0.f);
-            if (t < len && n < N) v[k] = base[t * R.row + n];
+            const int t = (k * 64 + lane) / NP, n = (k * 64 + lane) % NP;
+            v[k] = buf_load<T, 1>(rs, t0 + t < te && n < N ? (t * (int)R.row + n) * (unsigned)sizeof(T) : BUF_OUT);
         }
+    }
+    // per-channel parameters of the staged channels, in LDS for the whole run
+    __device__ __forceinline__ void stage_param(const float* p, float* s) const {
+        if (lane < WC) s[lane] = p && c0 + lane < cend ? p[c0 + lane] : 0.f;
     }
     __device__ __forceinline__ void lane_a(const Args& A, float (&a2)[CH][NS]) const {
 #pragma unroll
@@ -182,9 +185,39 @@ template <typename T, int CH, int NS, int VE> struct Wave {
 __device__ __forceinline__ int length_of(const Args& A, int b) {
     return A.lengths ? max(0, min(A.L, A.lengths[b])) : A.L;
 }
-__device__ __forceinline__ float step_of(const Args& A, float raw, int c) {
-    const float v = raw + (A.dt_bias ? A.dt_bias[c] : 0.f);
-    return A.softplus ? softplus_f(v) : v;
+// dt of staged raw values; 0 past the end (a token that moves no state) and past the channels
+template <typename W, typename R, int NV, int VE>
+__device__ __forceinline__ void stage_steps(const W& w, const R (&d)[NV], const float* s_bias, int softplus, int t0, int te,
+                                            float (&dt)[NV][VE]) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int v = 0; v < VE; ++v) dt[k][v] = d[k].get(v) + s_bias[w.tcol(k) + v];
+    if (softplus) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int v = 0; v < VE; ++v) dt[k][v] = softplus_f(dt[k][v]);
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int v = 0; v < VE; ++v)
+            if (t0 + w.trow(k) >= te || w.c0 + w.tcol(k) + v >= w.cend) dt[k][v] = 0.f;
+}
+// dy silu(gate)
+template <typename W, typename R, int NV, int VE>
+__device__ __forceinline__ void stage_core(const R (&gy)[NV], const R (&z)[NV], bool gated, float (&dc)[NV][VE]) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int v = 0; v < VE; ++v) dc[k][v] = gy[k].get(v);
+    if (gated) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int v = 0; v < VE; ++v) dc[k][v] *= silu_f(z[k].get(v));
+    }
 }
 
 // FULL: the forward.  Otherwise the first pass over a segment: its end state from 0, and sum dt.
@@ -192,7 +225,7 @@ template <typename T, int CH, int NS, int VE, bool FULL>
 __global__ __launch_bounds__(64) void scan_fwd(Args A) {
     typedef Wave<T, CH, NS, VE> W;
     __shared__ __attribute__((aligned(16))) float s_dt[TT * W::WC], s_dtx[TT * W::WC], s_y[FULL ? TT * W::WC : 4],
-        s_b[TT * W::NP], s_c[FULL ? TT * W::NP : 4];
+        s_b[TT * W::NP], s_c[FULL ? TT * W::NP : 4], s_bias[W::WC], s_skip[FULL ? W::WC : 4];
     const int blks = A.nblk * A.G;
     const int blk = blockIdx.x % blks, seg = blockIdx.x / blks % A.segs, b = blockIdx.x / blks / A.segs;
     const W w(A, blk);
@@ -201,6 +234,8 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
     const int ntile = (A.L + TT - 1) / TT;
     float a2[CH][NS], h[CH][NS], sum_dt[CH];
     w.lane_a(A, a2);
+    w.stage_param(A.dt_bias, s_bias);
+    if (FULL) w.stage_param(A.skip, s_skip);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         sum_dt[i] = 0.f;
@@ -212,7 +247,7 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
         else w.load_state(A.state, b, A.D, A.N, h);
     }
     Raw<T, VE> x[W::NV], d[W::NV], z[W::NV], xn[W::NV], dn[W::NV], zn[W::NV];
-    T bn[W::NBC], cn[W::NBC];
+    Raw<T, 1> bn[W::NBC], cn[W::NBC];
     auto fetch = [&](int t0) {
         w.fetch(A.x, b, t0, min(len, te), xn);
         w.fetch(A.dt, b, t0, min(len, te), dn);
@@ -234,20 +269,20 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
 #pragma unroll
         for (int k = 0; k < W::NV; ++k) { x[k] = xn[k]; d[k] = dn[k]; if (FULL) z[k] = zn[k]; }
         lds_order();                                       // (the last tile's reads are done)
+        float step[W::NV][VE];
+        stage_steps(w, d, s_bias, A.softplus, t0, min(len, te), step);
 #pragma unroll
-        for (int k = 0; k < W::NV; ++k) {
-            const int at = w.trow(k) * W::WC + w.tcol(k), c = w.c0 + w.tcol(k);
+        for (int k = 0; k < W::NV; ++k)
 #pragma unroll
             for (int v = 0; v < VE; ++v) {
-                const float dt = t0 + w.trow(k) < len && c + v < w.cend ? step_of(A, d[k].get(v), c + v) : 0.f;
-                s_dt[at + v] = dt;
-                s_dtx[at + v] = dt * x[k].get(v);
+                const int at = w.trow(k) * W::WC + w.tcol(k) + v;
+                s_dt[at] = step[k][v];
+                s_dtx[at] = step[k][v] * x[k].get(v);
             }
-        }
 #pragma unroll
         for (int k = 0; k < W::NBC; ++k) {
-            s_b[k * 64 + w.lane] = to_f32(bn[k]);
-            if (FULL) s_c[k * 64 + w.lane] = to_f32(cn[k]);
+            s_b[k * 64 + w.lane] = bn[k].get(0);
+            if (FULL) s_c[k * 64 + w.lane] = cn[k].get(0);
         }
         lds_order();
         if (t0 + TT < te) fetch(t0 + TT);
@@ -275,16 +310,22 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
             lds_order();
 #pragma unroll
             for (int k = 0; k < W::NV; ++k) {
-                const int at = w.trow(k) * W::WC + w.tcol(k), c = w.c0 + w.tcol(k);
-                const bool live = t0 + w.trow(k) < len;
+                const int at = w.trow(k) * W::WC + w.tcol(k);
 #pragma unroll
                 for (int v = 0; v < VE; ++v) {
-                    float y = s_y[at + v];
-                    if (A.skip && c + v < w.cend) y += A.skip[c + v] * x[k].get(v);
-                    if (A.gate.p) y *= silu_f(z[k].get(v));
-                    d[k].set(v, live ? y : 0.f);
+                    step[k][v] = s_y[at + v] + s_skip[w.tcol(k) + v] * x[k].get(v);
                 }
             }
+            if (A.gate.p) {
+#pragma unroll
+                for (int k = 0; k < W::NV; ++k)
+#pragma unroll
+                    for (int v = 0; v < VE; ++v) step[k][v] *= silu_f(z[k].get(v));
+            }
+#pragma unroll
+            for (int k = 0; k < W::NV; ++k)
+#pragma unroll
+                for (int v = 0; v < VE; ++v) d[k].set(v, t0 + w.trow(k) < len ? step[k][v] : 0.f);
             w.put(A.y, b, A.L, A.D, t0, te, d);
         }
     }
@@ -347,7 +388,8 @@ __global__ __launch_bounds__(64) void scan_chain(Args A) {
 template <typename T, int CH, int NS, int VE>
 __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
     typedef Wave<T, CH, NS, VE> W;
-    __shared__ __attribute__((aligned(16))) float s_dt[TT * W::WC], s_g[TT * W::WC], s_c[TT * W::NP];
+    __shared__ __attribute__((aligned(16))) float s_dt[TT * W::WC], s_g[TT * W::WC], s_c[TT * W::NP],
+        s_bias[W::WC];
     const int blks = A.nblk * A.G;
     const int blk = blockIdx.x % blks, seg = blockIdx.x / blks % A.segs, b = blockIdx.x / blks / A.segs;
     const W w(A, blk);
@@ -355,6 +397,7 @@ __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
     const long wave = ((long)b * blks + blk) * A.segs + seg;
     float a2[CH][NS], g[CH][NS], sum_dt[CH];
     w.lane_a(A, a2);
+    w.stage_param(A.dt_bias, s_bias);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
         sum_dt[i] = 0.f;
@@ -362,7 +405,7 @@ __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
         for (int j = 0; j < NS; ++j) g[i][j] = 0.f;
     }
     Raw<T, VE> dn[W::NV], zn[W::NV], gn[W::NV];
-    T cn[W::NBC];
+    Raw<T, 1> cn[W::NBC];
     auto fetch = [&](int t0) {
         w.fetch(A.dt, b, t0, te, dn);
         if (A.gate.p) w.fetch(A.gate, b, t0, te, zn);
@@ -373,17 +416,18 @@ __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
     if (te > ts) fetch(t0);
     for (; te > ts && t0 >= ts; t0 -= TT) {
         lds_order();
+        float step[W::NV][VE], dcore[W::NV][VE];
+        stage_steps(w, dn, s_bias, A.softplus, t0, te, step);
+        stage_core<W>(gn, zn, A.gate.p != nullptr, dcore);
 #pragma unroll
-        for (int k = 0; k < W::NV; ++k) {
-            const int at = w.trow(k) * W::WC + w.tcol(k), c = w.c0 + w.tcol(k);
+        for (int k = 0; k < W::NV; ++k)
 #pragma unroll
             for (int v = 0; v < VE; ++v) {
-                s_dt[at + v] = t0 + w.trow(k) < te && c + v < w.cend ? step_of(A, dn[k].get(v), c + v) : 0.f;
-                s_g[at + v] = gn[k].get(v) * (A.gate.p ? silu_f(zn[k].get(v)) : 1.f);
+                s_dt[w.trow(k) * W::WC + w.tcol(k) + v] = step[k][v];
+                s_g[w.trow(k) * W::WC + w.tcol(k) + v] = dcore[k][v];
             }
-        }
 #pragma unroll
-        for (int k = 0; k < W::NBC; ++k) s_c[k * 64 + w.lane] = to_f32(cn[k]);
+        for (int k = 0; k < W::NBC; ++k) s_c[k * 64 + w.lane] = cn[k].get(0);
         lds_order();
         if (t0 > ts) fetch(t0 - TT);
 #pragma unroll
@@ -415,11 +459,10 @@ __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
 template <typename T, int CH, int NS, int VE>
 __global__ __launch_bounds__(64, 2) void scan_bwd(Args A) {
     typedef Wave<T, CH, NS, VE> W;
-    // s_dtx's row of a token is read for the last time where s_gb's is written, so they share their place; the sums over
-    // tokens (s_da, s_sum) wait here while the states of a tile fill the registers
+    // s_dtx's row of a token is read for the last time where s_gb's is written, so they share their place
     __shared__ __attribute__((aligned(16))) float s_dt[TT * W::WC], s_dtx[TT * W::WC], s_g[TT * W::WC], s_y[TT * W::WC],
-        s_ta[TT * W::WC], s_b[TT * W::NP], s_c[TT * W::NP], s_db[TT * W::NP], s_dc[TT * W::NP], s_da[LANE_STATE],
-        s_sum[2][W::PER * 64];
+        s_ta[TT * W::WC], s_b[TT * W::NP], s_c[TT * W::NP], s_db[TT * W::NP], s_dc[TT * W::NP], s_bias[W::WC],
+        s_skip[W::WC], s_sum[2][W::PER * 64];
     float* s_gb = s_dtx;
     const int blks = A.nblk * A.G;
     const int blk = blockIdx.x % blks, seg = blockIdx.x / blks % A.segs, group = blockIdx.x / blks / A.segs;
@@ -427,13 +470,15 @@ __global__ __launch_bounds__(64, 2) void scan_bwd(Args A) {
     const int ntile = (A.L + TT - 1) / TT, ts = seg * A.seg_len, tend = min(A.L, ts + A.seg_len);
     float a2[CH][NS], g[CH][NS], da[CH][NS];
     w.lane_a(A, a2);
+    w.stage_param(A.dt_bias, s_bias);
+    w.stage_param(A.skip, s_skip);
 #pragma unroll
     for (int i = 0; i < CH; ++i)
 #pragma unroll
         for (int j = 0; j < NS; ++j) da[i][j] = 0.f;
-    w.store_own(s_da, da);
 #pragma unroll
     for (int k = 0; k < W::PER; ++k) s_sum[0][k * 64 + w.lane] = s_sum[1][k * 64 + w.lane] = 0.f;
+    lds_order();
     for (int b = group; b < A.B; b += A.bgroups) {
         const int len = length_of(A, b), te = min(len, tend);
         if (A.segs > 1) w.load_own(A.seg_h + (((long)b * blks + blk) * A.segs + seg) * LANE_STATE, g);
@@ -454,25 +499,28 @@ __global__ __launch_bounds__(64, 2) void scan_bwd(Args A) {
             w.fetch(A.dt, b, t0, te, d);
             if (A.gate.p) w.fetch(A.gate, b, t0, te, z);
             w.fetch(A.dy, b, t0, te, gy);
-            T br[W::NBC], cr[W::NBC];
+            Raw<T, 1> br[W::NBC], cr[W::NBC];
             w.fetch_bc(A.b, b, t0, te, A.N, br);
             w.fetch_bc(A.c, b, t0, te, A.N, cr);
             lds_order();
+            {
+                float step[W::NV][VE], dcore[W::NV][VE];
+                stage_steps(w, d, s_bias, A.softplus, t0, te, step);
+                stage_core<W>(gy, z, A.gate.p != nullptr, dcore);
 #pragma unroll
-            for (int k = 0; k < W::NV; ++k) {
-                const int at = w.trow(k) * W::WC + w.tcol(k), c = w.c0 + w.tcol(k);
+                for (int k = 0; k < W::NV; ++k)
 #pragma unroll
-                for (int v = 0; v < VE; ++v) {
-                    const float dt = t0 + w.trow(k) < te && c + v < w.cend ? step_of(A, d[k].get(v), c + v) : 0.f;
-                    s_dt[at + v] = dt;
-                    s_dtx[at + v] = dt * x[k].get(v);
-                    s_g[at + v] = gy[k].get(v) * (A.gate.p ? silu_f(z[k].get(v)) : 1.f);
-                }
+                    for (int v = 0; v < VE; ++v) {
+                        const int at = w.trow(k) * W::WC + w.tcol(k) + v;
+                        s_dt[at] = step[k][v];
+                        s_dtx[at] = step[k][v] * x[k].get(v);
+                        s_g[at] = dcore[k][v];
+                    }
             }
 #pragma unroll
             for (int k = 0; k < W::NBC; ++k) {
-                s_b[k * 64 + w.lane] = to_f32(br[k]);
-                s_c[k * 64 + w.lane] = to_f32(cr[k]);
+                s_b[k * 64 + w.lane] = br[k].get(0);
+                s_c[k * 64 + w.lane] = cr[k].get(0);
             }
             lds_order();
 #pragma unroll
@@ -506,9 +554,14 @@ __global__ __launch_bounds__(64, 2) void scan_bwd(Args A) {
                 __builtin_amdgcn_sched_barrier(0);         // (later tokens' LDS reads would take registers hist needs)
             }
             lds_order();                                   // (and the decays are formed again, not held in 128 registers)
-            w.load_own(s_da, da);
 #pragma unroll
             for (int t = TT - 1; t >= 0; --t) {
+                if (t == TT / 2 - 1) {                     // (the rows again, from L2: half of hist's registers are free now)
+                    w.fetch(A.x, b, t0, te, x);
+                    w.fetch(A.dt, b, t0, te, d);
+                    if (A.gate.p) w.fetch(A.gate, b, t0, te, z);
+                    w.fetch(A.dy, b, t0, te, gy);
+                }
                 float dt[CH], dtx[CH], dc[CH], bv[NS], cv[NS], gb[CH], ta[CH], sb[NS];
                 lds_read<CH>(s_dt + t * W::WC + w.cl * CH, dt);
                 lds_read<CH>(s_dtx + t * W::WC + w.cl * CH, dtx);
@@ -541,50 +594,60 @@ __global__ __launch_bounds__(64, 2) void scan_bwd(Args A) {
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            w.store_own(s_da, da);
             lds_order();
 #pragma unroll
             for (int k = 0; k < W::NBC; ++k) {
-                const int t = t0 + (k * 64 + w.lane) / W::NP, n = (k * 64 + w.lane) % W::NP;
-                if (t < te && n < A.N) {
-                    float* p = A.part_bc + ((((long)(blk % A.nblk) * A.B + b) * A.L + t) * A.G + w.g) * 2 * A.N + n;
-                    p[0] = s_db[k * 64 + w.lane];
-                    p[A.N] = s_dc[k * 64 + w.lane];
-                }
+                const int t = (k * 64 + w.lane) / W::NP, n = (k * 64 + w.lane) % W::NP;
+                const auto rs = buffer_of(
+                    A.part_bc + ((((long)(blk % A.nblk) * A.B + b) * A.L + t0) * A.G + w.g) * 2 * A.N, BUF_BYTES);
+                const unsigned at = t0 + t < te && n < A.N ? (t * A.G * 2 * A.N + n) * 4u : BUF_OUT;
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s_db[k * 64 + w.lane]), rs, at, 0, 0);
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s_dc[k * 64 + w.lane]), rs, at, A.N * 4, 0);
             }
+            float dr[W::NV][VE], core[W::NV][VE];
 #pragma unroll
-            for (int k = 0; k < W::NV; ++k) {
-                const int at = w.trow(k) * W::WC + w.tcol(k), c = w.c0 + w.tcol(k);
-                const bool live = t0 + w.trow(k) < te;
+            for (int k = 0; k < W::NV; ++k)
 #pragma unroll
                 for (int v = 0; v < VE; ++v) {
-                    const bool on = live && c + v < w.cend;
-                    const float xv = x[k].get(v), gb = s_gb[at + v], dc = s_g[at + v];
-                    const float sk = on && A.skip ? A.skip[c + v] : 0.f, bias = on && A.dt_bias ? A.dt_bias[c + v] : 0.f;
-                    float dr = s_ta[at + v] * LN2 + xv * gb;
-                    if (A.softplus) {                      // softplus' = sigmoid, from whichever side does not overflow
-                        const float u = d[k].get(v) + bias, e = exp_f(-fabsf(u)), q = __builtin_amdgcn_rcpf(1.f + e);
-                        dr *= u < 0.f ? e * q : q;
-                    }
-                    s_sum[0][(k * VE + v) * 64 + w.lane] += on ? dc * xv : 0.f;
-                    s_sum[1][(k * VE + v) * 64 + w.lane] += on ? dr : 0.f;
-                    const float dxv = s_dt[at + v] * gb + sk * dc, core = s_y[at + v] + sk * xv;
-                    if (A.gate.p) {
-                        const float zv = z[k].get(v);
-                        z[k].set(v, on ? gy[k].get(v) * core * dsilu_f(zv) : 0.f);
-                    }
-                    x[k].set(v, on ? dxv : 0.f);
-                    d[k].set(v, on ? dr : 0.f);
+                    const int at = w.trow(k) * W::WC + w.tcol(k) + v;
+                    dr[k][v] = s_ta[at] * LN2 + x[k].get(v) * s_gb[at];
+                    core[k][v] = s_y[at] + s_skip[w.tcol(k) + v] * x[k].get(v);
                 }
+            if (A.softplus) {                              // softplus' = sigmoid, from the side that does not overflow
+#pragma unroll
+                for (int k = 0; k < W::NV; ++k)
+#pragma unroll
+                    for (int v = 0; v < VE; ++v) {
+                        const float u = d[k].get(v) + s_bias[w.tcol(k) + v], e = exp_f(-fabsf(u));
+                        dr[k][v] *= (u < 0.f ? e : 1.f) * __builtin_amdgcn_rcpf(1.f + e);
+                    }
             }
+            if (A.gate.p) {
+#pragma unroll
+                for (int k = 0; k < W::NV; ++k)
+#pragma unroll
+                    for (int v = 0; v < VE; ++v)
+                        z[k].set(v, w.staged(k, v, t0, te) ? gy[k].get(v) * core[k][v] * dsilu_f(z[k].get(v)) : 0.f);
+                w.put(A.dgate, b, A.L, A.D, t0, tend, z);
+            }
+#pragma unroll
+            for (int k = 0; k < W::NV; ++k)
+#pragma unroll
+                for (int v = 0; v < VE; ++v) {
+                    const int at = w.trow(k) * W::WC + w.tcol(k) + v;
+                    const bool on = w.staged(k, v, t0, te);
+                    const float dc = s_g[at], e = on ? dr[k][v] : 0.f;
+                    s_sum[0][(k * 64 + w.lane) * VE + v] += on ? dc * x[k].get(v) : 0.f;
+                    s_sum[1][(k * 64 + w.lane) * VE + v] += e;
+                    x[k].set(v, on ? s_dt[at] * s_gb[at] + s_skip[w.tcol(k) + v] * dc : 0.f);
+                    d[k].set(v, e);
+                }
             w.put(A.dx, b, A.L, A.D, t0, tend, x);
             w.put(A.ddt, b, A.L, A.D, t0, tend, d);
-            if (A.gate.p) w.put(A.dgate, b, A.L, A.D, t0, tend, z);
         }
         if (A.dstate && seg == 0) w.store_state(A.dstate, b, A.D, A.N, g);
     }
     float* out = A.part_p + (((long)group * A.segs + seg) * blks + blk) * (LANE_STATE + 2 * W::WC);
-    w.load_own(s_da, da);
     w.store_own(out, da);
     // sums over the tokens of a tile: lanes that staged the same channels meet in LDS
     for (int half = 0; half < 2; ++half) {
@@ -593,7 +656,7 @@ __global__ __launch_bounds__(64, 2) void scan_bwd(Args A) {
         for (int k = 0; k < W::NV; ++k)
 #pragma unroll
             for (int v = 0; v < VE; ++v)
-                s_dt[w.trow(k) * W::WC + w.tcol(k) + v] = s_sum[half][(k * VE + v) * 64 + w.lane];
+                s_dt[w.trow(k) * W::WC + w.tcol(k) + v] = s_sum[half][(k * 64 + w.lane) * VE + v];
         lds_order();
         if (w.lane < W::WC) {
             float s = 0.f;
@@ -747,7 +810,14 @@ bool bad_shape(int dtype, int B, int L, int D, int N, int G) {
            (double)B * L > 1e9 || (double)B * L * D > 4e11 || (double)B * D > 1e10 || (double)B * L * G * N > 1e11 ||
            (double)G * blocks_of(D, G, N) * B > 2e8;
 }
-bool rows_vec(const Rows& r, int e) { return !r.p || (vqa_vec_ok(r.p, r.batch, e) && vqa_vec_ok(r.p, r.row, e)); }
+// (buffer accesses of up to 16 bytes want their addresses on 4 bytes)
+bool on4(const void* p, long stride, int e) { return ((uintptr_t)p & 3) == 0 && stride * e % 4 == 0; }
+bool rows_vec(const Rows& r, int e) { return !r.p || (on4(r.p, r.batch, e) && on4(r.p, r.row, e)); }
+bool far_rows(const Rows& r) { return r.p && (r.row < 0 || r.row > 0x7fffffffL / (4 * TT)); }
+bool far_rows(const Args& A) {
+    return far_rows(A.x) || far_rows(A.dt) || far_rows(A.gate) || far_rows(A.b) || far_rows(A.c) || far_rows(A.dy) ||
+           A.D > 0x7fffffff / (4 * TT) || (long)A.G * A.N > 0x7fffffff / (8 * TT);
+}
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 template <typename T, int CH, int NS, int VE> int launch(int kind, const Args& A, hipStream_t st) {
@@ -824,12 +894,12 @@ extern "C" int vqa_scan_fwd(void* stream, int dtype, const void* x, long x_batch
     A.a = a; A.skip = skip; A.dt_bias = dt_bias; A.state = state; A.lengths = lengths; A.softplus = softplus;
     A.B = B; A.L = L; A.D = D; A.N = N; A.G = G; A.y = y; A.last = last; A.keep = keep;
     plan(A);
-    if ((A.segs > 1 && !ws) || !aligned16(ws) || !aligned16(keep)) return VQA_ERR_ARG;
+    if ((A.segs > 1 && !ws) || !aligned16(ws) || !aligned16(keep) || far_rows(A)) return VQA_ERR_ARG;
     A.seg_h = ws;
     A.seg_dt = ws ? ws + (long)B * A.nblk * G * A.segs * LANE_STATE : nullptr;
     const int e = vqa_elem_bytes(dtype);
     const bool vec = (D / G) % (16 / e) == 0 && rows_vec(A.x, e) && rows_vec(A.dt, e) && rows_vec(A.gate, e) &&
-                     vqa_vec_ok(y, D, e);
+                     on4(y, D, e);
     return by_type(0, dtype, vec, A, static_cast<hipStream_t>(stream));
 }
 
@@ -850,6 +920,7 @@ extern "C" int vqa_scan_bwd(void* stream, int dtype, const void* dy, long dy_bat
     A.a = a; A.skip = skip; A.dt_bias = dt_bias; A.dlast = dlast; A.lengths = lengths; A.softplus = softplus;
     A.B = B; A.L = L; A.D = D; A.N = N; A.G = G; A.keep = const_cast<float*>(keep);
     A.dx = dx; A.ddt = ddt; A.dgate = dgate; A.dstate = dstate;
+    if (far_rows(A)) return VQA_ERR_ARG;
     plan(A);
     A.seg_h = ws;
     A.seg_dt = ws + (A.segs > 1 ? (long)B * A.nblk * G * A.segs * LANE_STATE : 0);
@@ -857,7 +928,7 @@ extern "C" int vqa_scan_bwd(void* stream, int dtype, const void* dy, long dy_bat
     A.part_bc = A.part_p + part_p_floats(A);
     const int e = vqa_elem_bytes(dtype);
     const bool vec = (D / G) % (16 / e) == 0 && rows_vec(A.x, e) && rows_vec(A.dt, e) && rows_vec(A.gate, e) &&
-                     rows_vec(A.dy, e) && vqa_vec_ok(dx, D, e) && vqa_vec_ok(ddt, D, e) && vqa_vec_ok(dgate, D, e);
+                     rows_vec(A.dy, e) && on4(dx, D, e) && on4(ddt, D, e) && on4(dgate, D, e);
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const int rc = by_type(1, dtype, vec, A, st);
     if (rc != VQA_OK) return rc;

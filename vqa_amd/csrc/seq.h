@@ -29,6 +29,26 @@ template <typename T, int V> struct Raw {
     __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<typename RowVec<T, V>::type*>(p) = v; }
 };
 
+// Buffer accesses: a uniform base in scalar registers and a 32-bit byte offset per lane; an offset of BUF_OUT reads zeros
+// and writes nothing (the range check of the hardware), which is how rows and channels past the end are left out.
+constexpr unsigned BUF_OUT = 0x80000000u, BUF_BYTES = 0x7fffffffu;
+template <typename T, int V> __device__ __forceinline__ Raw<T, V> buf_load(__amdgpu_buffer_rsrc_t r, unsigned off) {
+    constexpr int N = V * sizeof(T);
+    Raw<T, V> o;
+    if constexpr (N == 16) o.v = __builtin_bit_cast(typename RowVec<T, V>::type, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+    else if constexpr (N == 8) o.v = __builtin_bit_cast(typename RowVec<T, V>::type, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+    else if constexpr (N == 4) o.v = __builtin_bit_cast(typename RowVec<T, V>::type, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+    else o.v = __builtin_bit_cast(typename RowVec<T, V>::type, __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0));
+    return o;
+}
+template <typename T, int V> __device__ __forceinline__ void buf_store(__amdgpu_buffer_rsrc_t r, unsigned off, const Raw<T, V>& o) {
+    constexpr int N = V * sizeof(T);
+    if constexpr (N == 16) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o.v), r, off, 0, 0);
+    else if constexpr (N == 8) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, o.v), r, off, 0, 0);
+    else if constexpr (N == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, o.v), r, off, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, o.v), r, off, 0, 0);
+}
+
 // exp through the hardware's base-2 exponential (1 ulp; results under 2^-126 become 0)
 __device__ __forceinline__ float exp_f(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 __device__ __forceinline__ float sigmoid_f(float x) { return __builtin_amdgcn_rcpf(1.f + exp_f(-x)); }
