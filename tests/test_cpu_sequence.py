@@ -60,11 +60,10 @@ def test_scan_workspaces_hold_what_the_kernels_write():
         sizes = (ctypes.c_long * 3)()
         assert lib.vqa_scan_ws_bytes(1, B, T, D, N, G, ctypes.addressof(sizes)) == 0
         fwd, keep, bwd = sizes
-        channels = 64 if N <= 16 else 32 if N <= 32 else 16
-        waves = G * -(-(D // G) // channels)
-        assert keep == 4 * 1024 * B * waves * -(-T // 8)
-        assert bwd >= fwd + 4 * (waves // G) * B * T * G * 2 * N + 4 * waves * 1024
+        padded, states = G * -(-(D // G) // (128 if N <= 16 else 64)) * (128 if N <= 16 else 64), 16 if N <= 16 else 32 if N <= 32 else 64
+        assert keep == 4 * B * -(-T // 8) * padded * states
+        assert bwd >= fwd + 4 * B * T * G * 2 * N + 4 * padded * (states + 2)
         assert all(s % 16 == 0 for s in (fwd, keep)) and fwd >= 0
         if fwd:
-            segments = fwd // (4 * B * waves * (1024 + channels))
-            assert fwd == 4 * B * waves * (1024 + channels) * segments and 1 < segments <= max(1, T // 64)
+            segments = fwd // (4 * B * padded * (states + 1))
+            assert fwd == 4 * B * padded * (states + 1) * segments and 1 < segments <= max(1, T // 64)

@@ -6,24 +6,25 @@
 //   dx = dt sum_n G b + skip dcore;  draw = (sum_n a th + x sum_n G b) softplus'(raw + dt_bias);  da = sum_t dt th
 //   db_t = sum_d G dt x;  dc_t = sum_d h dcore;  dgate = dy core silu'(gate);  dskip = sum dcore x;  ddt_bias = sum draw
 // Tokens at or past a sequence's length: dt = 0 (the state stands still), rows and gradients 0; what lies there is never read
-// into a sum (selected away, not multiplied by 0).
+// into a sum (left out by the load, not multiplied by 0).
 //
-// Arithmetic, not memory, bounds it: N exponentials and 4 N other operations per (token, channel) against 8 bytes.  It
-// stays in f32 on the vector ALU (the decay differs per channel AND state, so there is no matrix product in it).  One wave
-// works on 16 CH channels: lane = 16 channel lanes x 4 state rows, each lane holding CH channels x NS states (CH NS = 16) in
-// registers.  What a token needs per channel (dt, dt x, ...) and per state (b, c) is staged in LDS in f32, TT tokens at a
-// time, by a second mapping of the lanes in which global rows are read 16 bytes a lane; the next tile's rows are in flight
-// meanwhile.  Sums over states are three lane-swaps, sums over channels DPP adds.
+// Arithmetic, not memory, bounds it: N exponentials (two issue slots each) and 4 N other operations per (token, channel)
+// against 8 bytes.  It stays in f32 on the vector ALU (the decay differs per channel AND state, so there is no matrix
+// product in it).  One wave works on 16 CH channels: lane = 16 channel lanes x 4 state rows, each lane holding CH channels
+// x NS states in registers.  What a token needs per channel (dt, dt x, ...) and per state (b, c) is staged in LDS in f32, TT
+// tokens at a time, by a second mapping of the lanes in which global rows are read up to 16 bytes a lane; the next tile's
+// rows are in flight meanwhile.  Sums over states are lane swaps, sums over channels DPP adds.
 // With few rows the tokens are cut into segments: a first pass finds each segment's own end state and total decay (the
 // product of decays is exp(a sum dt)), a small one chains them, and the full pass starts every segment from its true
 // state.  The backward does the same from the other end.  For the backward the forward keeps h before every tile.
+// States in workspaces lie as [..][channel, a group's padded to per_pad][NP], NP = 16, 32 or 64 >= N.
 #include "seq.h"
 
 namespace {
 
 typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
 constexpr int TT = 8;                      // tokens of a tile
-constexpr int LANE_STATE = 1024;           // floats of one wave's states: 64 lanes x CH NS
+constexpr int BW = 4;                      // waves of a backward workgroup
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct Rows { const void* p; long batch, row; };          // [B][L][...], element strides; the last axis is contiguous
@@ -33,9 +34,10 @@ struct Args {
     const float *a, *skip, *dt_bias, *state, *dlast;
     const int* lengths;
     int softplus, B, L, D, N, G;
-    int nblk, segs, seg_len, bgroups;      // waves across a group's channels, segments, tokens per segment, batch groups
+    int per, per_pad, fblk, bblk;          // channels of a group, padded; forward waves, backward workgroups across it
+    int segs, seg_len, bgroups;            // segments, tokens of one, batch groups of the backward
     void* y; float* last;
-    float *keep, *seg_h, *seg_dt;          // h before every tile; per segment: state, then the true incoming state; sum dt
+    float *keep, *seg_h, *seg_dt;          // h before every tile; per segment: state, then the true incoming one; sum dt
     void *dx, *ddt, *dgate; float *part_bc, *part_p, *dstate;
 };
 
@@ -77,6 +79,29 @@ template <int CH> __device__ __forceinline__ float sum_states(const float (&v)[C
     else { const float s = swap_add32(v[0], v[0]); return swap_add16(s, s); }
 }
 
+// Each of four values summed over the 16 lanes of a row; lanes 4 k .. 4 k + 3 receive value sum16_of(k).  The first two steps
+// halve the values as well as the lanes: a DPP add writes only the banks (groups of four lanes) of its mask, so two adds
+// leave one value's sum in one half of the row and the other's in the other.  Eight adds in place of sixteen; the s_nops
+// cover the two wait states between a VALU write and a DPP read of it.
+__device__ __forceinline__ float sum16_four(float a, float b, float c, float d) {
+    float p, q, s;
+    asm("s_nop 1\n"
+        "v_add_f32_dpp %0, %3, %3 row_ror:8 row_mask:0xf bank_mask:0x3\n"
+        "v_add_f32_dpp %1, %5, %5 row_ror:8 row_mask:0xf bank_mask:0x3\n"
+        "v_add_f32_dpp %0, %4, %4 row_ror:8 row_mask:0xf bank_mask:0xc\n"
+        "v_add_f32_dpp %1, %6, %6 row_ror:8 row_mask:0xf bank_mask:0xc\n"
+        "s_nop 0\n"
+        "v_add_f32_dpp %2, %0, %0 row_half_mirror row_mask:0xf bank_mask:0x5\n"
+        "v_add_f32_dpp %2, %1, %1 row_half_mirror row_mask:0xf bank_mask:0xa\n"
+        "s_nop 1\n"
+        "v_add_f32_dpp %2, %2, %2 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n"
+        "s_nop 1\n"
+        "v_add_f32_dpp %2, %2, %2 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n"
+        : "=&v"(p), "=&v"(q), "=&v"(s) : "v"(a), "v"(b), "v"(c), "v"(d));
+    return s;
+}
+__device__ __forceinline__ int sum16_of(int bank) { return (bank & 1) << 1 | bank >> 1; }
+
 template <int N> __device__ __forceinline__ void lds_read(const float* p, float (&v)[N]) {
     if constexpr (N % 4 == 0) {
 #pragma unroll
@@ -90,29 +115,31 @@ template <int N> __device__ __forceinline__ void lds_read(const float* p, float 
     } else v[0] = *p;
 }
 
-// Where a wave is: its channels [c0, c0 + 16 CH) of group g up to the group's end, and its lane's places in both mappings.
+// Where a wave is: its channels [c0, c0 + 16 CH) of group g up to the group's end (p0: the first one's place in a
+// workspace), and its lane's places in both mappings.
 template <typename T, int CH, int NS, int VE> struct Wave {
-    static constexpr int WC = 16 * CH, NP = 4 * NS, PER = TT * WC / 64, NV = PER / VE, NBC = TT * NP / 64;
-    int lane, cl, r, g, c0, cend;
-    __device__ __forceinline__ Wave(const Args& A, int blk) {
-        lane = threadIdx.x;
+    static constexpr int WC = 16 * CH, NP = 4 * NS, NV = TT * WC / 64 / VE;
+    int lane, cl, r, g, c0, cend, p0;
+    __device__ __forceinline__ Wave(const Args& A, int group, int first) {
+        lane = threadIdx.x & 63;
         cl = lane & 15;
         r = lane >> 4;
-        g = blk / A.nblk;
-        const int per = A.D / A.G;
-        c0 = g * per + (blk % A.nblk) * WC;
-        cend = (g + 1) * per;
+        g = group;
+        c0 = g * A.per + first;
+        cend = (g + 1) * A.per;
+        p0 = g * A.per_pad + first;
     }
     __device__ __forceinline__ int channel(int i) const { return c0 + cl * CH + i; }
     // staging: vector k of this lane is token trow(k) of the tile, channels c0 + tcol(k) ...
     __device__ __forceinline__ int trow(int k) const { return (k * 64 + lane) / (WC / VE); }
     __device__ __forceinline__ int tcol(int k) const { return (k * 64 + lane) % (WC / VE) * VE; }
+    __device__ __forceinline__ int tat(int k) const { return trow(k) * WC + tcol(k); }
+    __device__ __forceinline__ bool staged(int k, int v, int t0, int te) const {
+        return t0 + trow(k) < te && c0 + tcol(k) + v < cend;
+    }
     // (a tile's base is uniform; 8 rows of any tensor span less than 2^31 bytes: the host sees to it)
     __device__ __forceinline__ unsigned place(int k, int row, int t0, int te) const {
         return t0 + trow(k) < te && c0 + tcol(k) < cend ? (trow(k) * row + tcol(k)) * (unsigned)sizeof(T) : BUF_OUT;
-    }
-    __device__ __forceinline__ bool staged(int k, int v, int t0, int te) const {
-        return t0 + trow(k) < te && c0 + tcol(k) + v < cend;
     }
     __device__ __forceinline__ void fetch(const Rows& R, int b, int t0, int te, Raw<T, VE> (&v)[NV]) const {
         const auto rs = buffer_of(static_cast<const T*>(R.p) + b * R.batch + t0 * R.row + c0, BUF_BYTES);
@@ -123,14 +150,6 @@ template <typename T, int CH, int NS, int VE> struct Wave {
         const auto rs = buffer_of(static_cast<T*>(p) + ((long)b * L + t0) * D + c0, BUF_BYTES);
 #pragma unroll
         for (int k = 0; k < NV; ++k) buf_store<T, VE>(rs, place(k, D, t0, te), v[k]);
-    }
-    __device__ __forceinline__ void fetch_bc(const Rows& R, int b, int t0, int te, int N, Raw<T, 1> (&v)[NBC]) const {
-        const auto rs = buffer_of(static_cast<const T*>(R.p) + b * R.batch + t0 * R.row + (long)g * N, BUF_BYTES);
-#pragma unroll
-        for (int k = 0; k < NBC; ++k) {
-            const int t = (k * 64 + lane) / NP, n = (k * 64 + lane) % NP;
-            v[k] = buf_load<T, 1>(rs, t0 + t < te && n < N ? (t * (int)R.row + n) * (unsigned)sizeof(T) : BUF_OUT);
-        }
     }
     // per-channel parameters of the staged channels, in LDS for the whole run
     __device__ __forceinline__ void stage_param(const float* p, float* s) const {
@@ -146,7 +165,7 @@ template <typename T, int CH, int NS, int VE> struct Wave {
             }
     }
     // a state in its public layout [B][D][N]
-    __device__ __forceinline__ void load_state(const float* s, int b, int D, int N, float (&h)[CH][NS]) const {
+    __device__ __forceinline__ void load_public(const float* s, int b, int D, int N, float (&h)[CH][NS]) const {
 #pragma unroll
         for (int i = 0; i < CH; ++i)
 #pragma unroll
@@ -155,7 +174,7 @@ template <typename T, int CH, int NS, int VE> struct Wave {
                 h[i][j] = s && channel(i) < cend && n < N ? s[((long)b * D + channel(i)) * N + n] : 0.f;
             }
     }
-    __device__ __forceinline__ void store_state(float* s, int b, int D, int N, const float (&h)[CH][NS]) const {
+    __device__ __forceinline__ void store_public(float* s, int b, int D, int N, const float (&h)[CH][NS]) const {
 #pragma unroll
         for (int i = 0; i < CH; ++i)
 #pragma unroll
@@ -164,23 +183,42 @@ template <typename T, int CH, int NS, int VE> struct Wave {
                 if (channel(i) < cend && n < N) s[((long)b * D + channel(i)) * N + n] = h[i][j];
             }
     }
-    // ... and in the wave's own: 4 x 16 bytes a lane, lanes side by side
+    // ... and in a workspace: p = its first channel's place in it.  Channels past the end: 0, nothing
+    __device__ __forceinline__ unsigned own_place(int i, int j) const {
+        return channel(i) < cend ? (unsigned)((cl * CH + i) * NP + r * NS + j) * 4u : BUF_OUT;
+    }
     __device__ __forceinline__ void load_own(const float* p, float (&h)[CH][NS]) const {
+        const auto rs = buffer_of(p, BUF_BYTES);
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            const float4 f = *reinterpret_cast<const float4*>(p + (v * 64 + lane) * 4);
-            h[v * 4 / NS][v * 4 % NS] = f.x; h[v * 4 / NS][v * 4 % NS + 1] = f.y;
-            h[v * 4 / NS][v * 4 % NS + 2] = f.z; h[v * 4 / NS][v * 4 % NS + 3] = f.w;
-        }
+        for (int i = 0; i < CH; ++i)
+#pragma unroll
+            for (int j = 0; j < NS; j += 4) {
+                const Raw<float, 4> f = buf_load<float, 4>(rs, own_place(i, j));
+#pragma unroll
+                for (int q = 0; q < 4; ++q) h[i][j + q] = f.get(q);
+            }
     }
     __device__ __forceinline__ void store_own(float* p, const float (&h)[CH][NS]) const {
+        const auto rs = buffer_of(p, BUF_BYTES);
 #pragma unroll
-        for (int v = 0; v < 4; ++v)
-            *reinterpret_cast<float4*>(p + (v * 64 + lane) * 4) =
-                make_float4(h[v * 4 / NS][v * 4 % NS], h[v * 4 / NS][v * 4 % NS + 1], h[v * 4 / NS][v * 4 % NS + 2],
-                            h[v * 4 / NS][v * 4 % NS + 3]);
+        for (int i = 0; i < CH; ++i)
+#pragma unroll
+            for (int j = 0; j < NS; j += 4) {
+                Raw<float, 4> f;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) f.set(q, h[i][j + q]);
+                buf_store<float, 4>(rs, own_place(i, j), f);
+            }
     }
 };
+
+// b or c of a tile: element id = token * NP + state of [TT][NP], 0 past the tokens and the states
+template <typename T, int NP>
+__device__ __forceinline__ Raw<T, 1> fetch_shared(const Rows& R, int b, int t0, int te, int g, int N, int id) {
+    const auto rs = buffer_of(static_cast<const T*>(R.p) + b * R.batch + t0 * R.row + (long)g * N, BUF_BYTES);
+    const int t = id / NP, n = id % NP;
+    return buf_load<T, 1>(rs, t0 + t < te && n < N ? (t * (int)R.row + n) * (unsigned)sizeof(T) : BUF_OUT);
+}
 
 __device__ __forceinline__ int length_of(const Args& A, int b) {
     return A.lengths ? max(0, min(A.L, A.lengths[b])) : A.L;
@@ -224,13 +262,14 @@ __device__ __forceinline__ void stage_core(const R (&gy)[NV], const R (&z)[NV], 
 template <typename T, int CH, int NS, int VE, bool FULL>
 __global__ __launch_bounds__(64) void scan_fwd(Args A) {
     typedef Wave<T, CH, NS, VE> W;
+    constexpr int NBC = TT * W::NP / 64;
     __shared__ __attribute__((aligned(16))) float s_dt[TT * W::WC], s_dtx[TT * W::WC], s_y[FULL ? TT * W::WC : 4],
         s_b[TT * W::NP], s_c[FULL ? TT * W::NP : 4], s_bias[W::WC], s_skip[FULL ? W::WC : 4];
-    const int blks = A.nblk * A.G;
+    const int blks = A.fblk * A.G;
     const int blk = blockIdx.x % blks, seg = blockIdx.x / blks % A.segs, b = blockIdx.x / blks / A.segs;
-    const W w(A, blk);
-    const int len = length_of(A, b), ts = seg * A.seg_len, te = min(A.L, ts + A.seg_len);
-    const long wave = ((long)b * blks + blk) * A.segs + seg;
+    const W w(A, blk / A.fblk, blk % A.fblk * W::WC);
+    const int len = length_of(A, b), ts = seg * A.seg_len, te = min(A.L, ts + A.seg_len), live = min(len, te);
+    const long chans = (long)A.G * A.per_pad, at_seg = ((long)b * A.segs + seg) * chans + w.p0;
     const int ntile = (A.L + TT - 1) / TT;
     float a2[CH][NS], h[CH][NS], sum_dt[CH];
     w.lane_a(A, a2);
@@ -243,18 +282,19 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
         for (int j = 0; j < NS; ++j) h[i][j] = 0.f;
     }
     if (FULL) {
-        if (A.segs > 1) w.load_own(A.seg_h + wave * LANE_STATE, h);
-        else w.load_state(A.state, b, A.D, A.N, h);
+        if (A.segs > 1) w.load_own(A.seg_h + at_seg * W::NP, h);
+        else w.load_public(A.state, b, A.D, A.N, h);
     }
     Raw<T, VE> x[W::NV], d[W::NV], z[W::NV], xn[W::NV], dn[W::NV], zn[W::NV];
-    Raw<T, 1> bn[W::NBC], cn[W::NBC];
+    Raw<T, 1> bn[NBC], cn[NBC];
     auto fetch = [&](int t0) {
-        w.fetch(A.x, b, t0, min(len, te), xn);
-        w.fetch(A.dt, b, t0, min(len, te), dn);
-        w.fetch_bc(A.b, b, t0, min(len, te), A.N, bn);
-        if (FULL) {
-            if (A.gate.p) w.fetch(A.gate, b, t0, min(len, te), zn);
-            w.fetch_bc(A.c, b, t0, min(len, te), A.N, cn);
+        w.fetch(A.x, b, t0, live, xn);
+        w.fetch(A.dt, b, t0, live, dn);
+        if (FULL && A.gate.p) w.fetch(A.gate, b, t0, live, zn);
+#pragma unroll
+        for (int k = 0; k < NBC; ++k) {
+            bn[k] = fetch_shared<T, W::NP>(A.b, b, t0, live, w.g, A.N, k * 64 + w.lane);
+            if (FULL) cn[k] = fetch_shared<T, W::NP>(A.c, b, t0, live, w.g, A.N, k * 64 + w.lane);
         }
     };
     fetch(ts);
@@ -270,23 +310,22 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
         for (int k = 0; k < W::NV; ++k) { x[k] = xn[k]; d[k] = dn[k]; if (FULL) z[k] = zn[k]; }
         lds_order();                                       // (the last tile's reads are done)
         float step[W::NV][VE];
-        stage_steps(w, d, s_bias, A.softplus, t0, min(len, te), step);
+        stage_steps(w, d, s_bias, A.softplus, t0, live, step);
 #pragma unroll
         for (int k = 0; k < W::NV; ++k)
 #pragma unroll
             for (int v = 0; v < VE; ++v) {
-                const int at = w.trow(k) * W::WC + w.tcol(k) + v;
-                s_dt[at] = step[k][v];
-                s_dtx[at] = step[k][v] * x[k].get(v);
+                s_dt[w.tat(k) + v] = step[k][v];
+                s_dtx[w.tat(k) + v] = step[k][v] * x[k].get(v);
             }
 #pragma unroll
-        for (int k = 0; k < W::NBC; ++k) {
+        for (int k = 0; k < NBC; ++k) {
             s_b[k * 64 + w.lane] = bn[k].get(0);
             if (FULL) s_c[k * 64 + w.lane] = cn[k].get(0);
         }
         lds_order();
         if (t0 + TT < te) fetch(t0 + TT);
-        if (FULL && A.keep) w.store_own(A.keep + (((long)b * blks + blk) * ntile + t0 / TT) * LANE_STATE, h);
+        if (FULL && A.keep) w.store_own(A.keep + (((long)b * ntile + t0 / TT) * chans + w.p0) * W::NP, h);
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
             float dt[CH], dtx[CH], bv[NS], cv[NS], y[CH];
@@ -309,13 +348,9 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
         if (FULL) {
             lds_order();
 #pragma unroll
-            for (int k = 0; k < W::NV; ++k) {
-                const int at = w.trow(k) * W::WC + w.tcol(k);
+            for (int k = 0; k < W::NV; ++k)
 #pragma unroll
-                for (int v = 0; v < VE; ++v) {
-                    step[k][v] = s_y[at + v] + s_skip[w.tcol(k) + v] * x[k].get(v);
-                }
-            }
+                for (int v = 0; v < VE; ++v) step[k][v] = s_y[w.tat(k) + v] + s_skip[w.tcol(k) + v] * x[k].get(v);
             if (A.gate.p) {
 #pragma unroll
                 for (int k = 0; k < W::NV; ++k)
@@ -330,51 +365,48 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
         }
     }
     if (FULL) {
-        if (A.last && seg == A.segs - 1) w.store_state(A.last, b, A.D, A.N, h);
+        if (A.last && seg == A.segs - 1) w.store_public(A.last, b, A.D, A.N, h);
     } else {
-        w.store_own(A.seg_h + wave * LANE_STATE, h);
+        w.store_own(A.seg_h + at_seg * W::NP, h);
         if (w.r == 0) {
 #pragma unroll
-            for (int i = 0; i < CH; ++i) A.seg_dt[wave * W::WC + w.cl * CH + i] = sum_dt[i];
+            for (int i = 0; i < CH; ++i)
+                if (w.channel(i) < w.cend) A.seg_dt[at_seg + w.cl * CH + i] = sum_dt[i];
         }
     }
 }
 
-// Chains the segments: seg_h[s] becomes the state (REV: the adjoint) that comes into segment s.  A wave takes 16 bytes per
-// lane of one wave's states; eight segments are in flight.
-template <int CH, int NS, bool REV>
-__global__ __launch_bounds__(64) void scan_chain(Args A) {
-    typedef Wave<float, CH, NS, 1> W;
-    const int blks = A.nblk * A.G, v = blockIdx.x & 3, blk = (blockIdx.x >> 2) % blks, b = (blockIdx.x >> 2) / blks;
-    const W w(A, blk);
-    float a2[CH][NS], h0[CH][NS];
-    w.lane_a(A, a2);
-    w.load_state(REV ? A.dlast : A.state, b, A.D, A.N, h0);
+// Chains the segments: seg_h[s] becomes the state (REV: the adjoint) that comes into segment s.  A thread takes four states
+// of a channel; eight segments are in flight.
+template <int NP, bool REV> __global__ __launch_bounds__(256) void scan_chain(Args A) {
+    const long chans = (long)A.G * A.per_pad, id = (long)blockIdx.x * 256 + threadIdx.x;
+    if (id >= A.B * chans * (NP / 4)) return;
+    const int n = (int)(id % (NP / 4)) * 4, p = (int)(id / (NP / 4) % chans), b = (int)(id / (NP / 4) / chans);
+    const int g = p / A.per_pad, off = p % A.per_pad, c = g * A.per + off;
+    if (off >= A.per) return;
+    const float* start = REV ? A.dlast : A.state;
     float a[4], h[4];
-    int chan = 0;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)                            // (selects with constant indices: v is the same in all lanes)
-        if (u == v) {
-            chan = u * 4 / NS;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) { a[k] = a2[u * 4 / NS][u * 4 % NS + k]; h[k] = h0[u * 4 / NS][u * 4 % NS + k]; }
-        }
-    const long first = ((long)b * blks + blk) * A.segs;
-    float4* p = reinterpret_cast<float4*>(A.seg_h + first * LANE_STATE) + v * 64 + w.lane;
-    const float* q = A.seg_dt + first * W::WC + w.cl * CH + chan;
+    for (int k = 0; k < 4; ++k) {
+        a[k] = n + k < A.N ? A.a[(long)c * A.N + n + k] * LOG2E : 0.f;
+        h[k] = start && n + k < A.N ? start[((long)b * A.D + c) * A.N + n + k] : 0.f;
+    }
+    const long first = (long)b * A.segs * chans + p;
+    float4* q = reinterpret_cast<float4*>(A.seg_h + first * NP + n);
+    const float* dt = A.seg_dt + first;
     for (int s0 = 0; s0 < A.segs; s0 += 8) {
         float4 e[8];
         float d[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const int s = REV ? A.segs - 1 - s0 - u : s0 + u;
-            if (s >= 0 && s < A.segs) { e[u] = p[(long)s * (LANE_STATE / 4)]; d[u] = q[(long)s * W::WC]; }
+            if (s >= 0 && s < A.segs) { e[u] = q[s * chans * (NP / 4)]; d[u] = dt[s * chans]; }
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             const int s = REV ? A.segs - 1 - s0 - u : s0 + u;
             if (s >= 0 && s < A.segs) {
-                p[(long)s * (LANE_STATE / 4)] = make_float4(h[0], h[1], h[2], h[3]);
+                q[s * chans * (NP / 4)] = make_float4(h[0], h[1], h[2], h[3]);
                 h[0] = __builtin_amdgcn_exp2f(d[u] * a[0]) * h[0] + e[u].x;
                 h[1] = __builtin_amdgcn_exp2f(d[u] * a[1]) * h[1] + e[u].y;
                 h[2] = __builtin_amdgcn_exp2f(d[u] * a[2]) * h[2] + e[u].z;
@@ -388,13 +420,13 @@ __global__ __launch_bounds__(64) void scan_chain(Args A) {
 template <typename T, int CH, int NS, int VE>
 __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
     typedef Wave<T, CH, NS, VE> W;
-    __shared__ __attribute__((aligned(16))) float s_dt[TT * W::WC], s_g[TT * W::WC], s_c[TT * W::NP],
-        s_bias[W::WC];
-    const int blks = A.nblk * A.G;
+    constexpr int NBC = TT * W::NP / 64;
+    __shared__ __attribute__((aligned(16))) float s_dt[TT * W::WC], s_g[TT * W::WC], s_c[TT * W::NP], s_bias[W::WC];
+    const int blks = A.fblk * A.G;
     const int blk = blockIdx.x % blks, seg = blockIdx.x / blks % A.segs, b = blockIdx.x / blks / A.segs;
-    const W w(A, blk);
+    const W w(A, blk / A.fblk, blk % A.fblk * W::WC);
     const int ts = seg * A.seg_len, te = min(length_of(A, b), min(A.L, ts + A.seg_len));
-    const long wave = ((long)b * blks + blk) * A.segs + seg;
+    const long chans = (long)A.G * A.per_pad, at_seg = ((long)b * A.segs + seg) * chans + w.p0;
     float a2[CH][NS], g[CH][NS], sum_dt[CH];
     w.lane_a(A, a2);
     w.stage_param(A.dt_bias, s_bias);
@@ -405,12 +437,13 @@ __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
         for (int j = 0; j < NS; ++j) g[i][j] = 0.f;
     }
     Raw<T, VE> dn[W::NV], zn[W::NV], gn[W::NV];
-    Raw<T, 1> cn[W::NBC];
+    Raw<T, 1> cn[NBC];
     auto fetch = [&](int t0) {
         w.fetch(A.dt, b, t0, te, dn);
         if (A.gate.p) w.fetch(A.gate, b, t0, te, zn);
         w.fetch(A.dy, b, t0, te, gn);
-        w.fetch_bc(A.c, b, t0, te, A.N, cn);
+#pragma unroll
+        for (int k = 0; k < NBC; ++k) cn[k] = fetch_shared<T, W::NP>(A.c, b, t0, te, w.g, A.N, k * 64 + w.lane);
     };
     int t0 = ts + (te - ts - 1) / TT * TT;
     if (te > ts) fetch(t0);
@@ -423,11 +456,11 @@ __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
         for (int k = 0; k < W::NV; ++k)
 #pragma unroll
             for (int v = 0; v < VE; ++v) {
-                s_dt[w.trow(k) * W::WC + w.tcol(k) + v] = step[k][v];
-                s_g[w.trow(k) * W::WC + w.tcol(k) + v] = dcore[k][v];
+                s_dt[w.tat(k) + v] = step[k][v];
+                s_g[w.tat(k) + v] = dcore[k][v];
             }
 #pragma unroll
-        for (int k = 0; k < W::NBC; ++k) s_c[k * 64 + w.lane] = cn[k].get(0);
+        for (int k = 0; k < NBC; ++k) s_c[k * 64 + w.lane] = cn[k].get(0);
         lds_order();
         if (t0 > ts) fetch(t0 - TT);
 #pragma unroll
@@ -445,30 +478,38 @@ __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
             }
         }
     }
-    w.store_own(A.seg_h + wave * LANE_STATE, g);
+    w.store_own(A.seg_h + at_seg * W::NP, g);
     if (w.r == 0) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) A.seg_dt[wave * W::WC + w.cl * CH + i] = sum_dt[i];
+        for (int i = 0; i < CH; ++i)
+            if (w.channel(i) < w.cend) A.seg_dt[at_seg + w.cl * CH + i] = sum_dt[i];
     }
 }
 
 // The backward.  Tiles from the last to the first; inside a tile the states are computed again from the kept one, forwards,
-// staying in registers (h before each of the TT tokens), then the adjoint runs backwards over them.
-// One wave takes the sequences of its batch group one after the other, so that its sums over tokens leave once:
-// part_p[(group * segs + seg)][block]{da: LANE_STATE, dskip: WC, ddt_bias: WC}; part_bc[block of group][B][L][G][2][N].
+// staying in registers (h before each of the TT tokens), then the adjoint runs backwards over them.  Those TT CH NS
+// registers are why a lane has half the forward's channels: at 16 states a lane they do not fit, and the spills cost more
+// than all the rest (566 us against 88 of the forward at 4 x 2048 tokens x 2048 channels).
+// The BW waves of a workgroup take neighbouring channels, share b and c in LDS and join their sums db, dc over channels
+// there: part_bc[workgroup of the group][B][L][G][2][N].  A workgroup takes the sequences of its batch group one after the
+// other, so that its sums over tokens leave once: part_p[(batch group, segment)]{da [channel][NP], dskip, ddt_bias}.
 template <typename T, int CH, int NS, int VE>
-__global__ __launch_bounds__(64, 2) void scan_bwd(Args A) {
+__global__ __launch_bounds__(64 * BW) void scan_bwd(Args A) {
     typedef Wave<T, CH, NS, VE> W;
-    // s_dtx's row of a token is read for the last time where s_gb's is written, so they share their place
-    __shared__ __attribute__((aligned(16))) float s_dt[TT * W::WC], s_dtx[TT * W::WC], s_g[TT * W::WC], s_y[TT * W::WC],
-        s_ta[TT * W::WC], s_b[TT * W::NP], s_c[TT * W::NP], s_db[TT * W::NP], s_dc[TT * W::NP], s_bias[W::WC],
-        s_skip[W::WC], s_sum[2][W::PER * 64];
-    float* s_gb = s_dtx;
-    const int blks = A.nblk * A.G;
+    constexpr int TILE = TT * W::WC, SH = TT * W::NP, NBC = 2 * SH / (64 * BW);
+    __shared__ __attribute__((aligned(16))) float lds[BW][6 * TILE + 2 * W::WC], s_bc[2 * SH], s_part[BW][2 * SH];
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int blks = A.bblk * A.G;
     const int blk = blockIdx.x % blks, seg = blockIdx.x / blks % A.segs, group = blockIdx.x / blks / A.segs;
-    const W w(A, blk);
+    const W w(A, blk / A.bblk, (blk % A.bblk * BW + wv) * W::WC);
+    const bool live = w.c0 < w.cend;                       // (a wave past the group's end only keeps step)
+    float *s_dt = lds[wv], *s_dtx = s_dt + TILE, *s_g = s_dtx + TILE, *s_y = s_g + TILE, *s_gt = s_y + TILE,
+          *s_bias = s_gt + 2 * TILE, *s_skip = s_bias + W::WC, *s_db = s_part[wv], *s_dc = s_db + SH;
+    const float *s_b = s_bc, *s_c = s_bc + SH;
+    const long chans = (long)A.G * A.per_pad;
     const int ntile = (A.L + TT - 1) / TT, ts = seg * A.seg_len, tend = min(A.L, ts + A.seg_len);
-    float a2[CH][NS], g[CH][NS], da[CH][NS];
+    const int state_at = w.r * NS + sum16_of(w.cl >> 2);   // where this lane's value of sum16_four belongs
+    float a2[CH][NS], g[CH][NS], da[CH][NS], sum_skip[W::NV][VE], sum_bias[W::NV][VE];
     w.lane_a(A, a2);
     w.stage_param(A.dt_bias, s_bias);
     w.stage_param(A.skip, s_skip);
@@ -477,12 +518,15 @@ __global__ __launch_bounds__(64, 2) void scan_bwd(Args A) {
 #pragma unroll
         for (int j = 0; j < NS; ++j) da[i][j] = 0.f;
 #pragma unroll
-    for (int k = 0; k < W::PER; ++k) s_sum[0][k * 64 + w.lane] = s_sum[1][k * 64 + w.lane] = 0.f;
-    lds_order();
+    for (int k = 0; k < W::NV; ++k)
+#pragma unroll
+        for (int v = 0; v < VE; ++v) sum_skip[k][v] = sum_bias[k][v] = 0.f;
+    if (!live)
+        for (int k = w.lane; k < 2 * SH; k += 64) s_db[k] = 0.f;
     for (int b = group; b < A.B; b += A.bgroups) {
-        const int len = length_of(A, b), te = min(len, tend);
-        if (A.segs > 1) w.load_own(A.seg_h + (((long)b * blks + blk) * A.segs + seg) * LANE_STATE, g);
-        else w.load_state(A.dlast, b, A.D, A.N, g);
+        const int te = min(length_of(A, b), tend);
+        if (A.segs > 1) w.load_own(A.seg_h + (((long)b * A.segs + seg) * chans + w.p0) * W::NP, g);
+        else w.load_public(A.dlast, b, A.D, A.N, g);
         for (int t0 = ts + (tend - ts - 1) / TT * TT; t0 >= ts; t0 -= TT) {
             Raw<T, VE> x[W::NV], d[W::NV], z[W::NV], gy[W::NV];
             if (t0 >= te) {                                // past the end of this sequence: zero rows
@@ -494,16 +538,17 @@ __global__ __launch_bounds__(64, 2) void scan_bwd(Args A) {
                 continue;
             }
             float hist[TT][CH][NS], h[CH][NS];
-            w.load_own(A.keep + (((long)b * blks + blk) * ntile + t0 / TT) * LANE_STATE, h);
+            w.load_own(A.keep + (((long)b * ntile + t0 / TT) * chans + w.p0) * W::NP, h);
             w.fetch(A.x, b, t0, te, x);
             w.fetch(A.dt, b, t0, te, d);
             if (A.gate.p) w.fetch(A.gate, b, t0, te, z);
             w.fetch(A.dy, b, t0, te, gy);
-            Raw<T, 1> br[W::NBC], cr[W::NBC];
-            w.fetch_bc(A.b, b, t0, te, A.N, br);
-            w.fetch_bc(A.c, b, t0, te, A.N, cr);
-            lds_order();
-            {
+#pragma unroll
+            for (int k = 0; k < NBC; ++k) {
+                const int id = k * 64 * BW + threadIdx.x;
+                s_bc[id] = fetch_shared<T, W::NP>(id < SH ? A.b : A.c, b, t0, te, w.g, A.N, id % SH).get(0);
+            }
+            if (live) {
                 float step[W::NV][VE], dcore[W::NV][VE];
                 stage_steps(w, d, s_bias, A.softplus, t0, te, step);
                 stage_core<W>(gy, z, A.gate.p != nullptr, dcore);
@@ -511,169 +556,155 @@ __global__ __launch_bounds__(64, 2) void scan_bwd(Args A) {
                 for (int k = 0; k < W::NV; ++k)
 #pragma unroll
                     for (int v = 0; v < VE; ++v) {
-                        const int at = w.trow(k) * W::WC + w.tcol(k) + v;
-                        s_dt[at] = step[k][v];
-                        s_dtx[at] = step[k][v] * x[k].get(v);
-                        s_g[at] = dcore[k][v];
+                        s_dt[w.tat(k) + v] = step[k][v];
+                        s_dtx[w.tat(k) + v] = step[k][v] * x[k].get(v);
+                        s_g[w.tat(k) + v] = dcore[k][v];
                     }
             }
+            __syncthreads();                               // b, c are there; the last tile's s_part has been read
+            if (live) {
 #pragma unroll
-            for (int k = 0; k < W::NBC; ++k) {
-                s_b[k * 64 + w.lane] = br[k].get(0);
-                s_c[k * 64 + w.lane] = cr[k].get(0);
-            }
-            lds_order();
+                for (int t = 0; t < TT; ++t) {
+                    float dt[CH], dtx[CH], dc[CH], bv[NS], cv[NS], y[CH], sc[NS];
+                    lds_read<CH>(s_dt + t * W::WC + w.cl * CH, dt);
+                    lds_read<CH>(s_dtx + t * W::WC + w.cl * CH, dtx);
+                    lds_read<CH>(s_g + t * W::WC + w.cl * CH, dc);
+                    lds_read<NS>(s_b + t * W::NP + w.r * NS, bv);
+                    lds_read<NS>(s_c + t * W::NP + w.r * NS, cv);
 #pragma unroll
-            for (int t = 0; t < TT; ++t) {
-                float dt[CH], dtx[CH], dc[CH], bv[NS], cv[NS], y[CH], sc[NS];
-                lds_read<CH>(s_dt + t * W::WC + w.cl * CH, dt);
-                lds_read<CH>(s_dtx + t * W::WC + w.cl * CH, dtx);
-                lds_read<CH>(s_g + t * W::WC + w.cl * CH, dc);
-                lds_read<NS>(s_b + t * W::NP + w.r * NS, bv);
-                lds_read<NS>(s_c + t * W::NP + w.r * NS, cv);
+                    for (int j = 0; j < NS; ++j) sc[j] = 0.f;
 #pragma unroll
-                for (int j = 0; j < NS; ++j) sc[j] = 0.f;
+                    for (int i = 0; i < CH; ++i) {
+                        y[i] = 0.f;
 #pragma unroll
-                for (int i = 0; i < CH; ++i) {
-                    y[i] = 0.f;
-#pragma unroll
-                    for (int j = 0; j < NS; ++j) {
-                        hist[t][i][j] = h[i][j];
-                        h[i][j] = __builtin_amdgcn_exp2f(dt[i] * a2[i][j]) * h[i][j] + dtx[i] * bv[j];
-                        y[i] += h[i][j] * cv[j];
-                        sc[j] += h[i][j] * dc[i];
+                        for (int j = 0; j < NS; ++j) {
+                            hist[t][i][j] = h[i][j];
+                            h[i][j] = __builtin_amdgcn_exp2f(dt[i] * a2[i][j]) * h[i][j] + dtx[i] * bv[j];
+                            y[i] += h[i][j] * cv[j];
+                            sc[j] += h[i][j] * dc[i];
+                        }
                     }
+                    s_y[t * W::WC + w.cl * CH + own_channel<CH>(w.r)] = sum_states<CH>(y);
+#pragma unroll
+                    for (int j = 0; j < NS; j += 4)
+                        s_dc[t * W::NP + state_at + j] = sum16_four(sc[j], sc[j + 1], sc[j + 2], sc[j + 3]);
                 }
-                s_y[t * W::WC + w.cl * CH + own_channel<CH>(w.r)] = sum_states<CH>(y);
+                lds_order();                               // (and the decays are formed again, not held in registers)
 #pragma unroll
-                for (int j = 0; j < NS; j += 4) sum16_x4(sc[j], sc[j + 1], sc[j + 2], sc[j + 3]);
-                if (w.cl == 0) {
+                for (int t = TT - 1; t >= 0; --t) {
+                    float dt[CH], dtx[CH], dc[CH], bv[NS], cv[NS], gb[CH], ta[CH], sb[NS];
+                    lds_read<CH>(s_dt + t * W::WC + w.cl * CH, dt);
+                    lds_read<CH>(s_dtx + t * W::WC + w.cl * CH, dtx);
+                    lds_read<CH>(s_g + t * W::WC + w.cl * CH, dc);
+                    lds_read<NS>(s_b + t * W::NP + w.r * NS, bv);
+                    lds_read<NS>(s_c + t * W::NP + w.r * NS, cv);
 #pragma unroll
-                    for (int j = 0; j < NS; ++j) s_dc[t * W::NP + w.r * NS + j] = sc[j];
-                }
-                __builtin_amdgcn_sched_barrier(0);         // (later tokens' LDS reads would take registers hist needs)
-            }
-            lds_order();                                   // (and the decays are formed again, not held in 128 registers)
+                    for (int j = 0; j < NS; ++j) sb[j] = 0.f;
 #pragma unroll
-            for (int t = TT - 1; t >= 0; --t) {
-                if (t == TT / 2 - 1) {                     // (the rows again, from L2: half of hist's registers are free now)
-                    w.fetch(A.x, b, t0, te, x);
-                    w.fetch(A.dt, b, t0, te, d);
-                    if (A.gate.p) w.fetch(A.gate, b, t0, te, z);
-                    w.fetch(A.dy, b, t0, te, gy);
-                }
-                float dt[CH], dtx[CH], dc[CH], bv[NS], cv[NS], gb[CH], ta[CH], sb[NS];
-                lds_read<CH>(s_dt + t * W::WC + w.cl * CH, dt);
-                lds_read<CH>(s_dtx + t * W::WC + w.cl * CH, dtx);
-                lds_read<CH>(s_g + t * W::WC + w.cl * CH, dc);
-                lds_read<NS>(s_b + t * W::NP + w.r * NS, bv);
-                lds_read<NS>(s_c + t * W::NP + w.r * NS, cv);
+                    for (int i = 0; i < CH; ++i) {
+                        gb[i] = ta[i] = 0.f;
 #pragma unroll
-                for (int j = 0; j < NS; ++j) sb[j] = 0.f;
-#pragma unroll
-                for (int i = 0; i < CH; ++i) {
-                    gb[i] = ta[i] = 0.f;
-#pragma unroll
-                    for (int j = 0; j < NS; ++j) {
-                        const float G = g[i][j] + dc[i] * cv[j];
-                        gb[i] += G * bv[j];
-                        sb[j] += G * dtx[i];
-                        g[i][j] = G * __builtin_amdgcn_exp2f(dt[i] * a2[i][j]);
-                        const float th = g[i][j] * hist[t][i][j];
-                        ta[i] += th * a2[i][j];
-                        da[i][j] += th * dt[i];
+                        for (int j = 0; j < NS; ++j) {
+                            const float G = g[i][j] + dc[i] * cv[j];
+                            gb[i] += G * bv[j];
+                            sb[j] += G * dtx[i];
+                            g[i][j] = G * __builtin_amdgcn_exp2f(dt[i] * a2[i][j]);
+                            const float th = g[i][j] * hist[t][i][j];
+                            ta[i] += th * a2[i][j];
+                            da[i][j] += th * dt[i];
+                        }
                     }
+                    // both sums over states at once: even rows receive gb's, odd rows ta's
+                    float both;
+                    if constexpr (CH == 2) both = swap_add16(swap_add32(gb[0], gb[1]), swap_add32(ta[0], ta[1]));
+                    else both = swap_add16(swap_add32(gb[0], gb[0]), swap_add32(ta[0], ta[0]));
+                    s_gt[(w.r & 1) * TILE + t * W::WC + w.cl * CH + (CH == 2 ? w.r >> 1 : 0)] = both;
+#pragma unroll
+                    for (int j = 0; j < NS; j += 4)
+                        s_db[t * W::NP + state_at + j] = sum16_four(sb[j], sb[j + 1], sb[j + 2], sb[j + 3]);
                 }
-                s_gb[t * W::WC + w.cl * CH + own_channel<CH>(w.r)] = sum_states<CH>(gb);
-                s_ta[t * W::WC + w.cl * CH + own_channel<CH>(w.r)] = sum_states<CH>(ta);
-#pragma unroll
-                for (int j = 0; j < NS; j += 4) sum16_x4(sb[j], sb[j + 1], sb[j + 2], sb[j + 3]);
-                if (w.cl == 0) {
-#pragma unroll
-                    for (int j = 0; j < NS; ++j) s_db[t * W::NP + w.r * NS + j] = sb[j];
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            lds_order();
-#pragma unroll
-            for (int k = 0; k < W::NBC; ++k) {
-                const int t = (k * 64 + w.lane) / W::NP, n = (k * 64 + w.lane) % W::NP;
-                const auto rs = buffer_of(
-                    A.part_bc + ((((long)(blk % A.nblk) * A.B + b) * A.L + t0) * A.G + w.g) * 2 * A.N, BUF_BYTES);
-                const unsigned at = t0 + t < te && n < A.N ? (t * A.G * 2 * A.N + n) * 4u : BUF_OUT;
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s_db[k * 64 + w.lane]), rs, at, 0, 0);
-                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s_dc[k * 64 + w.lane]), rs, at, A.N * 4, 0);
-            }
-            float dr[W::NV][VE], core[W::NV][VE];
-#pragma unroll
-            for (int k = 0; k < W::NV; ++k)
-#pragma unroll
-                for (int v = 0; v < VE; ++v) {
-                    const int at = w.trow(k) * W::WC + w.tcol(k) + v;
-                    dr[k][v] = s_ta[at] * LN2 + x[k].get(v) * s_gb[at];
-                    core[k][v] = s_y[at] + s_skip[w.tcol(k) + v] * x[k].get(v);
-                }
-            if (A.softplus) {                              // softplus' = sigmoid, from the side that does not overflow
+                lds_order();
+                float dr[W::NV][VE], core[W::NV][VE];
 #pragma unroll
                 for (int k = 0; k < W::NV; ++k)
 #pragma unroll
                     for (int v = 0; v < VE; ++v) {
-                        const float u = d[k].get(v) + s_bias[w.tcol(k) + v], e = exp_f(-fabsf(u));
-                        dr[k][v] *= (u < 0.f ? e : 1.f) * __builtin_amdgcn_rcpf(1.f + e);
+                        dr[k][v] = s_gt[TILE + w.tat(k) + v] * LN2 + x[k].get(v) * s_gt[w.tat(k) + v];
+                        core[k][v] = s_y[w.tat(k) + v] + s_skip[w.tcol(k) + v] * x[k].get(v);
                     }
-            }
-            if (A.gate.p) {
+                if (A.softplus) {                          // softplus' = sigmoid, from the side that does not overflow
+#pragma unroll
+                    for (int k = 0; k < W::NV; ++k)
+#pragma unroll
+                        for (int v = 0; v < VE; ++v) {
+                            const float u = d[k].get(v) + s_bias[w.tcol(k) + v], e = exp_f(-fabsf(u));
+                            dr[k][v] *= (u < 0.f ? e : 1.f) * __builtin_amdgcn_rcpf(1.f + e);
+                        }
+                }
+                if (A.gate.p) {
+#pragma unroll
+                    for (int k = 0; k < W::NV; ++k)
+#pragma unroll
+                        for (int v = 0; v < VE; ++v)
+                            z[k].set(v, w.staged(k, v, t0, te) ? gy[k].get(v) * core[k][v] * dsilu_f(z[k].get(v)) : 0.f);
+                    w.put(A.dgate, b, A.L, A.D, t0, tend, z);
+                }
 #pragma unroll
                 for (int k = 0; k < W::NV; ++k)
 #pragma unroll
-                    for (int v = 0; v < VE; ++v)
-                        z[k].set(v, w.staged(k, v, t0, te) ? gy[k].get(v) * core[k][v] * dsilu_f(z[k].get(v)) : 0.f);
-                w.put(A.dgate, b, A.L, A.D, t0, tend, z);
+                    for (int v = 0; v < VE; ++v) {
+                        const bool on = w.staged(k, v, t0, te);
+                        const float dc = s_g[w.tat(k) + v], e = on ? dr[k][v] : 0.f;
+                        sum_skip[k][v] += on ? dc * x[k].get(v) : 0.f;
+                        sum_bias[k][v] += e;
+                        x[k].set(v, on ? s_dt[w.tat(k) + v] * s_gt[w.tat(k) + v] + s_skip[w.tcol(k) + v] * dc : 0.f);
+                        d[k].set(v, e);
+                    }
+                w.put(A.dx, b, A.L, A.D, t0, tend, x);
+                w.put(A.ddt, b, A.L, A.D, t0, tend, d);
             }
+            __syncthreads();                               // every wave's s_db, s_dc are there; b and c have been read
+            const auto rs = buffer_of(
+                A.part_bc + ((((long)(blk % A.bblk) * A.B + b) * A.L + t0) * A.G + w.g) * 2 * A.N, BUF_BYTES);
 #pragma unroll
-            for (int k = 0; k < W::NV; ++k)
+            for (int k = 0; k < NBC; ++k) {
+                const int id = k * 64 * BW + threadIdx.x, t = id % SH / W::NP, n = id % W::NP;
+                float s = 0.f;
 #pragma unroll
-                for (int v = 0; v < VE; ++v) {
-                    const int at = w.trow(k) * W::WC + w.tcol(k) + v;
-                    const bool on = w.staged(k, v, t0, te);
-                    const float dc = s_g[at], e = on ? dr[k][v] : 0.f;
-                    s_sum[0][(k * 64 + w.lane) * VE + v] += on ? dc * x[k].get(v) : 0.f;
-                    s_sum[1][(k * 64 + w.lane) * VE + v] += e;
-                    x[k].set(v, on ? s_dt[at] * s_gb[at] + s_skip[w.tcol(k) + v] * dc : 0.f);
-                    d[k].set(v, e);
-                }
-            w.put(A.dx, b, A.L, A.D, t0, tend, x);
-            w.put(A.ddt, b, A.L, A.D, t0, tend, d);
+                for (int u = 0; u < BW; ++u) s += s_part[u][id];
+                __builtin_amdgcn_raw_buffer_store_b32(
+                    __float_as_uint(s), rs,
+                    t0 + t < te && n < A.N ? ((t * A.G * 2 + (id < SH ? 0 : 1)) * A.N + n) * 4u : BUF_OUT, 0, 0);
+            }
         }
-        if (A.dstate && seg == 0) w.store_state(A.dstate, b, A.D, A.N, g);
+        if (A.dstate && seg == 0) w.store_public(A.dstate, b, A.D, A.N, g);
     }
-    float* out = A.part_p + (((long)group * A.segs + seg) * blks + blk) * (LANE_STATE + 2 * W::WC);
-    w.store_own(out, da);
+    if (!live) return;                                     // (no barrier follows)
+    float* out = A.part_p + ((long)group * A.segs + seg) * chans * (W::NP + 2);
+    w.store_own(out + (long)w.p0 * W::NP, da);
     // sums over the tokens of a tile: lanes that staged the same channels meet in LDS
     for (int half = 0; half < 2; ++half) {
         lds_order();
 #pragma unroll
         for (int k = 0; k < W::NV; ++k)
 #pragma unroll
-            for (int v = 0; v < VE; ++v)
-                s_dt[w.trow(k) * W::WC + w.tcol(k) + v] = s_sum[half][(k * 64 + w.lane) * VE + v];
+            for (int v = 0; v < VE; ++v) s_dt[w.tat(k) + v] = half ? sum_bias[k][v] : sum_skip[k][v];
         lds_order();
-        if (w.lane < W::WC) {
+        if (w.lane < W::WC && w.c0 + w.lane < w.cend) {
             float s = 0.f;
 #pragma unroll
             for (int t = 0; t < TT; ++t) s += s_dt[t * W::WC + w.lane];
-            out[LANE_STATE + half * W::WC + w.lane] = s;
+            out[chans * (W::NP + half) + w.p0 + w.lane] = s;
         }
     }
 }
 
 // part_p's rows summed in a fixed order (16 row lanes x 64 columns) and put in their public places.
-template <int CH, int NS>
-__global__ __launch_bounds__(1024) void scan_params(const float* __restrict__ part, int rows, int D, int N, int G,
-                                                    int nblk, float* __restrict__ da, float* __restrict__ dskip,
+template <int NP>
+__global__ __launch_bounds__(1024) void scan_params(const float* __restrict__ part, int rows, int per, int per_pad, int N,
+                                                    int G, float* __restrict__ da, float* __restrict__ dskip,
                                                     float* __restrict__ dbias) {
-    constexpr int WC = 16 * CH, PER = LANE_STATE + 2 * WC;
-    const long cols = (long)nblk * G * PER, col = (long)blockIdx.x * 64 + (threadIdx.x & 63);
+    const long chans = (long)G * per_pad, cols = chans * (NP + 2), col = (long)blockIdx.x * 64 + (threadIdx.x & 63);
     const int lr = threadIdx.x >> 6;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
     if (col < cols)
@@ -689,19 +720,15 @@ __global__ __launch_bounds__(1024) void scan_params(const float* __restrict__ pa
     float t = 0.f;
 #pragma unroll
     for (int u = 0; u < 16; ++u) t += s[u][threadIdx.x];
-    const int blk = (int)(col / PER), e = (int)(col % PER), per = D / G, g = blk / nblk;
-    const int c0 = g * per + blk % nblk * WC, cend = (g + 1) * per;
-    if (e < LANE_STATE) {
-        const int v = e / 256, lane = e / 4 % 64, k = v * 4 + e % 4;       // element k of the lane's CH x NS states
-        const int c = c0 + (lane & 15) * CH + k / NS, n = (lane >> 4) * NS + k % NS;
-        if (c < cend && n < N) da[(long)c * N + n] = t;
-    } else {
-        const int q = e - LANE_STATE, c = c0 + q % WC;
-        if (c < cend) {
-            if (q < WC) { if (dskip) dskip[c] = t; }
-            else if (dbias) dbias[c] = t;
-        }
-    }
+    const bool is_a = col < chans * NP;
+    const long p = is_a ? col / NP : (col - chans * NP) % chans;
+    if (p % per_pad >= per) return;                        // (a place between two groups)
+    const long c = p / per_pad * per + p % per_pad;
+    if (is_a) {
+        if (col % NP < N) da[c * N + col % NP] = t;
+    } else if (col < chans * (NP + 1)) {
+        if (dskip) dskip[c] = t;
+    } else if (dbias) dbias[c] = t;
 }
 
 // db and dc: the channel blocks' shares in a fixed order; rows past a sequence's length are 0
@@ -780,35 +807,36 @@ __global__ __launch_bounds__(256) void scan_token(Rows x, float* __restrict__ st
     }
 }
 
-// Channels a lane holds: CH x NS = 16 values, NS states a lane over 4 rows.
-int ch_of(int N) { return N <= 16 ? 4 : N <= 32 ? 2 : 1; }
-int blocks_of(int D, int G, int N) { return (D / G + 16 * ch_of(N) - 1) / (16 * ch_of(N)); }
+// Padded states, and channels of a forward wave and of a backward workgroup.
+int np_of(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : 64; }
+int fwd_channels(int N) { return N <= 16 ? 64 : N <= 32 ? 32 : 16; }
+int bwd_channels(int N) { return N <= 16 ? 32 * BW : 16 * BW; }
 
 // Segments: none while the waves of whole sequences keep the chip's 1024 SIMDs busy; else enough for some 4096 waves, each
 // of 8 tiles at least.
-void cut(int B, int L, int D, int G, int N, int& segs, int& seg_len) {
-    const long waves = (long)B * G * blocks_of(D, G, N);
+void plan(Args& A) {
+    A.per = A.D / A.G;
+    A.fblk = (A.per + fwd_channels(A.N) - 1) / fwd_channels(A.N);
+    A.bblk = (A.per + bwd_channels(A.N) - 1) / bwd_channels(A.N);
+    A.per_pad = A.bblk * bwd_channels(A.N);
+    const long waves = (long)A.B * A.G * A.fblk;
     long s = waves >= 1024 ? 1 : 4096 / waves;
-    const long most = L / (8 * TT);
+    const long most = A.L / (8 * TT);
     if (s > most) s = most;
     if (s < 1) s = 1;
-    long len = (L + s - 1) / s;
+    long len = (A.L + s - 1) / s;
     len = (len + TT - 1) / TT * TT;
-    seg_len = (int)len;
-    segs = (int)((L + len - 1) / len);
-}
-int batch_groups(int B, int L, int D, int G, int N) {
-    int segs, len;
-    cut(B, L, D, G, N, segs, len);
-    const long waves = (long)G * blocks_of(D, G, N) * segs;
-    const long g = 4096 / waves;
-    return (int)(g < 1 ? 1 : g > B ? B : g);
+    A.seg_len = (int)len;
+    A.segs = (int)((A.L + len - 1) / len);
+    // the backward's sums over tokens leave a workgroup once: as few workgroups as still fill the chip
+    const long g = 1024 / ((long)A.G * A.bblk * A.segs);
+    A.bgroups = (int)(g < 1 ? 1 : g > A.B ? A.B : g);
 }
 
 bool bad_shape(int dtype, int B, int L, int D, int N, int G) {
     return !vqa_dtype_ok(dtype) || B < 1 || L < 1 || L > 0x3fffffff || D < 1 || N < 1 || N > 64 || G < 1 || D % G != 0 ||
-           (double)B * L > 1e9 || (double)B * L * D > 4e11 || (double)B * D > 1e10 || (double)B * L * G * N > 1e11 ||
-           (double)G * blocks_of(D, G, N) * B > 2e8;
+           (double)B * L > 1e9 || (double)B * L * D > 4e11 || (double)B * D > 1e9 || (double)B * L * G * N > 1e11 ||
+           (double)G * (D / G + 128) * B > 2e9;
 }
 // (buffer accesses of up to 16 bytes want their addresses on 4 bytes)
 bool on4(const void* p, long stride, int e) { return ((uintptr_t)p & 3) == 0 && stride * e % 4 == 0; }
@@ -820,53 +848,48 @@ bool far_rows(const Args& A) {
 }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-template <typename T, int CH, int NS, int VE> int launch(int kind, const Args& A, hipStream_t st) {
-    const long blks = (long)A.nblk * A.G;
-    if (kind == 0) {
-        if (A.segs > 1) {
-            scan_fwd<T, CH, NS, VE, false><<<(unsigned)(blks * A.segs * A.B), 64, 0, st>>>(A);
-            CHECK_LAUNCH();
-            scan_chain<CH, NS, false><<<(unsigned)(blks * A.B * 4), 64, 0, st>>>(A);
-            CHECK_LAUNCH();
-        }
-        scan_fwd<T, CH, NS, VE, true><<<(unsigned)(blks * A.segs * A.B), 64, 0, st>>>(A);
-    } else {
-        if (A.segs > 1) {
-            scan_bwd_ends<T, CH, NS, VE><<<(unsigned)(blks * A.segs * A.B), 64, 0, st>>>(A);
-            CHECK_LAUNCH();
-            scan_chain<CH, NS, true><<<(unsigned)(blks * A.B * 4), 64, 0, st>>>(A);
-            CHECK_LAUNCH();
-        }
-        scan_bwd<T, CH, NS, VE><<<(unsigned)(blks * A.segs * A.bgroups), 64, 0, st>>>(A);
-    }
+// Workspaces, in floats: the segments' states and sums of dt (none without segments), the backward's partial sums
+long seg_floats(const Args& A) {
+    return A.segs > 1 ? (long)A.B * A.segs * A.G * A.per_pad * (np_of(A.N) + 1) : 0;
+}
+float* seg_dt_of(const Args& A, float* ws) { return ws + (long)A.B * A.segs * A.G * A.per_pad * np_of(A.N); }
+long part_p_floats(const Args& A) { return (long)A.bgroups * A.segs * A.G * A.per_pad * (np_of(A.N) + 2); }
+long part_bc_floats(const Args& A) { return (long)A.bblk * A.B * A.L * A.G * 2 * A.N; }
+
+template <int NP, bool REV> int chain(const Args& A, hipStream_t st) {
+    const long n = (long)A.B * A.G * A.per_pad * (NP / 4);
+    scan_chain<NP, REV><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(A);
     CHECK_LAUNCH();
     return VQA_OK;
 }
-template <typename T> int by_states(int kind, bool vec, const Args& A, hipStream_t st) {
-    constexpr int V = 16 / sizeof(T);
-    if (A.N <= 16) return vec ? launch<T, 4, 4, V>(kind, A, st) : launch<T, 4, 4, 1>(kind, A, st);
-    if (A.N <= 32) return vec ? launch<T, 2, 8, 4>(kind, A, st) : launch<T, 2, 8, 1>(kind, A, st);
-    return vec ? launch<T, 1, 16, 2>(kind, A, st) : launch<T, 1, 16, 1>(kind, A, st);
-}
-int by_type(int kind, int dtype, bool vec, const Args& A, hipStream_t st) {
-    if (dtype == VQA_F32) return by_states<float>(kind, vec, A, st);
-    if (dtype == VQA_BF16) return by_states<bf16>(kind, vec, A, st);
-    return by_states<_Float16>(kind, vec, A, st);
-}
 
-void plan(Args& A) {
-    A.nblk = blocks_of(A.D, A.G, A.N);
-    cut(A.B, A.L, A.D, A.G, A.N, A.segs, A.seg_len);
-    A.bgroups = batch_groups(A.B, A.L, A.D, A.G, A.N);
+// CH, VE: the forward's channels a lane and elements a load; BCH, BVE: the backward's
+template <typename T, int NS, int CH, int VE, int BCH, int BVE> int launch(bool bwd, const Args& A, hipStream_t st) {
+    const unsigned waves = (unsigned)((long)A.fblk * A.G * A.segs * A.B);
+    int rc = VQA_OK;
+    if (A.segs > 1) {
+        if (bwd) scan_bwd_ends<T, CH, NS, VE><<<waves, 64, 0, st>>>(A);
+        else scan_fwd<T, CH, NS, VE, false><<<waves, 64, 0, st>>>(A);
+        CHECK_LAUNCH();
+        rc = bwd ? chain<4 * NS, true>(A, st) : chain<4 * NS, false>(A, st);
+        if (rc != VQA_OK) return rc;
+    }
+    if (bwd) scan_bwd<T, BCH, NS, BVE><<<(unsigned)((long)A.bblk * A.G * A.segs * A.bgroups), 64 * BW, 0, st>>>(A);
+    else scan_fwd<T, CH, NS, VE, true><<<waves, 64, 0, st>>>(A);
+    CHECK_LAUNCH();
+    return VQA_OK;
 }
-// Workspace, in floats: the segments' states and sums of dt (none without segments), the backward's partial sums
-long seg_floats(const Args& A) {
-    return A.segs > 1 ? (long)A.B * A.nblk * A.G * A.segs * (LANE_STATE + 16 * ch_of(A.N)) : 0;
+template <typename T> int by_states(bool bwd, bool vec, const Args& A, hipStream_t st) {
+    constexpr int V = 16 / sizeof(T);
+    if (A.N <= 16) return vec ? launch<T, 4, 4, V, 2, 4>(bwd, A, st) : launch<T, 4, 4, 1, 2, 1>(bwd, A, st);
+    if (A.N <= 32) return vec ? launch<T, 8, 2, 4, 1, 2>(bwd, A, st) : launch<T, 8, 2, 1, 1, 1>(bwd, A, st);
+    return vec ? launch<T, 16, 1, 2, 1, 2>(bwd, A, st) : launch<T, 16, 1, 1, 1, 1>(bwd, A, st);
 }
-long part_p_floats(const Args& A) {
-    return (long)A.bgroups * A.segs * A.nblk * A.G * (LANE_STATE + 32 * ch_of(A.N));
+int by_type(bool bwd, int dtype, bool vec, const Args& A, hipStream_t st) {
+    if (dtype == VQA_F32) return by_states<float>(bwd, vec, A, st);
+    if (dtype == VQA_BF16) return by_states<bf16>(bwd, vec, A, st);
+    return by_states<_Float16>(bwd, vec, A, st);
 }
-long part_bc_floats(const Args& A) { return (long)A.nblk * A.B * A.L * A.G * 2 * A.N; }
 
 }  // namespace
 
@@ -876,7 +899,7 @@ extern "C" int vqa_scan_ws_bytes(int dtype, int B, int L, int D, int N, int G, l
     A.B = B; A.L = L; A.D = D; A.N = N; A.G = G;
     plan(A);
     sizes[0] = 4 * seg_floats(A);
-    sizes[1] = 4L * B * A.nblk * G * ((L + TT - 1) / TT) * LANE_STATE;
+    sizes[1] = 4L * B * ((L + TT - 1) / TT) * G * A.per_pad * np_of(N);
     sizes[2] = 4 * (seg_floats(A) + part_p_floats(A) + part_bc_floats(A));
     return VQA_OK;
 }
@@ -896,11 +919,10 @@ extern "C" int vqa_scan_fwd(void* stream, int dtype, const void* x, long x_batch
     plan(A);
     if ((A.segs > 1 && !ws) || !aligned16(ws) || !aligned16(keep) || far_rows(A)) return VQA_ERR_ARG;
     A.seg_h = ws;
-    A.seg_dt = ws ? ws + (long)B * A.nblk * G * A.segs * LANE_STATE : nullptr;
+    A.seg_dt = ws ? seg_dt_of(A, ws) : nullptr;
     const int e = vqa_elem_bytes(dtype);
-    const bool vec = (D / G) % (16 / e) == 0 && rows_vec(A.x, e) && rows_vec(A.dt, e) && rows_vec(A.gate, e) &&
-                     on4(y, D, e);
-    return by_type(0, dtype, vec, A, static_cast<hipStream_t>(stream));
+    const bool vec = A.per % (16 / e) == 0 && rows_vec(A.x, e) && rows_vec(A.dt, e) && rows_vec(A.gate, e) && on4(y, D, e);
+    return by_type(false, dtype, vec, A, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int vqa_scan_bwd(void* stream, int dtype, const void* dy, long dy_batch, long dy_row, const float* dlast,
@@ -923,26 +945,28 @@ extern "C" int vqa_scan_bwd(void* stream, int dtype, const void* dy, long dy_bat
     if (far_rows(A)) return VQA_ERR_ARG;
     plan(A);
     A.seg_h = ws;
-    A.seg_dt = ws + (A.segs > 1 ? (long)B * A.nblk * G * A.segs * LANE_STATE : 0);
+    A.seg_dt = seg_dt_of(A, ws);
     A.part_p = ws + seg_floats(A);
     A.part_bc = A.part_p + part_p_floats(A);
     const int e = vqa_elem_bytes(dtype);
-    const bool vec = (D / G) % (16 / e) == 0 && rows_vec(A.x, e) && rows_vec(A.dt, e) && rows_vec(A.gate, e) &&
+    const bool vec = A.per % (16 / e) == 0 && rows_vec(A.x, e) && rows_vec(A.dt, e) && rows_vec(A.gate, e) &&
                      rows_vec(A.dy, e) && on4(dx, D, e) && on4(ddt, D, e) && on4(dgate, D, e);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const int rc = by_type(1, dtype, vec, A, st);
+    const int rc = by_type(true, dtype, vec, A, st);
     if (rc != VQA_OK) return rc;
-    const int rows = A.bgroups * A.segs;
-    const long cols = (long)A.nblk * G * (LANE_STATE + 32 * ch_of(N));
-    const unsigned pg = (unsigned)((cols + 63) / 64);
-    if (N <= 16) scan_params<4, 4><<<pg, 1024, 0, st>>>(A.part_p, rows, D, N, G, A.nblk, da, dskip, ddt_bias);
-    else if (N <= 32) scan_params<2, 8><<<pg, 1024, 0, st>>>(A.part_p, rows, D, N, G, A.nblk, da, dskip, ddt_bias);
-    else scan_params<1, 16><<<pg, 1024, 0, st>>>(A.part_p, rows, D, N, G, A.nblk, da, dskip, ddt_bias);
+    const int rows = A.bgroups * A.segs, np = np_of(N);
+    const unsigned pg = (unsigned)(((long)G * A.per_pad * (np + 2) + 63) / 64);
+    if (np == 16) scan_params<16><<<pg, 1024, 0, st>>>(A.part_p, rows, A.per, A.per_pad, N, G, da, dskip, ddt_bias);
+    else if (np == 32) scan_params<32><<<pg, 1024, 0, st>>>(A.part_p, rows, A.per, A.per_pad, N, G, da, dskip, ddt_bias);
+    else scan_params<64><<<pg, 1024, 0, st>>>(A.part_p, rows, A.per, A.per_pad, N, G, da, dskip, ddt_bias);
     CHECK_LAUNCH();
     const unsigned sg = (unsigned)(((long)B * L * G * 2 * N + 255) / 256);
-    if (dtype == VQA_F32) scan_shared<float><<<sg, 256, 0, st>>>(A.part_bc, lengths, B, L, G, N, A.nblk, static_cast<float*>(db), static_cast<float*>(dc));
-    else if (dtype == VQA_BF16) scan_shared<bf16><<<sg, 256, 0, st>>>(A.part_bc, lengths, B, L, G, N, A.nblk, static_cast<bf16*>(db), static_cast<bf16*>(dc));
-    else scan_shared<_Float16><<<sg, 256, 0, st>>>(A.part_bc, lengths, B, L, G, N, A.nblk, static_cast<_Float16*>(db), static_cast<_Float16*>(dc));
+    if (dtype == VQA_F32)
+        scan_shared<float><<<sg, 256, 0, st>>>(A.part_bc, lengths, B, L, G, N, A.bblk, static_cast<float*>(db), static_cast<float*>(dc));
+    else if (dtype == VQA_BF16)
+        scan_shared<bf16><<<sg, 256, 0, st>>>(A.part_bc, lengths, B, L, G, N, A.bblk, static_cast<bf16*>(db), static_cast<bf16*>(dc));
+    else
+        scan_shared<_Float16><<<sg, 256, 0, st>>>(A.part_bc, lengths, B, L, G, N, A.bblk, static_cast<_Float16*>(db), static_cast<_Float16*>(dc));
     CHECK_LAUNCH();
     return VQA_OK;
 }
