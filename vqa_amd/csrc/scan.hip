@@ -164,23 +164,32 @@ template <typename T, int CH, int NS, int VE> struct Wave {
                 a2[i][j] = channel(i) < cend && n < A.N ? A.a[(long)channel(i) * A.N + n] * LOG2E : 0.f;
             }
     }
-    // a state in its public layout [B][D][N]
+    // a state in its public layout [B][D][N].  (The lane is hidden from the compiler: these run once a sequence, and their
+    // addresses and masks, known before the loop over tiles, would be kept in registers all through it.)
+    __device__ __forceinline__ unsigned public_place(int l, int i, int j, int N) const {
+        const int off = (l & 15) * CH + i, n = (l >> 4) * NS + j;
+        return c0 + off < cend && n < N ? (unsigned)(off * N + n) * 4u : BUF_OUT;
+    }
     __device__ __forceinline__ void load_public(const float* s, int b, int D, int N, float (&h)[CH][NS]) const {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        const auto rs = buffer_of(s + ((long)b * D + c0) * N, s ? BUF_BYTES : 0);
 #pragma unroll
         for (int i = 0; i < CH; ++i)
 #pragma unroll
-            for (int j = 0; j < NS; ++j) {
-                const int n = r * NS + j;
-                h[i][j] = s && channel(i) < cend && n < N ? s[((long)b * D + channel(i)) * N + n] : 0.f;
-            }
+            for (int j = 0; j < NS; ++j) h[i][j] = buf_load<float, 1>(rs, public_place(l, i, j, N)).get(0);
     }
     __device__ __forceinline__ void store_public(float* s, int b, int D, int N, const float (&h)[CH][NS]) const {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        const auto rs = buffer_of(s + ((long)b * D + c0) * N, BUF_BYTES);
 #pragma unroll
         for (int i = 0; i < CH; ++i)
 #pragma unroll
             for (int j = 0; j < NS; ++j) {
-                const int n = r * NS + j;
-                if (channel(i) < cend && n < N) s[((long)b * D + channel(i)) * N + n] = h[i][j];
+                Raw<float, 1> f;
+                f.set(0, h[i][j]);
+                buf_store<float, 1>(rs, public_place(l, i, j, N), f);
             }
     }
     // ... and in a workspace: p = its first channel's place in it.  Channels past the end: 0, nothing
@@ -285,12 +294,11 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
         if (A.segs > 1) w.load_own(A.seg_h + at_seg * W::NP, h);
         else w.load_public(A.state, b, A.D, A.N, h);
     }
-    Raw<T, VE> x[W::NV], d[W::NV], z[W::NV], xn[W::NV], dn[W::NV], zn[W::NV];
+    Raw<T, VE> x[W::NV], d[W::NV], z[W::NV], xn[W::NV], dn[W::NV];
     Raw<T, 1> bn[NBC], cn[NBC];
     auto fetch = [&](int t0) {
         w.fetch(A.x, b, t0, live, xn);
         w.fetch(A.dt, b, t0, live, dn);
-        if (FULL && A.gate.p) w.fetch(A.gate, b, t0, live, zn);
 #pragma unroll
         for (int k = 0; k < NBC; ++k) {
             bn[k] = fetch_shared<T, W::NP>(A.b, b, t0, live, w.g, A.N, k * 64 + w.lane);
@@ -307,7 +315,7 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
             continue;
         }
 #pragma unroll
-        for (int k = 0; k < W::NV; ++k) { x[k] = xn[k]; d[k] = dn[k]; if (FULL) z[k] = zn[k]; }
+        for (int k = 0; k < W::NV; ++k) { x[k] = xn[k]; d[k] = dn[k]; }
         lds_order();                                       // (the last tile's reads are done)
         float step[W::NV][VE];
         stage_steps(w, d, s_bias, A.softplus, t0, live, step);
@@ -324,6 +332,7 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
             if (FULL) s_c[k * 64 + w.lane] = cn[k].get(0);
         }
         lds_order();
+        if (FULL && A.gate.p) w.fetch(A.gate, b, t0, live, z);
         if (t0 + TT < te) fetch(t0 + TT);
         if (FULL && A.keep) w.store_own(A.keep + (((long)b * ntile + t0 / TT) * chans + w.p0) * W::NP, h);
 #pragma unroll
