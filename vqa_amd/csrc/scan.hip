@@ -50,8 +50,7 @@ __device__ __forceinline__ void lds_order() {
 
 // log(1 + exp(v)) to relative precision on both sides: log1p(e) = 2 atanh(e / (2 + e)) as its series (e <= 1, so the
 // argument is at most 1/3 and the next term under 2e-8 of the sum)
-__device__ __forceinline__ float softplus_f(float v) {
-    const float e = exp_f(-fabsf(v));
+__device__ __forceinline__ float softplus_f(float v, float e) {          // e = exp(-|v|)
     const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
     float p = 1.f / 13.f;
     p = p * q + 1.f / 11.f;
@@ -232,38 +231,34 @@ __device__ __forceinline__ Raw<T, 1> fetch_shared(const Rows& R, int b, int t0, 
 __device__ __forceinline__ int length_of(const Args& A, int b) {
     return A.lengths ? max(0, min(A.L, A.lengths[b])) : A.L;
 }
-// dt of staged raw values; 0 past the end (a token that moves no state) and past the channels
-template <typename W, typename R, int NV, int VE>
+// dt of staged raw values, 0 past the end (a token that moves no state); slope: its derivative, softplus' = sigmoid.  What
+// a channel past the group's end has here is finite and meets only zeros.
+template <bool SLOPE, typename W, typename R, int NV, int VE>
 __device__ __forceinline__ void stage_steps(const W& w, const R (&d)[NV], const float* s_bias, int softplus, int t0, int te,
-                                            float (&dt)[NV][VE]) {
+                                            float (&dt)[NV][VE], float (&slope)[NV][VE]) {
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
-        for (int v = 0; v < VE; ++v) dt[k][v] = d[k].get(v) + s_bias[w.tcol(k) + v];
+        for (int v = 0; v < VE; ++v) {
+            dt[k][v] = d[k].get(v) + s_bias[w.tcol(k) + v];
+            if (SLOPE) slope[k][v] = 1.f;
+        }
     if (softplus) {
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
-            for (int v = 0; v < VE; ++v) dt[k][v] = softplus_f(dt[k][v]);
+            for (int v = 0; v < VE; ++v) {
+                const float u = dt[k][v], e = exp_f(-fabsf(u));
+                dt[k][v] = softplus_f(u, e);
+                if (SLOPE) slope[k][v] = (u < 0.f ? e : 1.f) * __builtin_amdgcn_rcpf(1.f + e);
+            }
     }
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int v = 0; v < VE; ++v)
-            if (t0 + w.trow(k) >= te || w.c0 + w.tcol(k) + v >= w.cend) dt[k][v] = 0.f;
-}
-// dy silu(gate)
-template <typename W, typename R, int NV, int VE>
-__device__ __forceinline__ void stage_core(const R (&gy)[NV], const R (&z)[NV], bool gated, float (&dc)[NV][VE]) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int v = 0; v < VE; ++v) dc[k][v] = gy[k].get(v);
-    if (gated) {
+    if (t0 + TT > te) {                                    // (the last tile of a sequence)
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
-            for (int v = 0; v < VE; ++v) dc[k][v] *= silu_f(z[k].get(v));
+            for (int v = 0; v < VE; ++v)
+                if (t0 + w.trow(k) >= te) dt[k][v] = 0.f;
     }
 }
 
@@ -318,7 +313,7 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
         for (int k = 0; k < W::NV; ++k) { x[k] = xn[k]; d[k] = dn[k]; }
         lds_order();                                       // (the last tile's reads are done)
         float step[W::NV][VE];
-        stage_steps(w, d, s_bias, A.softplus, t0, live, step);
+        stage_steps<false>(w, d, s_bias, A.softplus, t0, live, step, step);
 #pragma unroll
         for (int k = 0; k < W::NV; ++k)
 #pragma unroll
@@ -367,9 +362,11 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
                     for (int v = 0; v < VE; ++v) step[k][v] *= silu_f(z[k].get(v));
             }
 #pragma unroll
-            for (int k = 0; k < W::NV; ++k)
+            for (int k = 0; k < W::NV; ++k) {
 #pragma unroll
-                for (int v = 0; v < VE; ++v) d[k].set(v, t0 + w.trow(k) < len ? step[k][v] : 0.f);
+                for (int v = 0; v < VE; ++v) d[k].set(v, step[k][v]);
+                if (t0 + TT > len && t0 + w.trow(k) >= len) d[k].zero();
+            }
             w.put(A.y, b, A.L, A.D, t0, te, d);
         }
     }
@@ -459,8 +456,17 @@ __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
     for (; te > ts && t0 >= ts; t0 -= TT) {
         lds_order();
         float step[W::NV][VE], dcore[W::NV][VE];
-        stage_steps(w, dn, s_bias, A.softplus, t0, te, step);
-        stage_core<W>(gn, zn, A.gate.p != nullptr, dcore);
+        stage_steps<false>(w, dn, s_bias, A.softplus, t0, te, step, step);
+#pragma unroll
+        for (int k = 0; k < W::NV; ++k)
+#pragma unroll
+            for (int v = 0; v < VE; ++v) dcore[k][v] = gn[k].get(v);
+        if (A.gate.p) {
+#pragma unroll
+            for (int k = 0; k < W::NV; ++k)
+#pragma unroll
+                for (int v = 0; v < VE; ++v) dcore[k][v] *= silu_f(zn[k].get(v));
+        }
 #pragma unroll
         for (int k = 0; k < W::NV; ++k)
 #pragma unroll
@@ -557,10 +563,22 @@ __global__ __launch_bounds__(64 * BW) void scan_bwd(Args A) {
                 const int id = k * 64 * BW + threadIdx.x;
                 s_bc[id] = fetch_shared<T, W::NP>(id < SH ? A.b : A.c, b, t0, te, w.g, A.N, id % SH).get(0);
             }
+            float step[W::NV][VE], slope[W::NV][VE], sig[W::NV][VE], dcore[W::NV][VE];
             if (live) {
-                float step[W::NV][VE], dcore[W::NV][VE];
-                stage_steps(w, d, s_bias, A.softplus, t0, te, step);
-                stage_core<W>(gy, z, A.gate.p != nullptr, dcore);
+                stage_steps<true>(w, d, s_bias, A.softplus, t0, te, step, slope);
+#pragma unroll
+                for (int k = 0; k < W::NV; ++k)
+#pragma unroll
+                    for (int v = 0; v < VE; ++v) dcore[k][v] = gy[k].get(v);
+                if (A.gate.p) {
+#pragma unroll
+                    for (int k = 0; k < W::NV; ++k)
+#pragma unroll
+                        for (int v = 0; v < VE; ++v) {
+                            sig[k][v] = sigmoid_f(z[k].get(v));
+                            dcore[k][v] *= z[k].get(v) * sig[k][v];
+                        }
+                }
 #pragma unroll
                 for (int k = 0; k < W::NV; ++k)
 #pragma unroll
@@ -633,42 +651,33 @@ __global__ __launch_bounds__(64 * BW) void scan_bwd(Args A) {
                         s_db[t * W::NP + state_at + j] = sum16_four(sb[j], sb[j + 1], sb[j + 2], sb[j + 3]);
                 }
                 lds_order();
-                float dr[W::NV][VE], core[W::NV][VE];
-#pragma unroll
-                for (int k = 0; k < W::NV; ++k)
-#pragma unroll
-                    for (int v = 0; v < VE; ++v) {
-                        dr[k][v] = s_gt[TILE + w.tat(k) + v] * LN2 + x[k].get(v) * s_gt[w.tat(k) + v];
-                        core[k][v] = s_y[w.tat(k) + v] + s_skip[w.tcol(k) + v] * x[k].get(v);
-                    }
-                if (A.softplus) {                          // softplus' = sigmoid, from the side that does not overflow
-#pragma unroll
-                    for (int k = 0; k < W::NV; ++k)
-#pragma unroll
-                        for (int v = 0; v < VE; ++v) {
-                            const float u = d[k].get(v) + s_bias[w.tcol(k) + v], e = exp_f(-fabsf(u));
-                            dr[k][v] *= (u < 0.f ? e : 1.f) * __builtin_amdgcn_rcpf(1.f + e);
-                        }
-                }
                 if (A.gate.p) {
 #pragma unroll
-                    for (int k = 0; k < W::NV; ++k)
+                    for (int k = 0; k < W::NV; ++k) {
 #pragma unroll
-                        for (int v = 0; v < VE; ++v)
-                            z[k].set(v, w.staged(k, v, t0, te) ? gy[k].get(v) * core[k][v] * dsilu_f(z[k].get(v)) : 0.f);
+                        for (int v = 0; v < VE; ++v) {
+                            const float core = s_y[w.tat(k) + v] + s_skip[w.tcol(k) + v] * x[k].get(v);
+                            z[k].set(v, gy[k].get(v) * core * sig[k][v] * (1.f + z[k].get(v) * (1.f - sig[k][v])));
+                        }
+                        if (t0 + TT > te && t0 + w.trow(k) >= te) z[k].zero();
+                    }
                     w.put(A.dgate, b, A.L, A.D, t0, tend, z);
                 }
 #pragma unroll
-                for (int k = 0; k < W::NV; ++k)
+                for (int k = 0; k < W::NV; ++k) {
+                    const bool past = t0 + TT > te && t0 + w.trow(k) >= te;
 #pragma unroll
                     for (int v = 0; v < VE; ++v) {
-                        const bool on = w.staged(k, v, t0, te);
-                        const float dc = s_g[w.tat(k) + v], e = on ? dr[k][v] : 0.f;
-                        sum_skip[k][v] += on ? dc * x[k].get(v) : 0.f;
-                        sum_bias[k][v] += e;
-                        x[k].set(v, on ? s_dt[w.tat(k) + v] * s_gt[w.tat(k) + v] + s_skip[w.tcol(k) + v] * dc : 0.f);
-                        d[k].set(v, e);
+                        const float gb = s_gt[w.tat(k) + v], xv = x[k].get(v);
+                        float dr = (s_gt[TILE + w.tat(k) + v] * LN2 + xv * gb) * slope[k][v];
+                        if (past) dr = 0.f;
+                        sum_bias[k][v] += dr;
+                        sum_skip[k][v] += past ? 0.f : dcore[k][v] * xv;
+                        d[k].set(v, dr);
+                        x[k].set(v, step[k][v] * gb + s_skip[w.tcol(k) + v] * dcore[k][v]);
                     }
+                    if (past) x[k].zero();
+                }
                 w.put(A.dx, b, A.L, A.D, t0, tend, x);
                 w.put(A.ddt, b, A.L, A.D, t0, tend, d);
             }
@@ -793,7 +802,7 @@ __global__ __launch_bounds__(256) void scan_token(Rows x, float* __restrict__ st
     }
     const float xv = to_f32(static_cast<const T*>(x.p)[bi * x.batch + d]);
     float step = to_f32(static_cast<const T*>(dt.p)[bi * dt.batch + d]) + (dt_bias ? dt_bias[d] : 0.f);
-    if (softplus) step = softplus_f(step);
+    if (softplus) step = softplus_f(step, exp_f(-fabsf(step)));
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
