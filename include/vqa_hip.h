@@ -350,13 +350,12 @@ int vqa_clip_adamax(void* stream, float* p, const float* g, float* m, float* u, 
  * padding - zero rows out, zero gradients, no part in any sum or state, whatever they hold. */
 
 /* y = (x - mean) rstd weight + bias over the last axis; x [rows] with stride ldx, y contiguous; width <= 8192; weight /
- * bias may be NULL (1 / 0); mean, rstd [rows] (both or neither) are what the backward needs. */
+ * bias may be NULL (1 / 0); stats [2][rows] (mean, rstd; may be NULL) is what the backward needs. */
 int vqa_layer_norm_fwd(void* stream, int dtype, const void* x, long ldx, const float* weight, const float* bias, long rows,
-                       int width, float eps, void* y, float* mean, float* rstd);
+                       int width, float eps, void* y, float* stats);
 int vqa_layer_norm_bwd_part(long rows, int width);      /* partial rows: part is [that][2][width] f32 */
 int vqa_layer_norm_bwd(void* stream, int dtype, const void* dy, long lddy, const void* x, long ldx, const float* weight,
-                       const float* mean, const float* rstd, long rows, int width, void* dx, float* dweight, float* dbias,
-                       float* part);
+                       const float* stats, long rows, int width, void* dx, float* dweight, float* dbias, float* part);
 
 /* y_t = act(bias + sum_k weight[:, k] x_{t - taps + 1 + k}), act = silu or none; x [B][L][D], weight [D][taps], taps 2..4.
  * state [B][taps - 1][D] (dtype, may be NULL = zeros): the rows before the first; last (may be NULL): the rows that a

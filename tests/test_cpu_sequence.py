@@ -24,12 +24,12 @@ P = ctypes.c_void_p(64)          # never dereferenced: every call below is refus
 def test_entry_points_refuse_bad_arguments():
     from vqa_amd import _lib as L
     lib = L.lib()
-    norm = lambda dtype=0, x=P, rows=4, width=8, y=P, mean=P, rstd=P: lib.vqa_layer_norm_fwd(      # noqa: E731
-        None, dtype, x, width, None, None, rows, width, 1e-5, y, mean, rstd)
+    norm = lambda dtype=0, x=P, rows=4, width=8, y=P: lib.vqa_layer_norm_fwd(      # noqa: E731
+        None, dtype, x, width, None, None, rows, width, 1e-5, y, None)
     assert all(rc == 1 for rc in (norm(dtype=3), norm(x=None), norm(rows=0), norm(width=0), norm(width=8193),
-                                  norm(y=None), norm(mean=None), norm(rows=1 << 31)))
-    assert lib.vqa_layer_norm_bwd(None, 0, P, 8, P, 8, None, P, P, 4, 8, P, None, None, None) == 1
-    assert lib.vqa_layer_norm_bwd(None, 0, P, 8, P, 8, None, None, P, 4, 8, P, None, None, P) == 1
+                                  norm(y=None), norm(rows=1 << 31)))
+    assert lib.vqa_layer_norm_bwd(None, 0, P, 8, P, 8, None, P, 4, 8, P, None, None, None) == 1
+    assert lib.vqa_layer_norm_bwd(None, 0, P, 8, P, 8, None, None, 4, 8, P, None, None, P) == 1
     assert lib.vqa_layer_norm_bwd_part(0, 8) == 0 and lib.vqa_layer_norm_bwd_part(4, 9000) == 0
     conv = lambda dtype=0, B=1, T=4, D=8, taps=4, w=P: lib.vqa_causal_conv_fwd(                    # noqa: E731
         None, dtype, P, T * D, D, w, None, None, None, B, T, D, taps, 1, P, None)

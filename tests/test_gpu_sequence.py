@@ -596,6 +596,19 @@ def test_versions_and_second_derivatives():
         g.sum().backward()
 
 
+def test_inference_mode():
+    s = S()
+    with torch.inference_mode():
+        x = torch.randn(2, 5, 16, device='cuda')
+        w = torch.randn(16, 4, device='cuda')
+        y, state = s.causal_conv(x[:, :4], w, return_state=True)
+        assert torch.equal(s.causal_conv_step(x[:, 4], state, w), s.causal_conv(x, w)[:, 4])
+        a, b = -torch.rand(16, 8, device='cuda'), torch.randn(2, 5, 8, device='cuda')
+        y, h = s.selective_scan(x[:, :4], x[:, :4], a, b[:, :4], b[:, :4], return_state=True)
+        z = s.selective_scan_step(x[:, 4], h, x[:, 4], a, b[:, 4], b[:, 4])
+        assert z.shape == (2, 16) and s.layer_norm(x).shape == x.shape
+
+
 def test_refusals():
     s = S()
     from vqa_amd._lib import VqaHipError

@@ -56,6 +56,7 @@ def check(status, what):
         raise VqaHipError(f'{what} failed with status {status}')
 
 
+_Tensor = torch.Tensor
 _FN = {}
 _REC = None             # plan.Recorder of the pass being recorded (vqa_amd/plan.py), or None
 
@@ -79,7 +80,10 @@ def call(name, *args):
     if fn is None:
         fn = _FN[name] = getattr(lib(), name)
     raw = _raw_stream()
-    status = fn(raw, *[_conv(a) for a in args])
+    # (_conv's two cases inline: a call of some twenty arguments costs 4 us of host time this way and 7 with a function
+    # call per argument)
+    status = fn(raw, *[a.data_ptr() if isinstance(a, _Tensor) else _conv(a) if isinstance(a, (list, tuple)) else a
+                       for a in args])
     if status != 0:
         raise VqaHipError(f'{name} failed with status {status}', status)
     if _REC is not None:

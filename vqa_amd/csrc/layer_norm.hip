@@ -245,14 +245,14 @@ bool param_vec(const float* p) { return ((uintptr_t)p & 15) == 0; }      // (NUL
 }  // namespace
 
 extern "C" int vqa_layer_norm_fwd(void* stream, int dtype, const void* x, long ldx, const float* weight,
-                                  const float* bias, long rows, int width, float eps, void* y, float* mean,
-                                  float* rstd) {
-    if (bad_shape(dtype, rows, width) || !x || !y || (mean == nullptr) != (rstd == nullptr)) return VQA_ERR_ARG;
+                                  const float* bias, long rows, int width, float eps, void* y, float* stats) {
+    if (bad_shape(dtype, rows, width) || !x || !y) return VQA_ERR_ARG;
     const int e = vqa_elem_bytes(dtype);
     const bool vec = width % (16 / e) == 0 && vqa_vec_ok(x, ldx, e) && vqa_vec_ok(y, width, e) && param_vec(weight) &&
                      param_vec(bias);
     return by_type(dtype, vec, width,
-                   Fwd{static_cast<hipStream_t>(stream), x, ldx, weight, bias, rows, width, eps, y, mean, rstd});
+                   Fwd{static_cast<hipStream_t>(stream), x, ldx, weight, bias, rows, width, eps, y, stats,
+                       stats ? stats + rows : nullptr});
 }
 
 extern "C" int vqa_layer_norm_bwd_part(long rows, int width) {
@@ -260,13 +260,13 @@ extern "C" int vqa_layer_norm_bwd_part(long rows, int width) {
 }
 
 extern "C" int vqa_layer_norm_bwd(void* stream, int dtype, const void* dy, long lddy, const void* x, long ldx,
-                                  const float* weight, const float* mean, const float* rstd, long rows, int width,
-                                  void* dx, float* dweight, float* dbias, float* part) {
-    if (bad_shape(dtype, rows, width) || !dy || !x || !mean || !rstd || !dx || !part) return VQA_ERR_ARG;
+                                  const float* weight, const float* stats, long rows, int width, void* dx,
+                                  float* dweight, float* dbias, float* part) {
+    if (bad_shape(dtype, rows, width) || !dy || !x || !stats || !dx || !part) return VQA_ERR_ARG;
     const int e = vqa_elem_bytes(dtype);
     const bool vec = width % (16 / e) == 0 && vqa_vec_ok(x, ldx, e) && vqa_vec_ok(dy, lddy, e) && vqa_vec_ok(dx, width, e);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const int rc = by_type(dtype, vec, width, Bwd{st, dy, lddy, x, ldx, weight, mean, rstd, rows, width, dx, part});
+    const int rc = by_type(dtype, vec, width, Bwd{st, dy, lddy, x, ldx, weight, stats, stats + rows, rows, width, dx, part});
     if (rc != VQA_OK) return rc;
     if (dweight || dbias) {
         seq_sum_columns(st, part, bwd_groups(rows, width), 2L * width, dweight, width, dbias);

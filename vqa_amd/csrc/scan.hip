@@ -382,41 +382,35 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
     }
 }
 
-// Chains the segments: seg_h[s] becomes the state (REV: the adjoint) that comes into segment s.  A thread takes four states
-// of a channel; eight segments are in flight.
+// Chains the segments: seg_h[s] becomes the state (REV: the adjoint) that comes into segment s.  One thread a state, and it
+// is bound by the latency of its loads (a few segments' states of 2048 x 16 are a few hundred KB): CHAIN of them in flight.
+constexpr int CHAIN = 32;
 template <int NP, bool REV> __global__ __launch_bounds__(256) void scan_chain(Args A) {
     const long chans = (long)A.G * A.per_pad, id = (long)blockIdx.x * 256 + threadIdx.x;
-    if (id >= A.B * chans * (NP / 4)) return;
-    const int n = (int)(id % (NP / 4)) * 4, p = (int)(id / (NP / 4) % chans), b = (int)(id / (NP / 4) / chans);
+    if (id >= A.B * chans * NP) return;
+    const int n = (int)(id % NP), p = (int)(id / NP % chans), b = (int)(id / NP / chans);
     const int g = p / A.per_pad, off = p % A.per_pad, c = g * A.per + off;
-    if (off >= A.per) return;
+    if (off >= A.per || n >= A.N) return;
     const float* start = REV ? A.dlast : A.state;
-    float a[4], h[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        a[k] = n + k < A.N ? A.a[(long)c * A.N + n + k] * LOG2E : 0.f;
-        h[k] = start && n + k < A.N ? start[((long)b * A.D + c) * A.N + n + k] : 0.f;
-    }
+    const float a = A.a[(long)c * A.N + n] * LOG2E;
+    float h = start ? start[((long)b * A.D + c) * A.N + n] : 0.f;
     const long first = (long)b * A.segs * chans + p;
-    float4* q = reinterpret_cast<float4*>(A.seg_h + first * NP + n);
+    float* q = A.seg_h + first * NP + n;
     const float* dt = A.seg_dt + first;
-    for (int s0 = 0; s0 < A.segs; s0 += 8) {
-        float4 e[8];
-        float d[8];
+    for (int s0 = 0; s0 < A.segs; s0 += CHAIN) {
+        float e[CHAIN], d[CHAIN];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int s = REV ? A.segs - 1 - s0 - u : s0 + u;
-            if (s >= 0 && s < A.segs) { e[u] = q[s * chans * (NP / 4)]; d[u] = dt[s * chans]; }
+        for (int u = 0; u < CHAIN; ++u) {
+            const int s = REV ? max(A.segs - 1 - s0 - u, 0) : min(s0 + u, A.segs - 1);
+            e[u] = q[s * chans * NP];
+            d[u] = dt[s * chans];
         }
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
+        for (int u = 0; u < CHAIN; ++u) {
             const int s = REV ? A.segs - 1 - s0 - u : s0 + u;
             if (s >= 0 && s < A.segs) {
-                q[s * chans * (NP / 4)] = make_float4(h[0], h[1], h[2], h[3]);
-                h[0] = __builtin_amdgcn_exp2f(d[u] * a[0]) * h[0] + e[u].x;
-                h[1] = __builtin_amdgcn_exp2f(d[u] * a[1]) * h[1] + e[u].y;
-                h[2] = __builtin_amdgcn_exp2f(d[u] * a[2]) * h[2] + e[u].z;
-                h[3] = __builtin_amdgcn_exp2f(d[u] * a[3]) * h[3] + e[u].w;
+                q[s * chans * NP] = h;
+                h = __builtin_amdgcn_exp2f(d[u] * a) * h + e[u];
             }
         }
     }
@@ -875,7 +869,7 @@ long part_p_floats(const Args& A) { return (long)A.bgroups * A.segs * A.G * A.pe
 long part_bc_floats(const Args& A) { return (long)A.bblk * A.B * A.L * A.G * 2 * A.N; }
 
 template <int NP, bool REV> int chain(const Args& A, hipStream_t st) {
-    const long n = (long)A.B * A.G * A.per_pad * (NP / 4);
+    const long n = (long)A.B * A.G * A.per_pad * NP;
     scan_chain<NP, REV><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(A);
     CHECK_LAUNCH();
     return VQA_OK;

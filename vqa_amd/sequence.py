@@ -27,17 +27,19 @@ from torch.autograd.graph import increment_version
 from . import _lib as L
 
 _ROW_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+_F32 = torch.float32
 
 
 class _device_of:
     """Makes x's device the current one for the call where it is not (the kernels go to the current device's stream)."""
 
     def __init__(self, x):
-        self.want, self.had = x.device.index, None
+        self.want, self.had = x.get_device(), None
 
     def __enter__(self):
-        if torch._C._cuda_getDevice() != self.want:
-            self.had = torch._C._cuda_getDevice()
+        had = torch._C._cuda_getDevice()
+        if had != self.want:
+            self.had = had
             torch._C._cuda_setDevice(self.want)
 
     def __exit__(self, *exc):
@@ -49,24 +51,29 @@ def _fail(what):
     raise L.VqaHipError(what)
 
 
-def _rows(name, x, shape=None, like=None):
-    """A row tensor: on the GPU, of a row type, of `like`'s type and device, of this shape."""
+def _first(x, dims, what):
+    """The tensor that sets the type and the device: rows on the GPU, of a row type, with this many axes (None: any)."""
     if not x.is_cuda:
-        _fail(f'{name} must be on the GPU (there is no CPU fallback)')
-    if like is None:
-        if x.dtype not in _ROW_TYPES:
-            _fail(f'{name} must be float32, bfloat16 or float16, not {x.dtype}')
-    elif x.dtype != like.dtype or x.device != like.device:
-        _fail(f'{name} is {x.dtype} on {x.device}: {like.dtype} on {like.device} is wanted')
-    if shape is not None and x.shape != shape:
-        _fail(f'{name} has shape {tuple(x.shape)}: {tuple(shape)} is wanted')
+        _fail('x must be on the GPU (there is no CPU fallback)')
+    if x.dtype not in _ROW_TYPES:
+        _fail(f'x must be float32, bfloat16 or float16, not {x.dtype}')
+    if dims is not None and x.dim() != dims:
+        _fail(f'x has shape {tuple(x.shape)}: {what} is wanted')
+
+
+def _rows(name, t, shape, x):
+    """A row tensor of x's type and device and (shape not None) of this shape."""
+    if t.dtype is not x.dtype or t.get_device() != x.get_device():
+        _fail(f'{name} is {t.dtype} on {t.device}: {x.dtype} on {x.device} is wanted')
+    if shape is not None and t.shape != shape:
+        _fail(f'{name} has shape {tuple(t.shape)}: {tuple(shape)} is wanted')
 
 
 def _param(name, p, shape, x):
     """A float32 parameter or state of this shape on x's device, contiguous; None stays None."""
     if p is None:
         return None
-    if p.dtype != torch.float32 or p.device != x.device:
+    if p.dtype is not _F32 or p.get_device() != x.get_device():
         _fail(f'{name} is {p.dtype} on {p.device}: float32 on {x.device} is wanted')
     if p.shape != shape:
         _fail(f'{name} has shape {tuple(p.shape)}: {tuple(shape)} is wanted')
@@ -86,13 +93,35 @@ def _unit(x):
     return x if x.stride(-1) == 1 else x.contiguous()
 
 
+def _near(x):
+    """... and rows whose distance the scan's kernels can take (8 rows within 2 GiB)"""
+    return x if x.stride(-1) == 1 and (x.dim() == 2 or x.stride(1) < 1 << 26) else x.contiguous()
+
+
+def _touched(state):
+    """A kernel wrote into `state`: autograd's version of it moves on."""
+    if not state.is_inference():
+        increment_version(state)
+
+
 def _tracked(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _no_tracking(what, *tensors):
     if _tracked(*tensors):
         _fail(f'{what} has no gradient: call it under torch.no_grad()')
+
+
+def _backward(f):
+    """The backward of these operators, which has no derivative of its own: asked for one (create_graph) its results are
+    marked so.  (once_differentiable alone costs every ordinary backward a few microseconds.)"""
+    marked = once_differentiable(f)
+    return staticmethod(lambda ctx, *grads: marked(ctx, *grads) if torch.is_grad_enabled() else f(ctx, *grads))
 
 
 # ---------------------------------------------------------------------------------------------------------- layer norm
@@ -102,28 +131,26 @@ def _as_matrix(x):
     return _unit(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
 
 
-def _norm_fwd(x2, weight, bias, eps, shape, stats):
+def _norm_fwd(x, weight, bias, eps, stats):
+    x2 = _as_matrix(x)
     rows, width = x2.shape
-    y = torch.empty(shape, device=x2.device, dtype=x2.dtype)
-    st = torch.empty(2, rows, device=x2.device, dtype=torch.float32) if stats else None
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    st = torch.empty(2, rows, device=x.device, dtype=_F32) if stats else None
     if rows:
-        L.call('vqa_layer_norm_fwd', L.dt(x2), x2, x2.stride(0), weight, bias, rows, width, eps, y,
-               st[0] if stats else None, st[1] if stats else None)
+        L.call('vqa_layer_norm_fwd', L.dt(x), x2, x2.stride(0), weight, bias, rows, width, eps, y, st)
     return y, st
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        x2 = _as_matrix(x)
         with _device_of(x):
-            y, st = _norm_fwd(x2, weight, bias, eps, x.shape, True)
+            y, st = _norm_fwd(x, weight, bias, eps, True)
         ctx.save_for_backward(x, weight, st)
         ctx.has_bias = bias is not None
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_backward
     def backward(ctx, dy):
         x, weight, st = ctx.saved_tensors
         x2, dy2 = _as_matrix(x), _as_matrix(dy)
@@ -131,13 +158,12 @@ class _LayerNorm(torch.autograd.Function):
         dev = x.device
         with _device_of(x):
             dx = torch.empty(x.shape, device=dev, dtype=x.dtype)
-            dw = torch.empty(width, device=dev, dtype=torch.float32) if weight is not None else None
-            db = torch.empty(width, device=dev, dtype=torch.float32) if ctx.has_bias else None
+            dw = torch.empty(width, device=dev, dtype=_F32) if weight is not None else None
+            db = torch.empty(width, device=dev, dtype=_F32) if ctx.has_bias else None
             if rows:
-                part = torch.empty(L.lib().vqa_layer_norm_bwd_part(rows, width), 2, width, device=dev,
-                                   dtype=torch.float32)
-                L.call('vqa_layer_norm_bwd', L.dt(x), dy2, dy2.stride(0), x2, x2.stride(0), weight, st[0], st[1], rows,
-                       width, dx, dw, db, part)
+                part = torch.empty(_norm_parts(rows, width), 2, width, device=dev, dtype=_F32)
+                L.call('vqa_layer_norm_bwd', L.dt(x), dy2, dy2.stride(0), x2, x2.stride(0), weight, st, rows, width,
+                       dx, dw, db, part)
             else:
                 for g in (dw, db):
                     if g is not None:
@@ -145,17 +171,22 @@ class _LayerNorm(torch.autograd.Function):
         return dx, dw, db, None
 
 
+@lru_cache(maxsize=1024)
+def _norm_parts(rows, width):
+    return L.lib().vqa_layer_norm_bwd_part(rows, width)
+
+
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis (biased variance), statistics in float32.
     x [..., C] with C <= 8192; weight, bias float32 [C] or None."""
-    _rows('x', x)
+    _first(x, None, '')
     if x.dim() < 1 or not 1 <= x.shape[-1] <= 8192:
         _fail(f'x has shape {tuple(x.shape)}: a last axis of 1 to 8192 is wanted')
     weight, bias = _param('weight', weight, x.shape[-1:], x), _param('bias', bias, x.shape[-1:], x)
     if _tracked(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, eps)
     with _device_of(x):
-        return _norm_fwd(_as_matrix(x), weight, bias, eps, x.shape, False)[0]
+        return _norm_fwd(x, weight, bias, eps, False)[0]
 
 
 # --------------------------------------------------------------------------------------------------- causal convolution
@@ -195,8 +226,7 @@ class _CausalConv(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return y, last
 
-    @staticmethod
-    @once_differentiable
+    @_backward
     def backward(ctx, dy, dlast):
         x, weight, bias, state, lengths = ctx.saved_tensors
         B, T, D = x.shape
@@ -205,12 +235,11 @@ class _CausalConv(torch.autograd.Function):
             dy = torch.zeros(B, T, D, device=dev, dtype=x.dtype) if dy is None else _unit(dy)
             dlast = None if dlast is None else dlast.contiguous()
             dx = torch.empty(B, T, D, device=dev, dtype=x.dtype)
-            dw = torch.empty(D, taps, device=dev, dtype=torch.float32)
-            db = torch.empty(D, device=dev, dtype=torch.float32) if bias is not None else None
+            dw = torch.empty(D, taps, device=dev, dtype=_F32)
+            db = torch.empty(D, device=dev, dtype=_F32) if bias is not None else None
             dstate = torch.empty(B, taps - 1, D, device=dev, dtype=x.dtype) if state is not None else None
             if dx.numel():
-                part = torch.empty(L.lib().vqa_causal_conv_bwd_part(B, T, D), taps + 1, D, device=dev,
-                                   dtype=torch.float32)
+                part = torch.empty(_conv_parts(B, T, D), taps + 1, D, device=dev, dtype=_F32)
                 L.call('vqa_causal_conv_bwd', L.dt(x), dy, dy.stride(0), dy.stride(1), dlast, x, x.stride(0),
                        x.stride(1), weight, bias, state, lengths, B, T, D, taps, ctx.silu, dx, dw, db, dstate, part)
             else:
@@ -222,14 +251,17 @@ class _CausalConv(torch.autograd.Function):
         return dx, dw, db, None, dstate, None, None
 
 
+@lru_cache(maxsize=1024)
+def _conv_parts(B, T, D):
+    return L.lib().vqa_causal_conv_bwd_part(B, T, D)
+
+
 def causal_conv(x, weight, bias=None, activation='silu', state=None, lengths=None, return_state=False):
     """One filter of 2 to 4 taps per channel over the tokens of x [B, L, D], each token seeing itself and those before it:
     y_t = act(bias + sum_k weight[:, k] x_{t - taps + 1 + k}), act = silu or (activation=None) nothing; weight float32
     [D, taps], bias float32 [D].  state [B, taps - 1, D] (x's type): the rows before the first (None: zeros).  Returns y,
     or with return_state (y, state after each sequence's last token)."""
-    _rows('x', x)
-    if x.dim() != 3:
-        _fail(f'x has shape {tuple(x.shape)}: [B, L, D] is wanted')
+    _first(x, 3, '[B, L, D]')
     B, T, D = x.shape
     taps = _taps(weight, D)
     weight, bias = _param('weight', weight, (D, taps), x), _param('bias', bias, (D,), x)
@@ -250,9 +282,7 @@ def causal_conv(x, weight, bias=None, activation='silu', state=None, lengths=Non
 def causal_conv_step(x, state, weight, bias=None, activation='silu'):
     """causal_conv for ONE new token per sequence: x [B, D]; state [B, taps - 1, D] (x's type; rows may be strided) is
     shifted in place.  Returns y [B, D].  Forward only."""
-    _rows('x', x)
-    if x.dim() != 2:
-        _fail(f'x has shape {tuple(x.shape)}: [B, D] is wanted')
+    _first(x, 2, '[B, D]')
     B, D = x.shape
     taps = _taps(weight, D)
     weight, bias = _param('weight', weight, (D, taps), x), _param('bias', bias, (D,), x)
@@ -267,9 +297,14 @@ def causal_conv_step(x, state, weight, bias=None, activation='silu'):
             B == 1 or s0 >= (taps - 2) * s1 + D or (s0 >= D and s1 >= (B - 1) * s0 + D)):
         _fail(f'state has strides {state.stride()}: it is updated in place, so rows must be contiguous and apart')
     x = _unit(x)
-    with _device_of(x):
-        L.call('vqa_causal_conv_token', L.dt(x), x, x.stride(0), state, s0, s1, weight, bias, B, D, taps, silu, y)
-    increment_version(state)
+    if L._PROFILE is None and L._REC is None and torch._C._cuda_getDevice() == x.get_device():
+        L.check(L.lib().vqa_causal_conv_token(
+            L._raw_stream(), L.dt(x), x.data_ptr(), x.stride(0), state.data_ptr(), s0, s1, weight.data_ptr(),
+            None if bias is None else bias.data_ptr(), B, D, taps, silu, y.data_ptr()), 'vqa_causal_conv_token')
+    else:
+        with _device_of(x):
+            L.call('vqa_causal_conv_token', L.dt(x), x, x.stride(0), state, s0, s1, weight, bias, B, D, taps, silu, y)
+    _touched(state)
     return y
 
 
@@ -284,19 +319,19 @@ def _scan_bytes(dtype, B, T, D, N, G):
 
 
 def _floats(nbytes, dev):
-    return torch.empty(nbytes // 4, device=dev, dtype=torch.float32) if nbytes else None
+    return torch.empty(nbytes // 4, device=dev, dtype=_F32) if nbytes else None
 
 
-def _strides(x, tokens):
-    """the leading strides of a row tensor, zeros for None"""
-    return (0, 0) if x is None else (x.stride(0), x.stride(1)) if tokens else (x.stride(0),)
+def _strides(x):
+    """batch and row stride of a row tensor, zeros for None"""
+    return (0, 0) if x is None else (x.stride(0), x.stride(1))
 
 
 def _scan_fwd(x, dt, a, b, c, skip, gate, dt_bias, softplus, state, lengths, want_last, want_keep):
     B, T, D = x.shape
     G, N, dev, code = b.shape[2], b.shape[3], x.device, L.dt(x)
     y = torch.empty(B, T, D, device=dev, dtype=x.dtype)
-    last = torch.empty(B, D, N, device=dev, dtype=torch.float32) if want_last else None
+    last = torch.empty(B, D, N, device=dev, dtype=_F32) if want_last else None
     if not y.numel():
         if want_last and last.numel():
             last.zero_() if state is None else last.copy_(state)
@@ -305,7 +340,7 @@ def _scan_fwd(x, dt, a, b, c, skip, gate, dt_bias, softplus, state, lengths, wan
     ws = _floats(fwd, dev)
     keep = _floats(keep_bytes, dev) if want_keep else None
     L.call('vqa_scan_fwd', code, x, x.stride(0), x.stride(1), dt, dt.stride(0), dt.stride(1), gate,
-           *_strides(gate, True), a, b, b.stride(0), b.stride(1), c, c.stride(0), c.stride(1), skip, dt_bias, softplus,
+           *_strides(gate), a, b, b.stride(0), b.stride(1), c, c.stride(0), c.stride(1), skip, dt_bias, softplus,
            state, lengths, B, T, D, N, G, y, last, keep, ws)
     return y, last, keep
 
@@ -320,13 +355,12 @@ class _SelectiveScan(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return y, last
 
-    @staticmethod
-    @once_differentiable
+    @_backward
     def backward(ctx, dy, dlast):
         x, dt, a, b, c, skip, gate, dt_bias, lengths, keep = ctx.saved_tensors
         B, T, D = x.shape
         G, N, dev, code = b.shape[2], b.shape[3], x.device, L.dt(x)
-        f32 = lambda *s: torch.empty(*s, device=dev, dtype=torch.float32)       # noqa: E731
+        f32 = lambda *s: torch.empty(*s, device=dev, dtype=_F32)       # noqa: E731
         rows = lambda *s: torch.empty(*s, device=dev, dtype=x.dtype)            # noqa: E731
         with _device_of(x):
             dlast = None if dlast is None else dlast.contiguous()
@@ -341,10 +375,10 @@ class _SelectiveScan(torch.autograd.Function):
                 if dstate is not None:
                     dstate.zero_() if dlast is None else dstate.copy_(dlast)
             else:
-                dy = torch.zeros(B, T, D, device=dev, dtype=x.dtype) if dy is None else _unit(dy)
+                dy = torch.zeros(B, T, D, device=dev, dtype=x.dtype) if dy is None else _near(dy)
                 ws = _floats(_scan_bytes(code, B, T, D, N, G)[2], dev)
                 L.call('vqa_scan_bwd', code, dy, dy.stride(0), dy.stride(1), dlast, x, x.stride(0), x.stride(1), dt,
-                       dt.stride(0), dt.stride(1), gate, *_strides(gate, True), a, b, b.stride(0), b.stride(1), c,
+                       dt.stride(0), dt.stride(1), gate, *_strides(gate), a, b, b.stride(0), b.stride(1), c,
                        c.stride(0), c.stride(1), skip, dt_bias, ctx.softplus, lengths, B, T, D, N, G, keep, dx, ddt,
                        dgate, da, db, dc, dskip, dbias, dstate, ws)
         return dx, ddt, da, db, dc, dskip, dgate, dbias, None, dstate, None, None
@@ -359,7 +393,8 @@ def _shared(name, b, lead, x):
     if b.dim() == k + 1:
         b = b.unsqueeze(k)
     G, N = b.shape[k:]
-    return b if b.stride(-1) == 1 and (G == 1 or b.stride(-2) == N) else b.contiguous()
+    near = b.stride(-1) == 1 and (G == 1 or b.stride(-2) == N) and (k == 1 or b.stride(1) < 1 << 26)
+    return b if near else b.contiguous()
 
 
 def _scan_args(x, dt, a, b, c, skip, gate, dt_bias):
@@ -367,14 +402,14 @@ def _scan_args(x, dt, a, b, c, skip, gate, dt_bias):
     _rows('dt', dt, x.shape, x)
     if gate is not None:
         _rows('gate', gate, x.shape, x)
-        gate = _unit(gate)
+        gate = _near(gate)
     b, c = _shared('b', b, lead, x), _shared('c', c, lead, x)
     G, N = b.shape[-2:]
     if c.shape != b.shape:
         _fail(f'b and c have shapes {tuple(b.shape)} and {tuple(c.shape)}: the same is wanted')
     if not 1 <= N <= 64 or G < 1 or D % G:
         _fail(f'{N} states in {G} groups over {D} channels: 1 to 64 states and a whole number of channels a group')
-    return (_unit(x), _unit(dt), _param('a', a, (D, N), x), b, c, _param('skip', skip, (D,), x), gate,
+    return (_near(x), _near(dt), _param('a', a, (D, N), x), b, c, _param('skip', skip, (D,), x), gate,
             _param('dt_bias', dt_bias, (D,), x))
 
 
@@ -386,9 +421,7 @@ def selective_scan(x, dt, a, b, c, skip=None, gate=None, dt_bias=None, softplus=
     dt, gate [B, L, D]; b, c [B, L, N], or [B, L, G, N] where each of G groups of D / G channels has its own; a float32
     [D, N]; skip, dt_bias float32 [D]; state float32 [B, D, N] (None: zeros).  gate, skip, dt_bias may be None.
     Returns y, or with return_state (y, state after each sequence's last token)."""
-    _rows('x', x)
-    if x.dim() != 3:
-        _fail(f'x has shape {tuple(x.shape)}: [B, L, D] is wanted')
+    _first(x, 3, '[B, L, D]')
     args = x, dt, a, b, c, skip, gate, dt_bias = _scan_args(x, dt, a, b, c, skip, gate, dt_bias)
     state = _param('state', state, (x.shape[0], *a.shape), x)
     lengths = _lengths(lengths, x)
@@ -403,9 +436,7 @@ def selective_scan(x, dt, a, b, c, skip=None, gate=None, dt_bias=None, softplus=
 def selective_scan_step(x, state, dt, a, b, c, skip=None, gate=None, dt_bias=None, softplus=True):
     """selective_scan for ONE new token per sequence: x, dt, gate [B, D]; b, c [B, N] or [B, G, N]; state float32
     [B, D, N] is updated in place (its batch axis may be strided).  Returns y [B, D].  Forward only."""
-    _rows('x', x)
-    if x.dim() != 2:
-        _fail(f'x has shape {tuple(x.shape)}: [B, D] is wanted')
+    _first(x, 2, '[B, D]')
     x, dt, a, b, c, skip, gate, dt_bias = _scan_args(x, dt, a, b, c, skip, gate, dt_bias)
     B, D = x.shape
     G, N = b.shape[1:]
@@ -417,8 +448,17 @@ def selective_scan_step(x, state, dt, a, b, c, skip=None, gate=None, dt_bias=Non
         return y
     if (state.stride(2) != 1 and N > 1) or (state.stride(1) != N and D > 1) or (B > 1 and state.stride(0) < D * N):
         _fail(f'state has strides {state.stride()}: it is updated in place, so [D, N] must be contiguous and apart')
-    with _device_of(x):
-        L.call('vqa_scan_token', L.dt(x), x, x.stride(0), state, state.stride(0), dt, dt.stride(0), gate,
-               *_strides(gate, False)[:1], a, b, b.stride(0), c, c.stride(0), skip, dt_bias, int(softplus), B, D, N, G, y)
-    increment_version(state)
+    sg = 0 if gate is None else gate.stride(0)
+    if L._PROFILE is None and L._REC is None and torch._C._cuda_getDevice() == x.get_device():
+        # (one token's latency is host time: pointers are taken here, 3 us less than by L.call)
+        L.check(L.lib().vqa_scan_token(
+            L._raw_stream(), L.dt(x), x.data_ptr(), x.stride(0), state.data_ptr(), state.stride(0), dt.data_ptr(),
+            dt.stride(0), None if gate is None else gate.data_ptr(), sg, a.data_ptr(), b.data_ptr(), b.stride(0),
+            c.data_ptr(), c.stride(0), None if skip is None else skip.data_ptr(),
+            None if dt_bias is None else dt_bias.data_ptr(), softplus, B, D, N, G, y.data_ptr()), 'vqa_scan_token')
+    else:
+        with _device_of(x):
+            L.call('vqa_scan_token', L.dt(x), x, x.stride(0), state, state.stride(0), dt, dt.stride(0), gate, sg, a, b,
+                   b.stride(0), c, c.stride(0), skip, dt_bias, softplus, B, D, N, G, y)
+    _touched(state)
     return y
