@@ -3,14 +3,16 @@
 //   g_t = dy_t (silu'(pre_t));  dx_t = sum_k w[:, k] g_{t + W - 1 - k};  dw[:, k] = sum g_t x_{t - W + 1 + k};  db = sum g_t
 // Rows before the first are the W - 1 rows of `state` (zeros without one); rows at or past a sequence's length are neither
 // read into a sum nor answered (zero rows); the state handed on is the last W - 1 rows before that length.
-// All of it is bound by HBM (a few operations per element): a thread owns V channels (16 bytes) and walks down a chunk of
-// rows with the filter's window in registers, so a row is loaded once per chunk, plus W - 1 rows at its border.  The backward
-// recomputes pre_t from x (nothing is saved) and carries the window of g the same way.
+// All of it is bound by HBM, the backward nearly as much by its 35 operations per element: a thread owns four channels and
+// walks down a chunk of rows with the filter's window in registers, so a row is loaded once per chunk, plus W - 1 rows at its
+// border.  The backward recomputes pre_t from x (nothing is saved) and carries the window of g the same way.
+// Measured at 8 x 4096 x 2048 bf16, 4 taps, silu: forward 56 us = 4.8 TB/s, backward 94 us = 4.3 TB/s (a large copy: 5.1).
 #include "seq.h"
 
 namespace {
 
-constexpr int RB = 8;          // rows a thread has in flight
+constexpr int RB = 4;          // rows a forward thread has in flight (8 x 4096 x 2048 bf16: 56 us; with 8 rows, or 8 channels a thread, 64-68:
+                               // too few waves fit)
 
 template <typename T, int V, int W, bool SILU>
 __global__ __launch_bounds__(256) void conv_fwd(const T* __restrict__ x, long xb, long xl, const float* __restrict__ w,
@@ -118,48 +120,85 @@ __global__ __launch_bounds__(256) void conv_bwd(const T* __restrict__ dy, long g
         }
         // step s takes in g_s and gives out the gradient of row s - (W - 1): the first chunk begins with the state's rows
         const int end = t1 + W - 1;
-        for (int s0 = t0; s0 < end; s0 += RB / 2) {
-            Raw<T, V> rx[RB / 2], rg[RB / 2];
+        auto step = [&](int s) {                           // one row with every guard
+            Raw<T, V> rx, rg, o;
+            rx.zero();
+            rg.zero();
+            if (s < len) { rx.load(xr + s * xl); rg.load(gr + s * gl); }
+            const int t = s - (W - 1), r = s - len;        // row answered; its place among the rows handed on
+            float e[V];
 #pragma unroll
-            for (int i = 0; i < RB / 2; ++i) {
-                const int s = s0 + i;
-                rx[i].zero();
-                rg[i].zero();
-                if (s < end && s < len) { rx[i].load(xr + s * xl); rg[i].load(gr + s * gl); }
+            for (int v = 0; v < V; ++v) {
+                win[W - 1][v] = rx.get(v);
+                float p = bv[v];
+#pragma unroll
+                for (int k = 0; k < W; ++k) p += wk[k][v] * win[k][v];
+                const float d = rg.get(v);
+                gw[W - 1][v] = s < len ? (SILU ? d * dsilu_f(p) : d) : 0.f;
+                if (s < t1) {                              // (a row past the chunk is another's to sum)
+                    ab[v] += gw[W - 1][v];
+#pragma unroll
+                    for (int k = 0; k < W; ++k) aw[k][v] += gw[W - 1][v] * win[k][v];
+                }
+                e[v] = 0.f;
+#pragma unroll
+                for (int k = 0; k < W; ++k) e[v] += wk[k][v] * gw[W - 1 - k][v];
+#pragma unroll
+                for (int k = 0; k < W - 1; ++k) { win[k][v] = win[k + 1][v]; gw[k][v] = gw[k + 1][v]; }
+            }
+            if (dlast && r >= 0 && r < W - 1) {
+                Raw<T, V> dl;
+                dl.load(dlast + ((long)b * (W - 1) + r) * D + c);
+#pragma unroll
+                for (int v = 0; v < V; ++v) e[v] += dl.get(v);
             }
 #pragma unroll
-            for (int i = 0; i < RB / 2; ++i) {
-                const int s = s0 + i;
-                if (s >= end) continue;
-                const int t = s - (W - 1), r = s - len;    // row answered; its place among the rows handed on
-                const bool own = s < t1;
-                Raw<T, V> o, dl;
-                dl.zero();
-                if (dlast && r >= 0 && r < W - 1) dl.load(dlast + ((long)b * (W - 1) + r) * D + c);
+            for (int v = 0; v < V; ++v) o.set(v, e[v]);
+            if (t >= t0) o.store(dx + ((long)b * L + t) * D + c);
+            else if (t < 0 && dstate) o.store(dstate + ((long)b * (W - 1) + s) * D + c);
+        };
+        int s = t0;
+        for (; s < min(end, t0 + W - 1); ++s) step(s);
+        // the body: rows that are the chunk's own, before the sequence's end, and answer one of the chunk's.  U rows at a
+        // time, the next U in flight; the windows turn instead of moving (U is a multiple of W)
+        constexpr int U = W == 3 ? 3 : 4;
+        const int body = min(t1, len) - U;
+        if (s <= body) {
+            Raw<T, V> nx[U], ng[U];
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    win[W - 1][v] = rx[i].get(v);
-                    float p = bv[v];
+            for (int i = 0; i < U; ++i) { nx[i].load(xr + (s + i) * xl); ng[i].load(gr + (s + i) * gl); }
+            for (; s <= body; s += U) {
+                Raw<T, V> rx[U], rg[U];
 #pragma unroll
-                    for (int k = 0; k < W; ++k) p += wk[k][v] * win[k][v];
-                    const float d = rg[i].get(v);
-                    gw[W - 1][v] = s < len ? (SILU ? d * dsilu_f(p) : d) : 0.f;
-                    if (own) {
-                        ab[v] += gw[W - 1][v];
+                for (int i = 0; i < U; ++i) { rx[i] = nx[i]; rg[i] = ng[i]; }
+                if (s + U <= body) {
 #pragma unroll
-                        for (int k = 0; k < W; ++k) aw[k][v] += gw[W - 1][v] * win[k][v];
-                    }
-                    float e = dl.get(v);
-#pragma unroll
-                    for (int k = 0; k < W; ++k) e += wk[k][v] * gw[W - 1 - k][v];
-                    o.set(v, e);
-#pragma unroll
-                    for (int k = 0; k < W - 1; ++k) { win[k][v] = win[k + 1][v]; gw[k][v] = gw[k + 1][v]; }
+                    for (int i = 0; i < U; ++i) { nx[i].load(xr + (s + U + i) * xl); ng[i].load(gr + (s + U + i) * gl); }
                 }
-                if (t >= t0) o.store(dx + ((long)b * L + t) * D + c);
-                else if (t < 0 && dstate) o.store(dstate + ((long)b * (W - 1) + s) * D + c);
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    Raw<T, V> o;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        win[(i + W - 1) % W][v] = rx[i].get(v);
+                        float p = bv[v];
+#pragma unroll
+                        for (int k = 0; k < W; ++k) p += wk[k][v] * win[(i + k) % W][v];
+                        const float d = rg[i].get(v), g = SILU ? d * dsilu_f(p) : d;
+                        gw[(i + W - 1) % W][v] = g;
+                        ab[v] += g;
+                        float e = wk[0][v] * g;
+#pragma unroll
+                        for (int k = 1; k < W; ++k) e += wk[k][v] * gw[(i + W - 1 - k) % W][v];
+#pragma unroll
+                        for (int k = 0; k < W; ++k) aw[k][v] += g * win[(i + k) % W][v];
+                        o.set(v, e);
+                    }
+                    o.store(dx + ((long)b * L + s + i - (W - 1)) * D + c);
+                }
             }
         }
+        for (; s < end; ++s) step(s);
     }
     // the chunks that this workgroup worked on side by side are joined in a fixed order
     float* out = part + (long)blockIdx.y * (W + 1) * D;
@@ -213,10 +252,10 @@ template <typename T, int V, typename F> int by_taps(int taps, int silu, F f) {
     if (taps == 3) return silu ? f.template operator()<T, V, 3, true>() : f.template operator()<T, V, 3, false>();
     return silu ? f.template operator()<T, V, 4, true>() : f.template operator()<T, V, 4, false>();
 }
-template <int V16, typename F> int by_type(int dtype, bool vec, int taps, int silu, F f) {
+template <typename F> int by_type(int dtype, bool vec, int taps, int silu, F f) {
     if (dtype == VQA_F32) return vec ? by_taps<float, 4>(taps, silu, f) : by_taps<float, 1>(taps, silu, f);
-    if (dtype == VQA_BF16) return vec ? by_taps<bf16, V16>(taps, silu, f) : by_taps<bf16, 1>(taps, silu, f);
-    return vec ? by_taps<_Float16, V16>(taps, silu, f) : by_taps<_Float16, 1>(taps, silu, f);
+    if (dtype == VQA_BF16) return vec ? by_taps<bf16, 4>(taps, silu, f) : by_taps<bf16, 1>(taps, silu, f);
+    return vec ? by_taps<_Float16, 4>(taps, silu, f) : by_taps<_Float16, 1>(taps, silu, f);
 }
 
 bool bad_shape(int dtype, int B, long L, int D, int taps) {
@@ -225,7 +264,7 @@ bool bad_shape(int dtype, int B, long L, int D, int taps) {
 }
 
 int fwd_chunk(int B, int L, int nv) {
-    // rows per thread: long chunks read few border rows again, but 256 CUs want some 64k threads
+    // rows per thread: long chunks read few border rows again, but 256 CUs want some 256k threads
     int chunk = 32;
     while (chunk > 8 && (long)B * ((L + chunk - 1) / chunk) * nv < 262144) chunk /= 2;
     return chunk;
@@ -245,15 +284,18 @@ struct Fwd {
     }
 };
 
-// The backward's grid: lx lanes x V channels across, the rest of a workgroup's 256 threads down the chunks of rows.
+// The backward's grid: lx lanes x V channels across, the rest of a workgroup's 256 threads down the chunks of rows.  Chunks as
+// long as 100k threads allow (every chunk computes W - 1 rows of its neighbour's g again and steps in and out of the
+// body's unrolled rows): at 8 x 4096 x 2048 bf16 94 us with 128 rows, 105 with 64, 116 with 32; 64 x 256 x 1024 takes 32 us
+// where chunks shrink to keep 65k or 100k threads, 44 us where 32k are let through.
 struct Grid { int lx, gx, gy, chunk; };
 Grid bwd_grid(int B, int L, int D, int V) {
     const int nv = (D + V - 1) / V;
     int lx = 8;
     while (lx < 64 && lx < nv) lx *= 2;
     const int gx = (nv + lx - 1) / lx, ly = 256 / lx;
-    int chunk = 64;
-    while (chunk > 8 && (long)B * ((L + chunk - 1) / chunk) * gx * lx < 131072) chunk /= 2;
+    int chunk = 128;
+    while (chunk > 8 && (long)B * ((L + chunk - 1) / chunk) * gx * lx < 100000) chunk /= 2;
     const long chunks = (long)B * ((L + chunk - 1) / chunk);
     long gy = (chunks + ly - 1) / ly;
     const long most = gx >= 1024 ? 1 : 1024 / gx;
@@ -290,10 +332,10 @@ extern "C" int vqa_causal_conv_fwd(void* stream, int dtype, const void* x, long 
                                    const float* bias, const void* state, const int* lengths, int B, int L, int D,
                                    int taps, int silu, void* y, void* last) {
     if (bad_shape(dtype, B, L, D, taps) || !x || !weight || !y) return VQA_ERR_ARG;
-    const int e = vqa_elem_bytes(dtype);
-    const bool vec = D % (16 / e) == 0 && vqa_vec_ok(x, x_row, e) && vqa_vec_ok(x, x_batch, e) && vqa_vec_ok(y, D, e) &&
-                     vqa_vec_ok(state, D, e) && vqa_vec_ok(last, D, e);
-    return by_type<8>(dtype, vec, taps, silu,
+    const int e = vqa_elem_bytes(dtype), four = 4 * e;
+    const bool vec = D % 4 == 0 && vqa_vec_ok(x, x_row, e, four) && vqa_vec_ok(x, x_batch, e, four) && vqa_vec_ok(y, D, e, four) &&
+                     vqa_vec_ok(state, D, e, four) && vqa_vec_ok(last, D, e, four);
+    return by_type(dtype, vec, taps, silu,
                       Fwd{static_cast<hipStream_t>(stream), x, x_batch, x_row, weight, bias, state, lengths, B, L, D, y, last});
 }
 
@@ -308,12 +350,12 @@ extern "C" int vqa_causal_conv_bwd(void* stream, int dtype, const void* dy, long
                                    const void* state, const int* lengths, int B, int L, int D, int taps, int silu,
                                    void* dx, float* dweight, float* dbias, void* dstate, float* part) {
     if (bad_shape(dtype, B, L, D, taps) || !dy || !x || !weight || !dx || !dweight || !part) return VQA_ERR_ARG;
-    const int e = vqa_elem_bytes(dtype);
-    const bool vec = D % (16 / e) == 0 && vqa_vec_ok(x, x_row, e) && vqa_vec_ok(x, x_batch, e) &&
-                     vqa_vec_ok(dy, dy_row, e) && vqa_vec_ok(dy, dy_batch, e) && vqa_vec_ok(dx, D, e) &&
-                     vqa_vec_ok(state, D, e) && vqa_vec_ok(dstate, D, e) && vqa_vec_ok(dlast, D, e);
+    const int e = vqa_elem_bytes(dtype), four = 4 * e;
+    const bool vec = D % 4 == 0 && vqa_vec_ok(x, x_row, e, four) && vqa_vec_ok(x, x_batch, e, four) &&
+                     vqa_vec_ok(dy, dy_row, e, four) && vqa_vec_ok(dy, dy_batch, e, four) && vqa_vec_ok(dx, D, e, four) &&
+                     vqa_vec_ok(state, D, e, four) && vqa_vec_ok(dstate, D, e, four) && vqa_vec_ok(dlast, D, e, four);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const int rc = by_type<4>(dtype, vec, taps, silu,
+    const int rc = by_type(dtype, vec, taps, silu,
                               Bwd{st, dy, dy_batch, dy_row, dlast, x, x_batch, x_row, weight, bias, state, lengths, B, L, D,
                                   dx, dstate, part});
     if (rc != VQA_OK) return rc;
@@ -326,9 +368,9 @@ extern "C" int vqa_causal_conv_token(void* stream, int dtype, const void* x, lon
                                      long state_row, const float* weight, const float* bias, int B, int D, int taps,
                                      int silu, void* y) {
     if (bad_shape(dtype, B, 1, D, taps) || !x || !state || !weight || !y) return VQA_ERR_ARG;
-    const int e = vqa_elem_bytes(dtype);
-    const bool vec = D % (16 / e) == 0 && vqa_vec_ok(x, x_batch, e) && vqa_vec_ok(state, state_batch, e) &&
-                     vqa_vec_ok(state, state_row, e) && vqa_vec_ok(y, D, e);
-    return by_type<8>(dtype, vec, taps, silu,
+    const int e = vqa_elem_bytes(dtype), four = 4 * e;
+    const bool vec = D % 4 == 0 && vqa_vec_ok(x, x_batch, e, four) && vqa_vec_ok(state, state_batch, e, four) &&
+                     vqa_vec_ok(state, state_row, e, four) && vqa_vec_ok(y, D, e, four);
+    return by_type(dtype, vec, taps, silu,
                       Token{static_cast<hipStream_t>(stream), x, x_batch, state, state_batch, state_row, weight, bias, B, D, y});
 }

@@ -758,63 +758,66 @@ __global__ __launch_bounds__(256) void scan_shared(const float* __restrict__ par
     (e < N ? db[row * N + e] : dc[row * N + e - N]) = from_f32<T>(s);
 }
 
-// One token: a lane takes four states of a channel, LN lanes a channel.  Bound by the state's bytes, read and written once.
+// One token: a lane takes four states of a channel, LN lanes a channel, 256 / LN channels of one sequence a workgroup.  Bound
+// by the state's bytes, read and written once.
 template <typename T, int LN, bool VEC>
 __global__ __launch_bounds__(256) void scan_token(Rows x, float* __restrict__ state, long state_batch, Rows dt, Rows gate,
                                                   Rows b, Rows c, const float* __restrict__ a,
                                                   const float* __restrict__ skip, const float* __restrict__ dt_bias,
-                                                  int softplus, int B, int D, int N, int G, T* __restrict__ y) {
-    const long id = (long)blockIdx.x * 256 + threadIdx.x;
-    const int part = (int)(id % LN);
-    const long ch = id / LN;
-    if (ch >= (long)B * D) return;                         // (whole channels: the LN lanes stay together)
-    const int d = (int)(ch % D), bi = (int)(ch / D), g = d / (D / G), n0 = part * 4;
-    const T* bp = static_cast<const T*>(b.p) + bi * b.batch + (long)g * N;
-    const T* cp = static_cast<const T*>(c.p) + bi * c.batch + (long)g * N;
+                                                  int softplus, int D, int N, int per, int blocks, T* __restrict__ y) {
+    const int bi = blockIdx.x / blocks, d = (blockIdx.x - bi * blocks) * (256 / LN) + threadIdx.x / LN;
+    const int part = threadIdx.x % LN, n0 = part * 4;
+    if (d >= D) return;                                    // (whole channels: the LN lanes stay together)
+    const long shared = per == D ? 0 : (long)(d / per) * N;
+    const T* bp = static_cast<const T*>(b.p) + bi * b.batch + shared;
+    const T* cp = static_cast<const T*>(c.p) + bi * c.batch + shared;
     float* hp = state + bi * state_batch + (long)d * N;
-    float h[4], av[4], bv[4], cv[4];
+    Raw<float, 4> h, av;
+    Raw<T, 4> bv, cv;
+    h.zero();
+    av.zero();
+    bv.zero();
+    cv.zero();
     if constexpr (VEC) {
         if (n0 < N) {
-            const float4 t = *reinterpret_cast<const float4*>(hp + n0), u = *reinterpret_cast<const float4*>(a + (long)d * N + n0);
-            h[0] = t.x; h[1] = t.y; h[2] = t.z; h[3] = t.w;
-            av[0] = u.x; av[1] = u.y; av[2] = u.z; av[3] = u.w;
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) h[k] = av[k] = 0.f;
+            h.load(hp + n0);
+            av.load(a + (long)d * N + n0);
+            bv.load(bp + n0);
+            cv.load(cp + n0);
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            h[k] = n0 + k < N ? hp[n0 + k] : 0.f;
-            av[k] = n0 + k < N ? a[(long)d * N + n0 + k] : 0.f;
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        bv[k] = n0 + k < N ? to_f32(bp[n0 + k]) : 0.f;
-        cv[k] = n0 + k < N ? to_f32(cp[n0 + k]) : 0.f;
+        for (int k = 0; k < 4; ++k)
+            if (n0 + k < N) {
+                h.v[k] = hp[n0 + k];
+                av.v[k] = a[(long)d * N + n0 + k];
+                bv.v[k] = bp[n0 + k];
+                cv.v[k] = cp[n0 + k];
+            }
     }
     const float xv = to_f32(static_cast<const T*>(x.p)[bi * x.batch + d]);
+    const float zv = gate.p ? to_f32(static_cast<const T*>(gate.p)[bi * gate.batch + d]) : 0.f;
+    const float sk = skip ? skip[d] : 0.f;
     float step = to_f32(static_cast<const T*>(dt.p)[bi * dt.batch + d]) + (dt_bias ? dt_bias[d] : 0.f);
     if (softplus) step = softplus_f(step, exp_f(-fabsf(step)));
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        h[k] = exp_f(step * av[k]) * h[k] + step * xv * bv[k];
-        s += h[k] * cv[k];
+        h.v[k] = exp_f(step * av.v[k]) * h.v[k] + step * xv * bv.get(k);
+        s += h.v[k] * cv.get(k);
     }
     if constexpr (VEC) {
-        if (n0 < N) *reinterpret_cast<float4*>(hp + n0) = make_float4(h[0], h[1], h[2], h[3]);
+        if (n0 < N) h.store(hp + n0);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-            if (n0 + k < N) hp[n0 + k] = h[k];
+            if (n0 + k < N) hp[n0 + k] = h.v[k];
     }
 #pragma unroll
     for (int o = 1; o < LN; o <<= 1) s += __shfl_xor(s, o);
     if (part == 0) {
-        if (skip) s += skip[d] * xv;
-        if (gate.p) s *= silu_f(to_f32(static_cast<const T*>(gate.p)[bi * gate.batch + d]));
+        s += sk * xv;
+        if (gate.p) s *= silu_f(zv);
         y[(long)bi * D + d] = from_f32<T>(s);
     }
 }
@@ -987,13 +990,14 @@ namespace {
 template <typename T>
 int token(hipStream_t st, const Rows& x, float* state, long sb, const Rows& dt, const Rows& gate, const Rows& b, const Rows& c,
           const float* a, const float* skip, const float* bias, int softplus, int B, int D, int N, int G, void* y) {
-    const bool vec = N % 4 == 0 && sb % 4 == 0 && aligned16(state) && aligned16(a);
-    const int ln = N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16;
-    const unsigned grid = (unsigned)(((long)B * D * ln + 255) / 256);
+    constexpr int e = sizeof(T);
+    const bool vec = N % 4 == 0 && sb % 4 == 0 && aligned16(state) && aligned16(a) && vqa_vec_ok(b.p, b.batch, e, 4 * e) &&
+                     vqa_vec_ok(c.p, c.batch, e, 4 * e);
+    const int ln = N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16, blocks = (D * ln + 255) / 256;
 #define VQA_TOKEN(LN)                                                                                                    \
     if (ln == LN) {                                                                                                      \
-        if (vec) scan_token<T, LN, true><<<grid, 256, 0, st>>>(x, state, sb, dt, gate, b, c, a, skip, bias, softplus, B, D, N, G, static_cast<T*>(y)); \
-        else scan_token<T, LN, false><<<grid, 256, 0, st>>>(x, state, sb, dt, gate, b, c, a, skip, bias, softplus, B, D, N, G, static_cast<T*>(y));    \
+        if (vec) scan_token<T, LN, true><<<(unsigned)(B * blocks), 256, 0, st>>>(x, state, sb, dt, gate, b, c, a, skip, bias, softplus, D, N, D / G, blocks, static_cast<T*>(y)); \
+        else scan_token<T, LN, false><<<(unsigned)(B * blocks), 256, 0, st>>>(x, state, sb, dt, gate, b, c, a, skip, bias, softplus, D, N, D / G, blocks, static_cast<T*>(y));    \
     }
     VQA_TOKEN(1) VQA_TOKEN(2) VQA_TOKEN(4) VQA_TOKEN(8) VQA_TOKEN(16)
 #undef VQA_TOKEN
@@ -1006,7 +1010,7 @@ extern "C" int vqa_scan_token(void* stream, int dtype, const void* x, long x_bat
                               const void* dt, long dt_batch, const void* gate, long gate_batch, const float* a,
                               const void* b, long b_batch, const void* c, long c_batch, const float* skip,
                               const float* dt_bias, int softplus, int B, int D, int N, int G, void* y) {
-    if (bad_shape(dtype, B, 1, D, N, G) || !x || !state || !dt || !a || !b || !c || !y) return VQA_ERR_ARG;
+    if (bad_shape(dtype, B, 1, D, N, G) || D > 100000000 || !x || !state || !dt || !a || !b || !c || !y) return VQA_ERR_ARG;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const Rows rx = {x, x_batch, 0}, rd = {dt, dt_batch, 0}, rg = {gate, gate_batch, 0}, rb = {b, b_batch, 0}, rc = {c, c_batch, 0};
     if (dtype == VQA_F32) return token<float>(st, rx, state, state_batch, rd, rg, rb, rc, a, skip, dt_bias, softplus, B, D, N, G, y);

@@ -61,9 +61,9 @@ __device__ __forceinline__ float dsilu_f(float x) {
 
 static inline int vqa_elem_bytes(int dtype) { return dtype == VQA_F32 ? 4 : 2; }
 static inline bool vqa_dtype_ok(int dtype) { return dtype == VQA_F32 || dtype == VQA_BF16 || dtype == VQA_F16; }
-// a pointer whose rows start `stride` elements apart can be read 16 bytes at a time
-static inline bool vqa_vec_ok(const void* p, long stride, int elem) {
-    return ((uintptr_t)p & 15) == 0 && (stride * elem) % 16 == 0;
+// a pointer whose rows start `stride` elements apart can be read `bytes` at a time
+static inline bool vqa_vec_ok(const void* p, long stride, int elem, int bytes = 16) {
+    return ((uintptr_t)p & (bytes - 1)) == 0 && (stride * elem) % bytes == 0;
 }
 
 // Column sums of part[rows][cols] (f32) in a fixed order: 64 columns x 16 row lanes per workgroup, eight rows of each lane
