@@ -387,8 +387,8 @@ int vqa_scan_fwd(void* stream, int dtype, const void* x, long x_batch, long x_ro
 int vqa_scan_bwd(void* stream, int dtype, const void* dy, long dy_batch, long dy_row, const float* dlast, const void* x,
                  long x_batch, long x_row, const void* dt, long dt_batch, long dt_row, const void* gate, long gate_batch,
                  long gate_row, const float* a, const void* b, long b_batch, long b_row, const void* c, long c_batch,
-                 long c_row, const float* skip, const float* dt_bias, int softplus, const int* lengths, int B, int L, int D,
-                 int N, int G, const float* keep, void* dx, void* ddt, void* dgate, float* da, void* db, void* dc,
+                 long c_row, const float* skip, const float* dt_bias, int softplus, const float* state, const int* lengths,
+                 int B, int L, int D, int N, int G, const float* keep, void* dx, void* ddt, void* dgate, float* da, void* db, void* dc,
                  float* dskip, float* ddt_bias, float* dstate, float* ws);
 /* One token per sequence: x, dt, gate [B][D], b, c [B][G][N]; state [B][D][N] (batch stride given) in place. */
 int vqa_scan_token(void* stream, int dtype, const void* x, long x_batch, float* state, long state_batch, const void* dt,

@@ -16,7 +16,7 @@
 // rows are in flight meanwhile.  Sums over states are lane swaps, sums over channels DPP adds.
 // With few rows the tokens are cut into segments: a first pass finds each segment's own end state and total decay (the
 // product of decays is exp(a sum dt)), a small one chains them, and the full pass starts every segment from its true
-// state.  The backward does the same from the other end.  For the backward the forward keeps h before every tile.
+// state.  The backward does the same from the other end.  For the backward the forward keeps h before every tile but the first.
 // States in workspaces lie as [..][channel, a group's padded to per_pad][NP], NP = 16, 32 or 64 >= N.
 #include "seq.h"
 
@@ -37,7 +37,7 @@ struct Args {
     int per, per_pad, fblk, bblk;          // channels of a group, padded; forward waves, backward workgroups across it
     int segs, seg_len, bgroups;            // segments, tokens of one, batch groups of the backward
     void* y; float* last;
-    float *keep, *seg_h, *seg_dt;          // h before every tile; per segment: state, then the true incoming one; sum dt
+    float *keep, *seg_h, *seg_dt;          // h before the tiles; per segment: state, then the true incoming one; sum dt
     void *dx, *ddt, *dgate; float *part_bc, *part_p, *dstate;
 };
 
@@ -170,9 +170,14 @@ template <typename T, int CH, int NS, int VE> struct Wave {
         return c0 + off < cend && n < N ? (unsigned)(off * N + n) * 4u : BUF_OUT;
     }
     __device__ __forceinline__ void load_public(const float* s, int b, int D, int N, float (&h)[CH][NS]) const {
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+#pragma unroll
+            for (int j = 0; j < NS; ++j) h[i][j] = 0.f;
+        if (!s) return;
         int l = lane;
         asm volatile("" : "+v"(l));
-        const auto rs = buffer_of(s + ((long)b * D + c0) * N, s ? BUF_BYTES : 0);
+        const auto rs = buffer_of(s + ((long)b * D + c0) * N, BUF_BYTES);
 #pragma unroll
         for (int i = 0; i < CH; ++i)
 #pragma unroll
@@ -228,6 +233,8 @@ __device__ __forceinline__ Raw<T, 1> fetch_shared(const Rows& R, int b, int t0, 
     return buf_load<T, 1>(rs, t0 + t < te && n < N ? (t * (int)R.row + n) * (unsigned)sizeof(T) : BUF_OUT);
 }
 
+// h is kept before every tile but the first (there it is the incoming state)
+__host__ __device__ __forceinline__ int kept_tiles(int L) { return (L + TT - 1) / TT - 1; }
 __device__ __forceinline__ int length_of(const Args& A, int b) {
     return A.lengths ? max(0, min(A.L, A.lengths[b])) : A.L;
 }
@@ -274,7 +281,6 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
     const W w(A, blk / A.fblk, blk % A.fblk * W::WC);
     const int len = length_of(A, b), ts = seg * A.seg_len, te = min(A.L, ts + A.seg_len), live = min(len, te);
     const long chans = (long)A.G * A.per_pad, at_seg = ((long)b * A.segs + seg) * chans + w.p0;
-    const int ntile = (A.L + TT - 1) / TT;
     float a2[CH][NS], h[CH][NS], sum_dt[CH];
     w.lane_a(A, a2);
     w.stage_param(A.dt_bias, s_bias);
@@ -329,7 +335,8 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
         lds_order();
         if (FULL && A.gate.p) w.fetch(A.gate, b, t0, live, z);
         if (t0 + TT < te) fetch(t0 + TT);
-        if (FULL && A.keep) w.store_own(A.keep + (((long)b * ntile + t0 / TT) * chans + w.p0) * W::NP, h);
+        if (FULL && A.keep && t0 > 0)
+            w.store_own(A.keep + (((long)b * kept_tiles(A.L) + t0 / TT - 1) * chans + w.p0) * W::NP, h);
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
             float dt[CH], dtx[CH], bv[NS], cv[NS], y[CH];
@@ -516,7 +523,7 @@ __global__ __launch_bounds__(64 * BW) void scan_bwd(Args A) {
           *s_bias = s_gt + 2 * TILE, *s_skip = s_bias + W::WC, *s_db = s_part[wv], *s_dc = s_db + SH;
     const float *s_b = s_bc, *s_c = s_bc + SH;
     const long chans = (long)A.G * A.per_pad;
-    const int ntile = (A.L + TT - 1) / TT, ts = seg * A.seg_len, tend = min(A.L, ts + A.seg_len);
+    const int ts = seg * A.seg_len, tend = min(A.L, ts + A.seg_len);
     const int state_at = w.r * NS + sum16_of(w.cl >> 2);   // where this lane's value of sum16_four belongs
     float a2[CH][NS], g[CH][NS], da[CH][NS], sum_skip[W::NV][VE], sum_bias[W::NV][VE];
     w.lane_a(A, a2);
@@ -532,31 +539,57 @@ __global__ __launch_bounds__(64 * BW) void scan_bwd(Args A) {
         for (int v = 0; v < VE; ++v) sum_skip[k][v] = sum_bias[k][v] = 0.f;
     if (!live)
         for (int k = w.lane; k < 2 * SH; k += 64) s_db[k] = 0.f;
-    for (int b = group; b < A.B; b += A.bgroups) {
+    // what the next tile needs, in flight while this one is worked on: of this sequence, or of the batch group's next one
+    // that has tokens in this segment
+    Raw<T, VE> xn[W::NV], dn[W::NV], zn[W::NV], gn[W::NV];
+    Raw<T, 1> sn[NBC];
+    float hn[CH][NS];
+    auto last_tile = [&](int b) {
+        const int n = min(length_of(A, b), tend) - ts;
+        return n > 0 ? ts + (n - 1) / TT * TT : -1;
+    };
+    auto fetch = [&](int b, int t0) {
         const int te = min(length_of(A, b), tend);
+        w.fetch(A.x, b, t0, te, xn);
+        w.fetch(A.dt, b, t0, te, dn);
+        if (A.gate.p) w.fetch(A.gate, b, t0, te, zn);
+        w.fetch(A.dy, b, t0, te, gn);
+#pragma unroll
+        for (int k = 0; k < NBC; ++k) {
+            const int id = k * 64 * BW + threadIdx.x;
+            sn[k] = fetch_shared<T, W::NP>(id < SH ? A.b : A.c, b, t0, te, w.g, A.N, id % SH);
+        }
+        if (t0 > 0) w.load_own(A.keep + (((long)b * kept_tiles(A.L) + t0 / TT - 1) * chans + w.p0) * W::NP, hn);
+        else w.load_public(A.state, b, A.D, A.N, hn);
+    };
+    auto fetch_next = [&](int b) {                         // the first tile to come of sequence b or a later one
+        for (; b < A.B; b += A.bgroups)
+            if (last_tile(b) >= 0) { fetch(b, last_tile(b)); return; }
+    };
+    fetch_next(group);
+    for (int b = group; b < A.B; b += A.bgroups) {
+        const int te = min(length_of(A, b), tend), t_last = last_tile(b);
+        for (int t0 = t_last < 0 ? ts : t_last + TT; t0 < tend; t0 += TT) {      // past the end of this sequence: zero rows
+            Raw<T, VE> x[W::NV];
+#pragma unroll
+            for (int k = 0; k < W::NV; ++k) x[k].zero();
+            w.put(A.dx, b, A.L, A.D, t0, tend, x);
+            w.put(A.ddt, b, A.L, A.D, t0, tend, x);
+            if (A.gate.p) w.put(A.dgate, b, A.L, A.D, t0, tend, x);
+        }
         if (A.segs > 1) w.load_own(A.seg_h + (((long)b * A.segs + seg) * chans + w.p0) * W::NP, g);
         else w.load_public(A.dlast, b, A.D, A.N, g);
-        for (int t0 = ts + (tend - ts - 1) / TT * TT; t0 >= ts; t0 -= TT) {
+        for (int t0 = t_last; t0 >= ts; t0 -= TT) {
             Raw<T, VE> x[W::NV], d[W::NV], z[W::NV], gy[W::NV];
-            if (t0 >= te) {                                // past the end of this sequence: zero rows
-#pragma unroll
-                for (int k = 0; k < W::NV; ++k) x[k].zero();
-                w.put(A.dx, b, A.L, A.D, t0, tend, x);
-                w.put(A.ddt, b, A.L, A.D, t0, tend, x);
-                if (A.gate.p) w.put(A.dgate, b, A.L, A.D, t0, tend, x);
-                continue;
-            }
             float hist[TT][CH][NS], h[CH][NS];
-            w.load_own(A.keep + (((long)b * ntile + t0 / TT) * chans + w.p0) * W::NP, h);
-            w.fetch(A.x, b, t0, te, x);
-            w.fetch(A.dt, b, t0, te, d);
-            if (A.gate.p) w.fetch(A.gate, b, t0, te, z);
-            w.fetch(A.dy, b, t0, te, gy);
 #pragma unroll
-            for (int k = 0; k < NBC; ++k) {
-                const int id = k * 64 * BW + threadIdx.x;
-                s_bc[id] = fetch_shared<T, W::NP>(id < SH ? A.b : A.c, b, t0, te, w.g, A.N, id % SH).get(0);
-            }
+            for (int k = 0; k < W::NV; ++k) { x[k] = xn[k]; d[k] = dn[k]; z[k] = zn[k]; gy[k] = gn[k]; }
+#pragma unroll
+            for (int i = 0; i < CH; ++i)
+#pragma unroll
+                for (int j = 0; j < NS; ++j) h[i][j] = hn[i][j];
+#pragma unroll
+            for (int k = 0; k < NBC; ++k) s_bc[k * 64 * BW + threadIdx.x] = sn[k].get(0);
             float step[W::NV][VE], slope[W::NV][VE], sig[W::NV][VE], dcore[W::NV][VE];
             if (live) {
                 stage_steps<true>(w, d, s_bias, A.softplus, t0, te, step, slope);
@@ -583,6 +616,7 @@ __global__ __launch_bounds__(64 * BW) void scan_bwd(Args A) {
                     }
             }
             __syncthreads();                               // b, c are there; the last tile's s_part has been read
+            if (t0 > ts) fetch(b, t0 - TT); else fetch_next(b + A.bgroups);
             if (live) {
 #pragma unroll
                 for (int t = 0; t < TT; ++t) {
@@ -914,7 +948,7 @@ extern "C" int vqa_scan_ws_bytes(int dtype, int B, int L, int D, int N, int G, l
     A.B = B; A.L = L; A.D = D; A.N = N; A.G = G;
     plan(A);
     sizes[0] = 4 * seg_floats(A);
-    sizes[1] = 4L * B * ((L + TT - 1) / TT) * G * A.per_pad * np_of(N);
+    sizes[1] = 4L * B * kept_tiles(L) * G * A.per_pad * np_of(N);
     sizes[2] = 4 * (seg_floats(A) + part_p_floats(A) + part_bc_floats(A));
     return VQA_OK;
 }
@@ -944,17 +978,17 @@ extern "C" int vqa_scan_bwd(void* stream, int dtype, const void* dy, long dy_bat
                             const void* x, long x_batch, long x_row, const void* dt, long dt_batch, long dt_row,
                             const void* gate, long gate_batch, long gate_row, const float* a, const void* b, long b_batch,
                             long b_row, const void* c, long c_batch, long c_row, const float* skip, const float* dt_bias,
-                            int softplus, const int* lengths, int B, int L, int D, int N, int G, const float* keep,
-                            void* dx, void* ddt, void* dgate, float* da, void* db, void* dc, float* dskip,
+                            int softplus, const float* state, const int* lengths, int B, int L, int D, int N, int G,
+                            const float* keep, void* dx, void* ddt, void* dgate, float* da, void* db, void* dc, float* dskip,
                             float* ddt_bias, float* dstate, float* ws) {
-    if (bad_shape(dtype, B, L, D, N, G) || !dy || !x || !dt || !a || !b || !c || !keep || !dx || !ddt || !da || !db ||
+    if (bad_shape(dtype, B, L, D, N, G) || !dy || !x || !dt || !a || !b || !c || (!keep && L > TT) || !dx || !ddt || !da || !db ||
         !dc || !ws || (gate && !dgate) || !aligned16(ws) || !aligned16(keep))
         return VQA_ERR_ARG;
     Args A = {};
     A.dy = {dy, dy_batch, dy_row};
     A.x = {x, x_batch, x_row}; A.dt = {dt, dt_batch, dt_row}; A.gate = {gate, gate_batch, gate_row};
     A.b = {b, b_batch, b_row}; A.c = {c, c_batch, c_row};
-    A.a = a; A.skip = skip; A.dt_bias = dt_bias; A.dlast = dlast; A.lengths = lengths; A.softplus = softplus;
+    A.a = a; A.skip = skip; A.dt_bias = dt_bias; A.dlast = dlast; A.state = state; A.lengths = lengths; A.softplus = softplus;
     A.B = B; A.L = L; A.D = D; A.N = N; A.G = G; A.keep = const_cast<float*>(keep);
     A.dx = dx; A.ddt = ddt; A.dgate = dgate; A.dstate = dstate;
     if (far_rows(A)) return VQA_ERR_ARG;

@@ -66,35 +66,35 @@ static inline bool vqa_vec_ok(const void* p, long stride, int elem, int bytes = 
     return ((uintptr_t)p & (bytes - 1)) == 0 && (stride * elem) % bytes == 0;
 }
 
-// Column sums of part[rows][cols] (f32) in a fixed order: 64 columns x 16 row lanes per workgroup, eight rows of each lane
+// Column sums of part[rows][cols] (f32) in a fixed order: 32 columns x 32 row lanes per workgroup, eight rows of each lane
 // in flight, the lanes joined through LDS.  Column c of the first `n0` goes to out0[c], the rest to out1[c - n0].
 __global__ __launch_bounds__(1024) static void seq_column_sums(const float* __restrict__ part, int rows, long cols,
                                                                float* __restrict__ out0, long n0,
                                                                float* __restrict__ out1) {
-    const long c = (long)blockIdx.x * 64 + (threadIdx.x & 63);
-    const int lane_row = threadIdx.x >> 6;
+    const int lc = threadIdx.x & 31, lane_row = threadIdx.x >> 5;
+    const long c = (long)blockIdx.x * 32 + lc;
     float acc[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) acc[u] = 0.f;
     if (c < cols) {
-        for (int r = lane_row; r < rows; r += 128) {
+        for (int r = lane_row; r < rows; r += 256) {
 #pragma unroll
             for (int u = 0; u < 8; ++u)
-                if (r + 16 * u < rows) acc[u] += part[(long)(r + 16 * u) * cols + c];
+                if (r + 32 * u < rows) acc[u] += part[(long)(r + 32 * u) * cols + c];
         }
     }
-    __shared__ float s[16][64];
-    s[lane_row][threadIdx.x & 63] = ((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7]));
+    __shared__ float s[32][33];
+    s[lane_row][lc] = ((acc[0] + acc[1]) + (acc[2] + acc[3])) + ((acc[4] + acc[5]) + (acc[6] + acc[7]));
     __syncthreads();
     if (lane_row == 0 && c < cols) {
         float t = 0.f;
 #pragma unroll
-        for (int u = 0; u < 16; ++u) t += s[u][threadIdx.x];
+        for (int u = 0; u < 32; ++u) t += s[u][lc];
         if (c < n0) { if (out0) out0[c] = t; }
         else if (out1) out1[c - n0] = t;
     }
 }
 static inline void seq_sum_columns(hipStream_t st, const float* part, int rows, long cols, float* out0, long n0,
                                    float* out1) {
-    seq_column_sums<<<(unsigned)((cols + 63) / 64), 1024, 0, st>>>(part, rows, cols, out0, n0, out1);
+    seq_column_sums<<<(unsigned)((cols + 31) / 32), 1024, 0, st>>>(part, rows, cols, out0, n0, out1);
 }

@@ -350,14 +350,14 @@ class _SelectiveScan(torch.autograd.Function):
     def forward(ctx, x, dt, a, b, c, skip, gate, dt_bias, softplus, state, lengths, want_last):
         with _device_of(x):
             y, last, keep = _scan_fwd(x, dt, a, b, c, skip, gate, dt_bias, softplus, state, lengths, want_last, True)
-        ctx.save_for_backward(x, dt, a, b, c, skip, gate, dt_bias, lengths, keep)
-        ctx.softplus, ctx.has_state = softplus, state is not None
+        ctx.save_for_backward(x, dt, a, b, c, skip, gate, dt_bias, state, lengths, keep)
+        ctx.softplus = softplus
         ctx.set_materialize_grads(False)
         return y, last
 
     @_backward
     def backward(ctx, dy, dlast):
-        x, dt, a, b, c, skip, gate, dt_bias, lengths, keep = ctx.saved_tensors
+        x, dt, a, b, c, skip, gate, dt_bias, state, lengths, keep = ctx.saved_tensors
         B, T, D = x.shape
         G, N, dev, code = b.shape[2], b.shape[3], x.device, L.dt(x)
         f32 = lambda *s: torch.empty(*s, device=dev, dtype=_F32)       # noqa: E731
@@ -367,7 +367,7 @@ class _SelectiveScan(torch.autograd.Function):
             dx, ddt, dgate = rows(B, T, D), rows(B, T, D), rows(B, T, D) if gate is not None else None
             db, dc, da = rows(B, T, G, N), rows(B, T, G, N), f32(D, N)
             dskip, dbias = f32(D) if skip is not None else None, f32(D) if dt_bias is not None else None
-            dstate = f32(B, D, N) if ctx.has_state else None
+            dstate = f32(B, D, N) if state is not None else None
             if not dx.numel():
                 for g in (da, dskip, dbias):
                     if g is not None:
@@ -379,7 +379,7 @@ class _SelectiveScan(torch.autograd.Function):
                 ws = _floats(_scan_bytes(code, B, T, D, N, G)[2], dev)
                 L.call('vqa_scan_bwd', code, dy, dy.stride(0), dy.stride(1), dlast, x, x.stride(0), x.stride(1), dt,
                        dt.stride(0), dt.stride(1), gate, *_strides(gate), a, b, b.stride(0), b.stride(1), c,
-                       c.stride(0), c.stride(1), skip, dt_bias, ctx.softplus, lengths, B, T, D, N, G, keep, dx, ddt,
+                       c.stride(0), c.stride(1), skip, dt_bias, ctx.softplus, state, lengths, B, T, D, N, G, keep, dx, ddt,
                        dgate, da, db, dc, dskip, dbias, dstate, ws)
         return dx, ddt, da, db, dc, dskip, dgate, dbias, None, dstate, None, None
 
