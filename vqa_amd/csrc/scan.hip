@@ -505,14 +505,17 @@ __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
 // The backward.  Tiles from the last to the first; inside a tile the states are computed again from the kept one, forwards,
 // staying in registers (h before each of the TT tokens), then the adjoint runs backwards over them.  Those TT CH NS
 // registers are why a lane has half the forward's channels: at 16 states a lane they do not fit, and the spills cost more
-// than all the rest (566 us against 88 of the forward at 4 x 2048 tokens x 2048 channels).
+// than all the rest (566 us against 88 of the forward at 4 x 2048 tokens x 2048 channels, N = 16, bf16; this form: 231).  What
+// two waves a SIMD leave of 256 registers keeps the decays of a tile's last KD tokens for the way back (five: 251 -> 231 us;
+// with a sixth one wave fits, 308 us); the other tokens' are formed again.  The vector ALU is busy 3/4 of the time.
 // The BW waves of a workgroup take neighbouring channels, share b and c in LDS and join their sums db, dc over channels
 // there: part_bc[workgroup of the group][B][L][G][2][N].  A workgroup takes the sequences of its batch group one after the
 // other, so that its sums over tokens leave once: part_p[(batch group, segment)]{da [channel][NP], dskip, ddt_bias}.
 template <typename T, int CH, int NS, int VE>
-__global__ __launch_bounds__(64 * BW) void scan_bwd(Args A) {
+__global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A) {
     typedef Wave<T, CH, NS, VE> W;
-    constexpr int TILE = TT * W::WC, SH = TT * W::NP, NBC = 2 * SH / (64 * BW);
+    constexpr int TILE = TT * W::WC, SH = TT * W::NP, NBC = 2 * SH / (64 * BW), 
+                  KD = CH * NS > 8 ? 0 : CH == 1 || (VE > 1 && sizeof(T) == 2) ? 5 : VE > 1 ? 2 : 0;
     __shared__ __attribute__((aligned(16))) float lds[BW][6 * TILE + 2 * W::WC], s_bc[2 * SH], s_part[BW][2 * SH];
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int blks = A.bblk * A.G;
@@ -581,7 +584,7 @@ __global__ __launch_bounds__(64 * BW) void scan_bwd(Args A) {
         else w.load_public(A.dlast, b, A.D, A.N, g);
         for (int t0 = t_last; t0 >= ts; t0 -= TT) {
             Raw<T, VE> x[W::NV], d[W::NV], z[W::NV], gy[W::NV];
-            float hist[TT][CH][NS], h[CH][NS];
+            float hist[TT][CH][NS], h[CH][NS], kd[KD > 0 ? KD : 1][CH][NS];
 #pragma unroll
             for (int k = 0; k < W::NV; ++k) { x[k] = xn[k]; d[k] = dn[k]; z[k] = zn[k]; gy[k] = gn[k]; }
 #pragma unroll
@@ -634,7 +637,9 @@ __global__ __launch_bounds__(64 * BW) void scan_bwd(Args A) {
 #pragma unroll
                         for (int j = 0; j < NS; ++j) {
                             hist[t][i][j] = h[i][j];
-                            h[i][j] = __builtin_amdgcn_exp2f(dt[i] * a2[i][j]) * h[i][j] + dtx[i] * bv[j];
+                            const float decay = __builtin_amdgcn_exp2f(dt[i] * a2[i][j]);
+                            if (t >= TT - KD) kd[t >= TT - KD ? t - (TT - KD) : 0][i][j] = decay;
+                            h[i][j] = decay * h[i][j] + dtx[i] * bv[j];
                             y[i] += h[i][j] * cv[j];
                             sc[j] += h[i][j] * dc[i];
                         }
@@ -663,7 +668,8 @@ __global__ __launch_bounds__(64 * BW) void scan_bwd(Args A) {
                             const float G = g[i][j] + dc[i] * cv[j];
                             gb[i] += G * bv[j];
                             sb[j] += G * dtx[i];
-                            g[i][j] = G * __builtin_amdgcn_exp2f(dt[i] * a2[i][j]);
+                            g[i][j] = G * (t >= TT - KD ? kd[t >= TT - KD ? t - (TT - KD) : 0][i][j]
+                                                        : __builtin_amdgcn_exp2f(dt[i] * a2[i][j]));
                             const float th = g[i][j] * hist[t][i][j];
                             ta[i] += th * a2[i][j];
                             da[i][j] += th * dt[i];
