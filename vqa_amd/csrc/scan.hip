@@ -225,12 +225,20 @@ template <typename T, int CH, int NS, int VE> struct Wave {
     }
 };
 
-// b or c of a tile: element id = token * NP + state of [TT][NP], 0 past the tokens and the states
+// b or c of a tile: element id = token * NP + state of [TT][NP], 0 past the tokens and the states.  The bits stay in a
+// register each until they are used: two 16-bit values in an array would be packed into one register as soon as they are
+// loaded, which waits for them where they were meant to be in flight.
 template <typename T, int NP>
-__device__ __forceinline__ Raw<T, 1> fetch_shared(const Rows& R, int b, int t0, int te, int g, int N, int id) {
+__device__ __forceinline__ unsigned fetch_shared(const Rows& R, int b, int t0, int te, int g, int N, int id) {
     const auto rs = buffer_of(static_cast<const T*>(R.p) + b * R.batch + t0 * R.row + (long)g * N, BUF_BYTES);
     const int t = id / NP, n = id % NP;
-    return buf_load<T, 1>(rs, t0 + t < te && n < N ? (t * (int)R.row + n) * (unsigned)sizeof(T) : BUF_OUT);
+    const unsigned off = t0 + t < te && n < N ? (t * (int)R.row + n) * (unsigned)sizeof(T) : BUF_OUT;
+    if constexpr (sizeof(T) == 4) return __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0);
+    else return __builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, 0);
+}
+template <typename T> __device__ __forceinline__ float shared_value(unsigned bits) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(bits);
+    else return to_f32(__builtin_bit_cast(T, (unsigned short)bits));
 }
 
 // h is kept before every tile but the first (there it is the incoming state)
@@ -296,7 +304,7 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
         else w.load_public(A.state, b, A.D, A.N, h);
     }
     Raw<T, VE> x[W::NV], d[W::NV], z[W::NV], xn[W::NV], dn[W::NV];
-    Raw<T, 1> bn[NBC], cn[NBC];
+    unsigned bn[NBC], cn[NBC];
     auto fetch = [&](int t0) {
         w.fetch(A.x, b, t0, live, xn);
         w.fetch(A.dt, b, t0, live, dn);
@@ -329,8 +337,8 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
             }
 #pragma unroll
         for (int k = 0; k < NBC; ++k) {
-            s_b[k * 64 + w.lane] = bn[k].get(0);
-            if (FULL) s_c[k * 64 + w.lane] = cn[k].get(0);
+            s_b[k * 64 + w.lane] = shared_value<T>(bn[k]);
+            if (FULL) s_c[k * 64 + w.lane] = shared_value<T>(cn[k]);
         }
         lds_order();
         if (FULL && A.gate.p) w.fetch(A.gate, b, t0, live, z);
@@ -444,7 +452,7 @@ __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
         for (int j = 0; j < NS; ++j) g[i][j] = 0.f;
     }
     Raw<T, VE> dn[W::NV], zn[W::NV], gn[W::NV];
-    Raw<T, 1> cn[NBC];
+    unsigned cn[NBC];
     auto fetch = [&](int t0) {
         w.fetch(A.dt, b, t0, te, dn);
         if (A.gate.p) w.fetch(A.gate, b, t0, te, zn);
@@ -476,7 +484,7 @@ __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
                 s_g[w.tat(k) + v] = dcore[k][v];
             }
 #pragma unroll
-        for (int k = 0; k < NBC; ++k) s_c[k * 64 + w.lane] = cn[k].get(0);
+        for (int k = 0; k < NBC; ++k) s_c[k * 64 + w.lane] = shared_value<T>(cn[k]);
         lds_order();
         if (t0 > ts) fetch(t0 - TT);
 #pragma unroll
@@ -545,7 +553,7 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
     // what the next tile needs, in flight while this one is worked on: of this sequence, or of the batch group's next one
     // that has tokens in this segment
     Raw<T, VE> xn[W::NV], dn[W::NV], zn[W::NV], gn[W::NV];
-    Raw<T, 1> sn[NBC];
+    unsigned sn[NBC];
     float hn[CH][NS];
     auto last_tile = [&](int b) {
         const int n = min(length_of(A, b), tend) - ts;
@@ -592,7 +600,7 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
 #pragma unroll
                 for (int j = 0; j < NS; ++j) h[i][j] = hn[i][j];
 #pragma unroll
-            for (int k = 0; k < NBC; ++k) s_bc[k * 64 * BW + threadIdx.x] = sn[k].get(0);
+            for (int k = 0; k < NBC; ++k) s_bc[k * 64 * BW + threadIdx.x] = shared_value<T>(sn[k]);
             float step[W::NV][VE], slope[W::NV][VE], sig[W::NV][VE], dcore[W::NV][VE];
             if (live) {
                 stage_steps<true>(w, d, s_bias, A.softplus, t0, te, step, slope);
