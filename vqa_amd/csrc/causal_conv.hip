@@ -22,7 +22,7 @@ __global__ __launch_bounds__(256) void conv_fwd(const T* __restrict__ x, long xb
     const int nv = (D + V - 1) / V, nchunk = (L + chunk - 1) / chunk;
     const long id = (long)blockIdx.x * 256 + threadIdx.x;
     if (id >= (long)B * nchunk * nv) return;
-    const int c = (int)(id % nv) * V;
+    const int c = min((int)(id % nv) * V, D - V);          // (the last vector of an odd width overlaps: twice the same results)
     const int q = (int)(id / nv);
     const int b = q / nchunk, t0 = (q % nchunk) * chunk, t1 = min(L, t0 + chunk);
     const int len = lengths ? max(0, min(L, lengths[b])) : L;
@@ -90,8 +90,8 @@ __global__ __launch_bounds__(256) void conv_bwd(const T* __restrict__ dy, long g
     __shared__ float acc[256 * V];
     const int nchunk = (L + chunk - 1) / chunk, ly = 256 / lx;
     const int lane = threadIdx.x % lx, team = threadIdx.x / lx;
-    const int c = (blockIdx.x * lx + lane) * V;
-    const bool on = c < D;
+    const bool on = (blockIdx.x * lx + lane) * V < D;
+    const int c = min((int)(blockIdx.x * lx + lane) * V, D - V);      // (as in conv_fwd)
     float wk[W][V], bv[V], aw[W][V], ab[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -120,11 +120,8 @@ __global__ __launch_bounds__(256) void conv_bwd(const T* __restrict__ dy, long g
         }
         // step s takes in g_s and gives out the gradient of row s - (W - 1): the first chunk begins with the state's rows
         const int end = t1 + W - 1;
-        auto step = [&](int s) {                           // one row with every guard
-            Raw<T, V> rx, rg, o;
-            rx.zero();
-            rg.zero();
-            if (s < len) { rx.load(xr + s * xl); rg.load(gr + s * gl); }
+        auto step = [&](int s, const Raw<T, V>& rx, const Raw<T, V>& rg) {     // one row with every guard
+            Raw<T, V> o;
             const int t = s - (W - 1), r = s - len;        // row answered; its place among the rows handed on
             float e[V];
 #pragma unroll
@@ -157,11 +154,23 @@ __global__ __launch_bounds__(256) void conv_bwd(const T* __restrict__ dy, long g
             if (t >= t0) o.store(dx + ((long)b * L + t) * D + c);
             else if (t < 0 && dstate) o.store(dstate + ((long)b * (W - 1) + s) * D + c);
         };
-        int s = t0;
-        for (; s < min(end, t0 + W - 1); ++s) step(s);
+        constexpr int U = W == 3 ? 3 : 4;
+        auto some = [&](int from, int to) {                // up to U rows of them, loaded together
+            Raw<T, V> rx[U], rg[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                rx[i].zero();
+                rg[i].zero();
+                if (from + i < min(to, len)) { rx[i].load(xr + (from + i) * xl); rg[i].load(gr + (from + i) * gl); }
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+                if (from + i < to) step(from + i, rx[i], rg[i]);
+        };
+        int s = t0 + W - 1;
+        some(t0, s);
         // the body: rows that are the chunk's own, before the sequence's end, and answer one of the chunk's.  U rows at a
         // time, the next U in flight; the windows turn instead of moving (U is a multiple of W)
-        constexpr int U = W == 3 ? 3 : 4;
         const int body = min(t1, len) - U;
         if (s <= body) {
             Raw<T, V> nx[U], ng[U];
@@ -198,7 +207,7 @@ __global__ __launch_bounds__(256) void conv_bwd(const T* __restrict__ dy, long g
                 }
             }
         }
-        for (; s < end; ++s) step(s);
+        for (; s < end; s += U) some(s, min(s + U, end));
     }
     // the chunks that this workgroup worked on side by side are joined in a fixed order
     float* out = part + (long)blockIdx.y * (W + 1) * D;
@@ -291,8 +300,8 @@ struct Fwd {
 struct Grid { int lx, gx, gy, chunk; };
 Grid bwd_grid(int B, int L, int D, int V) {
     const int nv = (D + V - 1) / V;
-    int lx = 8;
-    while (lx < 64 && lx < nv) lx *= 2;
+    int lx = 64;                                           // a row's pieces as long as a quarter of idle lanes allows
+    while (lx > 8 && (nv + lx - 1) / lx * lx > nv + nv / 4) lx /= 2;
     const int gx = (nv + lx - 1) / lx, ly = 256 / lx;
     int chunk = 128;
     while (chunk > 8 && (long)B * ((L + chunk - 1) / chunk) * gx * lx < 100000) chunk /= 2;
@@ -332,10 +341,7 @@ extern "C" int vqa_causal_conv_fwd(void* stream, int dtype, const void* x, long 
                                    const float* bias, const void* state, const int* lengths, int B, int L, int D,
                                    int taps, int silu, void* y, void* last) {
     if (bad_shape(dtype, B, L, D, taps) || !x || !weight || !y) return VQA_ERR_ARG;
-    const int e = vqa_elem_bytes(dtype), four = 4 * e;
-    const bool vec = D % 4 == 0 && vqa_vec_ok(x, x_row, e, four) && vqa_vec_ok(x, x_batch, e, four) && vqa_vec_ok(y, D, e, four) &&
-                     vqa_vec_ok(state, D, e, four) && vqa_vec_ok(last, D, e, four);
-    return by_type(dtype, vec, taps, silu,
+    return by_type(dtype, D >= 4, taps, silu,
                       Fwd{static_cast<hipStream_t>(stream), x, x_batch, x_row, weight, bias, state, lengths, B, L, D, y, last});
 }
 
@@ -350,16 +356,12 @@ extern "C" int vqa_causal_conv_bwd(void* stream, int dtype, const void* dy, long
                                    const void* state, const int* lengths, int B, int L, int D, int taps, int silu,
                                    void* dx, float* dweight, float* dbias, void* dstate, float* part) {
     if (bad_shape(dtype, B, L, D, taps) || !dy || !x || !weight || !dx || !dweight || !part) return VQA_ERR_ARG;
-    const int e = vqa_elem_bytes(dtype), four = 4 * e;
-    const bool vec = D % 4 == 0 && vqa_vec_ok(x, x_row, e, four) && vqa_vec_ok(x, x_batch, e, four) &&
-                     vqa_vec_ok(dy, dy_row, e, four) && vqa_vec_ok(dy, dy_batch, e, four) && vqa_vec_ok(dx, D, e, four) &&
-                     vqa_vec_ok(state, D, e, four) && vqa_vec_ok(dstate, D, e, four) && vqa_vec_ok(dlast, D, e, four);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const int rc = by_type(dtype, vec, taps, silu,
+    const int rc = by_type(dtype, D >= 4, taps, silu,
                               Bwd{st, dy, dy_batch, dy_row, dlast, x, x_batch, x_row, weight, bias, state, lengths, B, L, D,
                                   dx, dstate, part});
     if (rc != VQA_OK) return rc;
-    seq_sum_columns(st, part, bwd_grid(B, L, D, vec ? 4 : 1).gy, (long)(taps + 1) * D, dweight, (long)taps * D, dbias);
+    seq_sum_columns(st, part, bwd_grid(B, L, D, D >= 4 ? 4 : 1).gy, (long)(taps + 1) * D, dweight, (long)taps * D, dbias);
     CHECK_LAUNCH();
     return VQA_OK;
 }
@@ -368,9 +370,6 @@ extern "C" int vqa_causal_conv_token(void* stream, int dtype, const void* x, lon
                                      long state_row, const float* weight, const float* bias, int B, int D, int taps,
                                      int silu, void* y) {
     if (bad_shape(dtype, B, 1, D, taps) || !x || !state || !weight || !y) return VQA_ERR_ARG;
-    const int e = vqa_elem_bytes(dtype), four = 4 * e;
-    const bool vec = D % 4 == 0 && vqa_vec_ok(x, x_batch, e, four) && vqa_vec_ok(state, state_batch, e, four) &&
-                     vqa_vec_ok(state, state_row, e, four) && vqa_vec_ok(y, D, e, four);
-    return by_type(dtype, vec, taps, silu,
-                      Token{static_cast<hipStream_t>(stream), x, x_batch, state, state_batch, state_row, weight, bias, B, D, y});
+    return by_type(dtype, D % 4 == 0, taps, silu,            // (in place: no two threads may take the same channel)
+                   Token{static_cast<hipStream_t>(stream), x, x_batch, state, state_batch, state_row, weight, bias, B, D, y});
 }

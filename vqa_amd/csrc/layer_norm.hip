@@ -26,7 +26,8 @@ template <int TEAM> __device__ __forceinline__ void team_sum2(float& a, float& b
     }
 }
 
-template <typename T, int V, int TEAM, int NV>
+// A row is NV vectors of V elements a lane and, where V does not divide the width, one more element of its first lanes.
+template <typename T, int V, int TEAM, int NV, bool TAIL>
 __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_fwd(const T* __restrict__ x, long ldx,
                                                                   const float* __restrict__ w,
                                                                   const float* __restrict__ bias, long rows, int width,
@@ -34,36 +35,42 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_fwd(const T* __res
                                                                   float* __restrict__ mean, float* __restrict__ rstd) {
     __shared__ float2 sh[2][TEAM / 64];
     int half = 0;
-    const int lane = threadIdx.x % TEAM;
+    const int lane = threadIdx.x % TEAM, main = TAIL ? width - width % V : width;
+    const bool tail = TAIL && lane < width - main;
     const long row = (long)blockIdx.x * (TEAM == 64 ? 4 : 1) + (TEAM == 64 ? threadIdx.x / 64 : 0);
     if (row >= rows) return;                               // (whole waves; only where a team is one wave)
     Raw<T, V> r[NV];
+    Raw<T, 1> rt;
     float sum = 0.f, zero = 0.f;
+    rt.zero();
+    if (tail) rt.load(x + row * ldx + main + lane);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * TEAM + lane) * V;
-        if (c < width) r[i].load(x + row * ldx + c); else r[i].zero();
+        if (c < main) r[i].load(x + row * ldx + c); else r[i].zero();
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int k = 0; k < V; ++k) sum += r[i].get(k);
+    if (TAIL) sum += rt.get(0);
     team_sum2<TEAM>(sum, zero, sh, half);
     const float mu = sum / width;
     float sq = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-        if ((i * TEAM + lane) * V < width) {
+        if ((i * TEAM + lane) * V < main) {
 #pragma unroll
             for (int k = 0; k < V; ++k) { const float d = r[i].get(k) - mu; sq += d * d; }
         }
+    if (tail) sq += (rt.get(0) - mu) * (rt.get(0) - mu);
     team_sum2<TEAM>(sq, zero, sh, half);
     const float rs = 1.f / sqrtf(sq / width + eps);
     if (lane == 0 && mean) { mean[row] = mu; rstd[row] = rs; }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int c = (i * TEAM + lane) * V;
-        if (c < width) {
+        if (c < main) {
             Raw<float, V> wv, bv;
             if (w) wv.load(w + c);
             if (bias) bv.load(bias + c);
@@ -78,9 +85,15 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_fwd(const T* __res
             o.store(y + row * width + c);
         }
     }
+    if (tail) {
+        const int c = main + lane;
+        const float v = (rt.get(0) - mu) * rs * (w ? w[c] : 1.f) + (bias ? bias[c] : 0.f);
+        rt.set(0, v);
+        rt.store(y + row * width + c);
+    }
 }
 
-template <typename T, int V, int TEAM, int NV>
+template <typename T, int V, int TEAM, int NV, bool TAIL>
 __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_bwd(const T* __restrict__ dy, long lddy,
                                                                   const T* __restrict__ x, long ldx,
                                                                   const float* __restrict__ w,
@@ -91,19 +104,23 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_bwd(const T* __res
     __shared__ float2 sh[2][TEAM / 64];
     int half = 0;
     const int lane = threadIdx.x % TEAM, team = TEAM == 64 ? threadIdx.x / 64 : 0;
-    float wv[NV][V], aw[NV][V], ab[NV][V];
+    const int main = TAIL ? width - width % V : width;
+    const bool tail = TAIL && lane < width - main;
+    float wv[NV][V], aw[NV][V], ab[NV][V], wt = 0.f, awt = 0.f, abt = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const int c = (i * TEAM + lane) * V + k;
-            wv[i][k] = c < width ? (w ? w[c] : 1.f) : 0.f;
+            wv[i][k] = c < main ? (w ? w[c] : 1.f) : 0.f;
             aw[i][k] = ab[i][k] = 0.f;
         }
+    if (tail) wt = w ? w[main + lane] : 1.f;
     const float inv = 1.f / width;
     const long step = (long)gridDim.x * TEAMS;
     long row = (long)blockIdx.x * TEAMS + team;
     Raw<T, V> xr[NV], gr[NV], xn[NV], gn[NV];
+    T xt, gt, xnt = from_f32<T>(0.f), gnt = from_f32<T>(0.f);
     float mu = 0.f, rs = 0.f, mun = 0.f, rsn = 0.f;
     auto fetch = [&](long at) {                            // the next row is in flight while this one is worked on
 #pragma unroll
@@ -111,14 +128,23 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_bwd(const T* __res
             const int c = (i * TEAM + lane) * V;
             xn[i].zero();
             gn[i].zero();
-            if (at < rows && c < width) { xn[i].load(x + at * ldx + c); gn[i].load(dy + at * lddy + c); }
+            if (at < rows && c < main) { xn[i].load(x + at * ldx + c); gn[i].load(dy + at * lddy + c); }
         }
-        if (at < rows) { mun = mean[at]; rsn = rstd[at]; }
+        if constexpr (TAIL) {
+            xnt = gnt = from_f32<T>(0.f);
+            if (at < rows && tail) { xnt = x[at * ldx + main + lane]; gnt = dy[at * lddy + main + lane]; }
+        }
+        // (conditional values, not conditional stores: those were sunk into stores through a chosen address, and the
+        // variables went to scratch memory)
+        mun = at < rows ? mean[at] : 0.f;
+        rsn = at < rows ? rstd[at] : 0.f;
     };
     fetch(row);
     for (; row < rows; row += step) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) { xr[i] = xn[i]; gr[i] = gn[i]; }
+        xt = xnt;
+        gt = gnt;
         mu = mun;
         rs = rsn;
         fetch(row + step);
@@ -133,13 +159,20 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_bwd(const T* __res
                 aw[i][k] += d * xh;
                 ab[i][k] += d;
             }
+        if (TAIL) {
+            const float xh = (to_f32(xt) - mu) * rs, d = to_f32(gt), g = d * wt;
+            s1 += g;
+            s2 += tail ? g * xh : 0.f;                     // (mu or rs may not be finite)
+            awt += tail ? d * xh : 0.f;
+            abt += d;
+        }
         team_sum2<TEAM>(s1, s2, sh, half);
         s1 *= inv;
         s2 *= inv;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * TEAM + lane) * V;
-            if (c < width) {
+            if (c < main) {
                 Raw<T, V> o;
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
@@ -148,6 +181,9 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_bwd(const T* __res
                 }
                 o.store(dx + row * width + c);
             }
+        }
+        if (tail) {
+            dx[row * width + main + lane] = from_f32<T>(rs * (to_f32(gt) * wt - s1 - (to_f32(xt) - mu) * rs * s2));
         }
     }
     // the workgroup's share of dw and db: part[blockIdx][2][width]; the four one-wave teams are joined through LDS
@@ -158,11 +194,12 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_bwd(const T* __res
 #pragma unroll
             for (int k = 0; k < V; ++k) {
                 const int c = (i * TEAM + lane) * V + k;
-                if (c < width) { out[c] = aw[i][k]; out[width + c] = ab[i][k]; }
+                if (c < main) { out[c] = aw[i][k]; out[width + c] = ab[i][k]; }
             }
+        if (tail) { out[main + lane] = awt; out[width + main + lane] = abt; }
     } else {
         constexpr int E = NV * V;
-        __shared__ float acc[2 * E * 64];
+        __shared__ float acc[2 * E * 64], acct[2][8];
         for (int t = 0; t < TEAMS; ++t) {
             if (team == t) {
 #pragma unroll
@@ -173,66 +210,84 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_bwd(const T* __res
                         a[0] = (t ? a[0] : 0.f) + aw[i][k];
                         a[E * 64] = (t ? a[E * 64] : 0.f) + ab[i][k];
                     }
+                if (tail) {
+                    acct[0][lane] = (t ? acct[0][lane] : 0.f) + awt;
+                    acct[1][lane] = (t ? acct[1][lane] : 0.f) + abt;
+                }
             }
             __syncthreads();
         }
         for (int j = threadIdx.x; j < 2 * E * 64; j += 256) {
-            const int half = j / (E * 64), e = (j / 64) % E, l = j & 63, c = ((e / V) * 64 + l) * V + e % V;
-            if (c < width) out[half * width + c] = acc[j];
+            const int half_at = j / (E * 64), e = (j / 64) % E, l = j & 63, c = ((e / V) * 64 + l) * V + e % V;
+            if (c < main) out[half_at * width + c] = acc[j];
         }
+        if (TAIL && team < 2 && tail) out[team * width + main + lane] = acct[team][lane];
     }
 }
 
-// Lanes per row and elements per lane.
+// Lanes per row and elements per lane.  A wave holds up to 2048 columns, 32 a lane, where its registers allow two waves a
+// SIMD: the forward, and the backward of 16-bit rows without a tail (65536 x 2048 bf16: 160 us, with 256 lanes a row
+// 194; forward 102 and 122).  Else (`wide`) those rows take 256 lanes (backward, 16000 x 1999 bf16: 47 us and 52 with one wave;
+// 16000 x 1600 f32: 55 and 65).
 struct Shape { int team, e; };
-Shape shape_of(int width) {
+Shape shape_of(int width, bool wide) {
     if (width <= 512) return {64, 8};
     if (width <= 1024) return {64, 16};
-    if (width <= 2048) return {64, 32};
+    if (width <= 2048) return wide ? Shape{256, 8} : Shape{64, 32};
     if (width <= 4096) return {256, 16};
     return {512, 16};
 }
 constexpr int MAX_WIDTH = 8192;
 
-int bwd_groups(long rows, int width) {
-    const Shape s = shape_of(width);
-    const long per = s.team == 64 ? 4 : 1;
-    long g = (rows + per * 4 - 1) / (per * 4);             // four rows a team, so that the partial rows stay few
+int bwd_groups(long rows, int team) {
+    const long per = team == 64 ? 4 : 1;
+    const long g = (rows + per * 4 - 1) / (per * 4);       // four rows a team, so that the partial rows stay few
     return (int)(g < 1 ? 1 : g > 512 ? 512 : g);
 }
 
-template <typename T, int V, typename F> int by_shape(int width, F f) {
-    const Shape s = shape_of(width);
-    if (s.team == 64 && s.e == 8) return f.template operator()<T, V, 64, 8 / V>();
-    if (s.team == 64 && s.e == 16) return f.template operator()<T, V, 64, 16 / V>();
-    if (s.team == 64) return f.template operator()<T, V, 64, 32 / V>();
-    if (s.team == 256) return f.template operator()<T, V, 256, 16 / V>();
-    return f.template operator()<T, V, 512, 16 / V>();
+template <typename T, int V, bool TAIL, typename F> int by_shape(int width, F f) {
+    const Shape s = shape_of(width - width % V, F::wide(sizeof(T), TAIL));
+    if (s.team == 64 && s.e == 8) return f.template operator()<T, V, 64, 8 / V, TAIL>();
+    if (s.team == 64 && s.e == 16) return f.template operator()<T, V, 64, 16 / V, TAIL>();
+    if (s.team == 64) return f.template operator()<T, V, 64, 32 / V, TAIL>();
+    if (s.team == 256 && s.e == 8) return f.template operator()<T, V, 256, 8 / V, TAIL>();
+    if (s.team == 256) return f.template operator()<T, V, 256, 16 / V, TAIL>();
+    return f.template operator()<T, V, 512, 16 / V, TAIL>();
 }
-template <typename F> int by_type(int dtype, bool vec, int width, F f) {
-    if (dtype == VQA_F32) return vec ? by_shape<float, 4>(width, f) : by_shape<float, 1>(width, f);
-    if (dtype == VQA_BF16) return vec ? by_shape<bf16, 8>(width, f) : by_shape<bf16, 1>(width, f);
-    return vec ? by_shape<_Float16, 8>(width, f) : by_shape<_Float16, 1>(width, f);
+template <typename T, typename F> int by_tail(int width, F f) {
+    constexpr int V = 16 / sizeof(T);
+    return width % V ? by_shape<T, V, true>(width, f) : by_shape<T, V, false>(width, f);
+}
+template <typename F> int by_type(int dtype, int width, F f) {
+    if (dtype == VQA_F32) return by_tail<float>(width, f);
+    if (dtype == VQA_BF16) return by_tail<bf16>(width, f);
+    return by_tail<_Float16>(width, f);
 }
 
 struct Fwd {
+    static bool wide(int bytes, bool) { return bytes == 4; }
     hipStream_t st; const void* x; long ldx; const float *w, *b; long rows; int width; float eps; void* y; float *mean, *rstd;
-    template <typename T, int V, int TEAM, int NV> int operator()() const {
+    template <typename T, int V, int TEAM, int NV, bool TAIL> int operator()() const {
         const long grid = TEAM == 64 ? (rows + 3) / 4 : rows;
-        ln_fwd<T, V, TEAM, NV><<<(unsigned)grid, TEAM == 64 ? 256 : TEAM, 0, st>>>(
+        ln_fwd<T, V, TEAM, NV, TAIL><<<(unsigned)grid, TEAM == 64 ? 256 : TEAM, 0, st>>>(
             static_cast<const T*>(x), ldx, w, b, rows, width, eps, static_cast<T*>(y), mean, rstd);
         CHECK_LAUNCH();
         return VQA_OK;
     }
 };
 struct Bwd {
+    static bool wide(int bytes, bool tail) { return bytes == 4 || tail; }
     hipStream_t st; const void* dy; long lddy; const void* x; long ldx; const float *w, *mean, *rstd; long rows; int width;
-    void* dx; float* part;
-    template <typename T, int V, int TEAM, int NV> int operator()() const {
-        ln_bwd<T, V, TEAM, NV><<<bwd_groups(rows, width), TEAM == 64 ? 256 : TEAM, 0, st>>>(
+    void* dx; float *dw, *db, *part;
+    template <typename T, int V, int TEAM, int NV, bool TAIL> int operator()() const {
+        ln_bwd<T, V, TEAM, NV, TAIL><<<bwd_groups(rows, TEAM), TEAM == 64 ? 256 : TEAM, 0, st>>>(
             static_cast<const T*>(dy), lddy, static_cast<const T*>(x), ldx, w, mean, rstd, rows, width,
             static_cast<T*>(dx), part);
         CHECK_LAUNCH();
+        if (dw || db) {
+            seq_sum_columns(st, part, bwd_groups(rows, TEAM), 2L * width, dw, width, db);
+            CHECK_LAUNCH();
+        }
         return VQA_OK;
     }
 };
@@ -240,37 +295,25 @@ struct Bwd {
 bool bad_shape(int dtype, long rows, int width) {
     return !vqa_dtype_ok(dtype) || rows < 1 || rows > 0x7fffffffL || width < 1 || width > MAX_WIDTH;
 }
-bool param_vec(const float* p) { return ((uintptr_t)p & 15) == 0; }      // (NULL is aligned)
 
 }  // namespace
 
 extern "C" int vqa_layer_norm_fwd(void* stream, int dtype, const void* x, long ldx, const float* weight,
                                   const float* bias, long rows, int width, float eps, void* y, float* stats) {
     if (bad_shape(dtype, rows, width) || !x || !y) return VQA_ERR_ARG;
-    const int e = vqa_elem_bytes(dtype);
-    const bool vec = width % (16 / e) == 0 && vqa_vec_ok(x, ldx, e) && vqa_vec_ok(y, width, e) && param_vec(weight) &&
-                     param_vec(bias);
-    return by_type(dtype, vec, width,
+    return by_type(dtype, width,
                    Fwd{static_cast<hipStream_t>(stream), x, ldx, weight, bias, rows, width, eps, y, stats,
                        stats ? stats + rows : nullptr});
 }
 
 extern "C" int vqa_layer_norm_bwd_part(long rows, int width) {
-    return rows < 1 || width < 1 || width > MAX_WIDTH ? 0 : bwd_groups(rows, width);
+    return rows < 1 || width < 1 || width > MAX_WIDTH ? 0 : bwd_groups(rows, 256);      // (the larger of the two)
 }
 
 extern "C" int vqa_layer_norm_bwd(void* stream, int dtype, const void* dy, long lddy, const void* x, long ldx,
                                   const float* weight, const float* stats, long rows, int width, void* dx,
                                   float* dweight, float* dbias, float* part) {
     if (bad_shape(dtype, rows, width) || !dy || !x || !stats || !dx || !part) return VQA_ERR_ARG;
-    const int e = vqa_elem_bytes(dtype);
-    const bool vec = width % (16 / e) == 0 && vqa_vec_ok(x, ldx, e) && vqa_vec_ok(dy, lddy, e) && vqa_vec_ok(dx, width, e);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const int rc = by_type(dtype, vec, width, Bwd{st, dy, lddy, x, ldx, weight, stats, stats + rows, rows, width, dx, part});
-    if (rc != VQA_OK) return rc;
-    if (dweight || dbias) {
-        seq_sum_columns(st, part, bwd_groups(rows, width), 2L * width, dweight, width, dbias);
-        CHECK_LAUNCH();
-    }
-    return VQA_OK;
+    return by_type(dtype, width, Bwd{st, dy, lddy, x, ldx, weight, stats, stats + rows, rows, width, dx, dweight, dbias, part});
 }

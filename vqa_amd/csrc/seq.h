@@ -1,15 +1,16 @@
 // Device helpers of the sequence operators (layer_norm.hip, causal_conv.hip, scan.hip): rows of float, bf16 or f16
-// elements are moved V at a time (16 bytes where base, strides and width allow it, else one element), the arithmetic is
-// f32, and each result is rounded once, to nearest even, when it is stored.
+// elements are moved V at a time, up to 16 bytes, the arithmetic is f32, and each result is rounded once, to nearest even,
+// when it is stored.
 #pragma once
 #include "common.h"
 
 template <> __device__ __forceinline__ _Float16 from_f32<_Float16>(float x) { return (_Float16)x; }
 
-template <typename T, int V> struct RowVec { typedef T type __attribute__((ext_vector_type(V))); };
+template <typename T, int V> struct RowVec { typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T)))); };
 template <typename T> struct RowVec<T, 1> { typedef T type; };
 
-// V consecutive elements as they lie in memory (p is aligned to V * sizeof(T))
+// V consecutive elements as they lie in memory, at any element's address (one access: the hardware takes vector loads and
+// stores of global memory at any alignment, so an odd width does not cost the wide accesses)
 template <typename T, int V> struct Raw {
     typename RowVec<T, V>::type v;
     __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const typename RowVec<T, V>::type*>(p); }
