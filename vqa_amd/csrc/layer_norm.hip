@@ -120,31 +120,32 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_bwd(const T* __res
     const long step = (long)gridDim.x * TEAMS;
     long row = (long)blockIdx.x * TEAMS + team;
     Raw<T, V> xr[NV], gr[NV], xn[NV], gn[NV];
-    T xt, gt, xnt = from_f32<T>(0.f), gnt = from_f32<T>(0.f);
+    Raw<T, 1> xt, gt, xnt, gnt;
     float mu = 0.f, rs = 0.f, mun = 0.f, rsn = 0.f;
-    auto fetch = [&](long at) {                            // the next row is in flight while this one is worked on
+    // The next row is in flight while this one is worked on.  The loads are straight-line code - a lane past the end loads
+    // the last columns again, which meet weights of 0, and past the last row that row - because behind a branch that may
+    // skip them the compiler waits for the new loads where it needs the old ones.
+    auto fetch = [&](long at) {
+        at = min(at, rows - 1);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * TEAM + lane) * V;
-            xn[i].zero();
-            gn[i].zero();
-            if (at < rows && c < main) { xn[i].load(x + at * ldx + c); gn[i].load(dy + at * lddy + c); }
+            const int c = min((i * TEAM + lane) * V, main - V);
+            xn[i].load(x + at * ldx + c);
+            gn[i].load(dy + at * lddy + c);
         }
         if constexpr (TAIL) {
-            xnt = gnt = from_f32<T>(0.f);
-            if (at < rows && tail) { xnt = x[at * ldx + main + lane]; gnt = dy[at * lddy + main + lane]; }
+            const int c = min(main + lane, width - 1);
+            xnt.load(x + at * ldx + c);
+            gnt.load(dy + at * lddy + c);
         }
-        // (conditional values, not conditional stores: those were sunk into stores through a chosen address, and the
-        // variables went to scratch memory)
-        mun = at < rows ? mean[at] : 0.f;
-        rsn = at < rows ? rstd[at] : 0.f;
+        mun = mean[at];
+        rsn = rstd[at];
     };
     fetch(row);
     for (; row < rows; row += step) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) { xr[i] = xn[i]; gr[i] = gn[i]; }
-        xt = xnt;
-        gt = gnt;
+        if (TAIL) { xt = xnt; gt = gnt; }
         mu = mun;
         rs = rsn;
         fetch(row + step);
@@ -160,10 +161,10 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_bwd(const T* __res
                 ab[i][k] += d;
             }
         if (TAIL) {
-            const float xh = (to_f32(xt) - mu) * rs, d = to_f32(gt), g = d * wt;
+            const float xh = (xt.get(0) - mu) * rs, d = gt.get(0), g = d * wt;
             s1 += g;
-            s2 += tail ? g * xh : 0.f;                     // (mu or rs may not be finite)
-            awt += tail ? d * xh : 0.f;
+            s2 += g * xh;
+            awt += d * xh;
             abt += d;
         }
         team_sum2<TEAM>(s1, s2, sh, half);
@@ -183,7 +184,8 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_bwd(const T* __res
             }
         }
         if (tail) {
-            dx[row * width + main + lane] = from_f32<T>(rs * (to_f32(gt) * wt - s1 - (to_f32(xt) - mu) * rs * s2));
+            xt.set(0, rs * (gt.get(0) * wt - s1 - (xt.get(0) - mu) * rs * s2));
+            xt.store(dx + row * width + main + lane);
         }
     }
     // the workgroup's share of dw and db: part[blockIdx][2][width]; the four one-wave teams are joined through LDS
@@ -256,6 +258,7 @@ template <typename T, int V, bool TAIL, typename F> int by_shape(int width, F f)
 }
 template <typename T, typename F> int by_tail(int width, F f) {
     constexpr int V = 16 / sizeof(T);
+    if (width < V) return f.template operator()<T, 1, 64, 8, false>();
     return width % V ? by_shape<T, V, true>(width, f) : by_shape<T, V, false>(width, f);
 }
 template <typename F> int by_type(int dtype, int width, F f) {
