@@ -60,7 +60,7 @@ def test_scan_workspaces_hold_what_the_kernels_write():
         sizes = (ctypes.c_long * 3)()
         assert lib.vqa_scan_ws_bytes(1, B, T, D, N, G, ctypes.addressof(sizes)) == 0
         fwd, keep, bwd = sizes
-        padded, states = G * -(-(D // G) // (128 if N <= 16 else 64)) * (128 if N <= 16 else 64), 16 if N <= 16 else 32 if N <= 32 else 64
+        padded, states = G * -(-(D // G) // (128 if N <= 16 else 64)) * (128 if N <= 16 else 64), 8 if N <= 8 else 16 if N <= 16 else 32 if N <= 32 else 64
         assert keep == 4 * B * (-(-T // 8) - 1) * padded * states      # (before every tile but the first)
         assert bwd >= fwd + 4 * B * T * G * 2 * N + 4 * padded * (states + 2)
         assert all(s % 16 == 0 for s in (fwd, keep)) and fwd >= 0

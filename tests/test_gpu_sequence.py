@@ -293,7 +293,8 @@ def test_selective_scan(B, T, D, N, G, dtype, lengths):
 
 @pytest.mark.parametrize('B,T,D,N,G,dtype,lengths', [
     (1, 600, 32, 16, 1, 'f32', None), (2, 333, 72, 16, 1, 'bf16', [200, 333]), (1, 257, 24, 40, 2, 'f32', [256]),
-    (2, 130, 17, 20, 1, 'bf16', [0, 64])])
+    (2, 130, 17, 20, 1, 'bf16', [0, 64]),
+    (1, 200, 70, 8, 1, 'bf16', None), (2, 150, 34, 5, 2, 'f32', [149, 3])])
 def test_selective_scan_in_segments(B, T, D, N, G, dtype, lengths):
     """Few rows and a long axis: the tokens are cut into segments that are joined again."""
     lens = torch.tensor(lengths, dtype=torch.int32) if lengths is not None else None

@@ -17,7 +17,7 @@
 // With few rows the tokens are cut into segments: a first pass finds each segment's own end state and total decay (the
 // product of decays is exp(a sum dt)), a small one chains them, and the full pass starts every segment from its true
 // state.  The backward does the same from the other end.  For the backward the forward keeps h before every tile but the first.
-// States in workspaces lie as [..][channel, a group's padded to per_pad][NP], NP = 16, 32 or 64 >= N.
+// States in workspaces lie as [..][channel, a group's padded to per_pad][NP], NP = 8, 16, 32 or 64 >= N.
 #include "seq.h"
 
 namespace {
@@ -100,6 +100,17 @@ __device__ __forceinline__ float sum16_four(float a, float b, float c, float d) 
     return s;
 }
 __device__ __forceinline__ int sum16_of(int bank) { return (bank & 1) << 1 | bank >> 1; }
+// A lane's NS values, one a state of its row, summed over the row's 16 lanes and put at s[4 rows x NS states]
+template <int NS> __device__ __forceinline__ void put_sums(float* s, const float (&v)[NS], int r, int cl) {
+    if constexpr (NS == 2) {
+        const float a = sum16(v[0]), b = sum16(v[1]);
+        s[r * 2 + (cl & 1)] = cl & 1 ? b : a;
+    } else {
+#pragma unroll
+        for (int j = 0; j < NS; j += 4)
+            s[r * NS + j + sum16_of(cl >> 2)] = sum16_four(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    }
+}
 
 template <int N> __device__ __forceinline__ void lds_read(const float* p, float (&v)[N]) {
     if constexpr (N % 4 == 0) {
@@ -117,7 +128,7 @@ template <int N> __device__ __forceinline__ void lds_read(const float* p, float 
 // Where a wave is: its channels [c0, c0 + 16 CH) of group g up to the group's end (p0: the first one's place in a
 // workspace), and its lane's places in both mappings.
 template <typename T, int CH, int NS, int VE> struct Wave {
-    static constexpr int WC = 16 * CH, NP = 4 * NS, NV = TT * WC / 64 / VE;
+    static constexpr int WC = 16 * CH, NP = 4 * NS, NV = TT * WC / 64 / VE, SV = NS < 4 ? NS : 4;
     int lane, cl, r, g, c0, cend, p0;
     __device__ __forceinline__ Wave(const Args& A, int group, int first) {
         lane = threadIdx.x & 63;
@@ -205,10 +216,10 @@ template <typename T, int CH, int NS, int VE> struct Wave {
 #pragma unroll
         for (int i = 0; i < CH; ++i)
 #pragma unroll
-            for (int j = 0; j < NS; j += 4) {
-                const Raw<float, 4> f = buf_load<float, 4>(rs, own_place(i, j));
+            for (int j = 0; j < NS; j += SV) {
+                const Raw<float, SV> f = buf_load<float, SV>(rs, own_place(i, j));
 #pragma unroll
-                for (int q = 0; q < 4; ++q) h[i][j + q] = f.get(q);
+                for (int q = 0; q < SV; ++q) h[i][j + q] = f.get(q);
             }
     }
     __device__ __forceinline__ void store_own(float* p, const float (&h)[CH][NS]) const {
@@ -216,11 +227,11 @@ template <typename T, int CH, int NS, int VE> struct Wave {
 #pragma unroll
         for (int i = 0; i < CH; ++i)
 #pragma unroll
-            for (int j = 0; j < NS; j += 4) {
-                Raw<float, 4> f;
+            for (int j = 0; j < NS; j += SV) {
+                Raw<float, SV> f;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) f.set(q, h[i][j + q]);
-                buf_store<float, 4>(rs, own_place(i, j), f);
+                for (int q = 0; q < SV; ++q) f.set(q, h[i][j + q]);
+                buf_store<float, SV>(rs, own_place(i, j), f);
             }
     }
 };
@@ -522,8 +533,8 @@ __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
 template <typename T, int CH, int NS, int VE>
 __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A) {
     typedef Wave<T, CH, NS, VE> W;
-    constexpr int TILE = TT * W::WC, SH = TT * W::NP, NBC = 2 * SH / (64 * BW), 
-                  KD = CH * NS > 8 ? 0 : CH == 1 || (VE > 1 && sizeof(T) == 2) ? 5 : VE > 1 ? 2 : 0;
+    constexpr int TILE = TT * W::WC, SH = TT * W::NP, NBC = (2 * SH + 64 * BW - 1) / (64 * BW), 
+                  KD = CH * NS > 8 ? 0 : CH * NS < 8 || CH == 1 || (VE > 1 && sizeof(T) == 2) ? 5 : VE > 1 ? 2 : 0;
     __shared__ __attribute__((aligned(16))) float lds[BW][6 * TILE + 2 * W::WC], s_bc[2 * SH], s_part[BW][2 * SH];
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int blks = A.bblk * A.G;
@@ -535,7 +546,6 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
     const float *s_b = s_bc, *s_c = s_bc + SH;
     const long chans = (long)A.G * A.per_pad;
     const int ts = seg * A.seg_len, tend = min(A.L, ts + A.seg_len);
-    const int state_at = w.r * NS + sum16_of(w.cl >> 2);   // where this lane's value of sum16_four belongs
     float a2[CH][NS], g[CH][NS], da[CH][NS], sum_skip[W::NV][VE], sum_bias[W::NV][VE];
     w.lane_a(A, a2);
     w.stage_param(A.dt_bias, s_bias);
@@ -568,7 +578,7 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
 #pragma unroll
         for (int k = 0; k < NBC; ++k) {
             const int id = k * 64 * BW + threadIdx.x;
-            sn[k] = fetch_shared<T, W::NP>(id < SH ? A.b : A.c, b, t0, te, w.g, A.N, id % SH);
+            sn[k] = fetch_shared<T, W::NP>(id < SH ? A.b : A.c, b, t0, id < 2 * SH ? te : t0, w.g, A.N, id % SH);
         }
         if (t0 > 0) w.load_own(A.keep + (((long)b * kept_tiles(A.L) + t0 / TT - 1) * chans + w.p0) * W::NP, hn);
         else w.load_public(A.state, b, A.D, A.N, hn);
@@ -600,7 +610,8 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
 #pragma unroll
                 for (int j = 0; j < NS; ++j) h[i][j] = hn[i][j];
 #pragma unroll
-            for (int k = 0; k < NBC; ++k) s_bc[k * 64 * BW + threadIdx.x] = shared_value<T>(sn[k]);
+            for (int k = 0; k < NBC; ++k)
+                if (k * 64 * BW + (int)threadIdx.x < 2 * SH) s_bc[k * 64 * BW + threadIdx.x] = shared_value<T>(sn[k]);
             float step[W::NV][VE], slope[W::NV][VE], sig[W::NV][VE], dcore[W::NV][VE];
             if (live) {
                 stage_steps<true>(w, d, s_bias, A.softplus, t0, te, step, slope);
@@ -653,9 +664,7 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
                         }
                     }
                     s_y[t * W::WC + w.cl * CH + own_channel<CH>(w.r)] = sum_states<CH>(y);
-#pragma unroll
-                    for (int j = 0; j < NS; j += 4)
-                        s_dc[t * W::NP + state_at + j] = sum16_four(sc[j], sc[j + 1], sc[j + 2], sc[j + 3]);
+                    put_sums<NS>(s_dc + t * W::NP, sc, w.r, w.cl);
                 }
                 lds_order();                               // (and the decays are formed again, not held in registers)
 #pragma unroll
@@ -688,9 +697,7 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
                     if constexpr (CH == 2) both = swap_add16(swap_add32(gb[0], gb[1]), swap_add32(ta[0], ta[1]));
                     else both = swap_add16(swap_add32(gb[0], gb[0]), swap_add32(ta[0], ta[0]));
                     s_gt[(w.r & 1) * TILE + t * W::WC + w.cl * CH + (CH == 2 ? w.r >> 1 : 0)] = both;
-#pragma unroll
-                    for (int j = 0; j < NS; j += 4)
-                        s_db[t * W::NP + state_at + j] = sum16_four(sb[j], sb[j + 1], sb[j + 2], sb[j + 3]);
+                    put_sums<NS>(s_db + t * W::NP, sb, w.r, w.cl);
                 }
                 lds_order();
                 if (A.gate.p) {
@@ -729,6 +736,7 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
 #pragma unroll
             for (int k = 0; k < NBC; ++k) {
                 const int id = k * 64 * BW + threadIdx.x, t = id % SH / W::NP, n = id % W::NP;
+                if (id >= 2 * SH) break;
                 float s = 0.f;
 #pragma unroll
                 for (int u = 0; u < BW; ++u) s += s_part[u][id];
@@ -871,7 +879,7 @@ __global__ __launch_bounds__(256) void scan_token(Rows x, float* __restrict__ st
 }
 
 // Padded states, and channels of a forward wave and of a backward workgroup.
-int np_of(int N) { return N <= 16 ? 16 : N <= 32 ? 32 : 64; }
+int np_of(int N) { return N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 int fwd_channels(int N) { return N <= 16 ? 64 : N <= 32 ? 32 : 16; }
 int bwd_channels(int N) { return N <= 16 ? 32 * BW : 16 * BW; }
 
@@ -944,6 +952,7 @@ template <typename T, int NS, int CH, int VE, int BCH, int BVE> int launch(bool 
 }
 template <typename T> int by_states(bool bwd, bool vec, const Args& A, hipStream_t st) {
     constexpr int V = 16 / sizeof(T);
+    if (A.N <= 8) return vec ? launch<T, 2, 4, V, 2, 4>(bwd, A, st) : launch<T, 2, 4, 1, 2, 1>(bwd, A, st);
     if (A.N <= 16) return vec ? launch<T, 4, 4, V, 2, 4>(bwd, A, st) : launch<T, 4, 4, 1, 2, 1>(bwd, A, st);
     if (A.N <= 32) return vec ? launch<T, 8, 2, 4, 1, 2>(bwd, A, st) : launch<T, 8, 2, 1, 1, 1>(bwd, A, st);
     return vec ? launch<T, 16, 1, 2, 1, 2>(bwd, A, st) : launch<T, 16, 1, 1, 1, 1>(bwd, A, st);
@@ -1019,7 +1028,8 @@ extern "C" int vqa_scan_bwd(void* stream, int dtype, const void* dy, long dy_bat
     if (rc != VQA_OK) return rc;
     const int rows = A.bgroups * A.segs, np = np_of(N);
     const unsigned pg = (unsigned)(((long)G * A.per_pad * (np + 2) + 63) / 64);
-    if (np == 16) scan_params<16><<<pg, 1024, 0, st>>>(A.part_p, rows, A.per, A.per_pad, N, G, da, dskip, ddt_bias);
+    if (np == 8) scan_params<8><<<pg, 1024, 0, st>>>(A.part_p, rows, A.per, A.per_pad, N, G, da, dskip, ddt_bias);
+    else if (np == 16) scan_params<16><<<pg, 1024, 0, st>>>(A.part_p, rows, A.per, A.per_pad, N, G, da, dskip, ddt_bias);
     else if (np == 32) scan_params<32><<<pg, 1024, 0, st>>>(A.part_p, rows, A.per, A.per_pad, N, G, da, dskip, ddt_bias);
     else scan_params<64><<<pg, 1024, 0, st>>>(A.part_p, rows, A.per, A.per_pad, N, G, da, dskip, ddt_bias);
     CHECK_LAUNCH();
