@@ -30,21 +30,10 @@ _ROW_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 _F32 = torch.float32
 
 
-class _device_of:
-    """Makes x's device the current one for the call where it is not (the kernels go to the current device's stream)."""
-
-    def __init__(self, x):
-        self.want, self.had = x.get_device(), None
-
-    def __enter__(self):
-        had = torch._C._cuda_getDevice()
-        if had != self.want:
-            self.had = had
-            torch._C._cuda_setDevice(self.want)
-
-    def __exit__(self, *exc):
-        if self.had is not None:
-            torch._C._cuda_setDevice(self.had)
+def _elsewhere(x):
+    """Whether x's device is not the current one (the kernels go to the current device's stream; autograd makes a
+    backward's device the current one by itself)."""
+    return torch._C._cuda_getDevice() != x.get_device()
 
 
 def _fail(what):
@@ -128,7 +117,9 @@ def _backward(f):
 
 def _as_matrix(x):
     """[..., C] -> [rows, C] with a contiguous last axis and one row stride; a view where the strides allow it"""
-    return _unit(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    return x if x.stride(1) == 1 else x.contiguous()
 
 
 def _norm_fwd(x, weight, bias, eps, stats):
@@ -144,8 +135,7 @@ def _norm_fwd(x, weight, bias, eps, stats):
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        with _device_of(x):
-            y, st = _norm_fwd(x, weight, bias, eps, True)
+        y, st = _norm_fwd(x, weight, bias, eps, True)
         ctx.save_for_backward(x, weight, st)
         ctx.has_bias = bias is not None
         return y
@@ -156,18 +146,17 @@ class _LayerNorm(torch.autograd.Function):
         x2, dy2 = _as_matrix(x), _as_matrix(dy)
         rows, width = x2.shape
         dev = x.device
-        with _device_of(x):
-            dx = torch.empty(x.shape, device=dev, dtype=x.dtype)
-            dw = torch.empty(width, device=dev, dtype=_F32) if weight is not None else None
-            db = torch.empty(width, device=dev, dtype=_F32) if ctx.has_bias else None
-            if rows:
-                part = torch.empty(_norm_parts(rows, width), 2, width, device=dev, dtype=_F32)
-                L.call('vqa_layer_norm_bwd', L.dt(x), dy2, dy2.stride(0), x2, x2.stride(0), weight, st, rows, width,
-                       dx, dw, db, part)
-            else:
-                for g in (dw, db):
-                    if g is not None:
-                        g.zero_()
+        dx = torch.empty(x.shape, device=dev, dtype=x.dtype)
+        dw = torch.empty(width, device=dev, dtype=_F32) if weight is not None else None
+        db = torch.empty(width, device=dev, dtype=_F32) if ctx.has_bias else None
+        if rows:
+            part = torch.empty(_norm_parts(rows, width), 2, width, device=dev, dtype=_F32)
+            L.call('vqa_layer_norm_bwd', L.dt(x), dy2, dy2.stride(0), x2, x2.stride(0), weight, st, rows, width,
+                   dx, dw, db, part)
+        else:
+            for g in (dw, db):
+                if g is not None:
+                    g.zero_()
         return dx, dw, db, None
 
 
@@ -180,13 +169,15 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis (biased variance), statistics in float32.
     x [..., C] with C <= 8192; weight, bias float32 [C] or None."""
     _first(x, None, '')
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return layer_norm(x, weight, bias, eps)
     if x.dim() < 1 or not 1 <= x.shape[-1] <= 8192:
         _fail(f'x has shape {tuple(x.shape)}: a last axis of 1 to 8192 is wanted')
     weight, bias = _param('weight', weight, x.shape[-1:], x), _param('bias', bias, x.shape[-1:], x)
     if _tracked(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, eps)
-    with _device_of(x):
-        return _norm_fwd(x, weight, bias, eps, False)[0]
+    return _norm_fwd(x, weight, bias, eps, False)[0]
 
 
 # --------------------------------------------------------------------------------------------------- causal convolution
@@ -219,8 +210,7 @@ def _conv_fwd(x, weight, bias, silu, state, lengths, want_last):
 class _CausalConv(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, silu, state, lengths, want_last):
-        with _device_of(x):
-            y, last = _conv_fwd(x, weight, bias, silu, state, lengths, want_last)
+        y, last = _conv_fwd(x, weight, bias, silu, state, lengths, want_last)
         ctx.save_for_backward(x, weight, bias, state, lengths)
         ctx.silu = silu
         ctx.set_materialize_grads(False)
@@ -231,23 +221,22 @@ class _CausalConv(torch.autograd.Function):
         x, weight, bias, state, lengths = ctx.saved_tensors
         B, T, D = x.shape
         taps, dev = weight.shape[1], x.device
-        with _device_of(x):
-            dy = torch.zeros(B, T, D, device=dev, dtype=x.dtype) if dy is None else _unit(dy)
-            dlast = None if dlast is None else dlast.contiguous()
-            dx = torch.empty(B, T, D, device=dev, dtype=x.dtype)
-            dw = torch.empty(D, taps, device=dev, dtype=_F32)
-            db = torch.empty(D, device=dev, dtype=_F32) if bias is not None else None
-            dstate = torch.empty(B, taps - 1, D, device=dev, dtype=x.dtype) if state is not None else None
-            if dx.numel():
-                part = torch.empty(_conv_parts(B, T, D), taps + 1, D, device=dev, dtype=_F32)
-                L.call('vqa_causal_conv_bwd', L.dt(x), dy, dy.stride(0), dy.stride(1), dlast, x, x.stride(0),
-                       x.stride(1), weight, bias, state, lengths, B, T, D, taps, ctx.silu, dx, dw, db, dstate, part)
-            else:
-                dw.zero_()
-                if db is not None:
-                    db.zero_()
-                if dstate is not None:
-                    dstate.zero_() if dlast is None else dstate.copy_(dlast)
+        dy = torch.zeros(B, T, D, device=dev, dtype=x.dtype) if dy is None else _unit(dy)
+        dlast = None if dlast is None else dlast.contiguous()
+        dx = torch.empty(B, T, D, device=dev, dtype=x.dtype)
+        dw = torch.empty(D, taps, device=dev, dtype=_F32)
+        db = torch.empty(D, device=dev, dtype=_F32) if bias is not None else None
+        dstate = torch.empty(B, taps - 1, D, device=dev, dtype=x.dtype) if state is not None else None
+        if dx.numel():
+            part = torch.empty(_conv_parts(B, T, D), taps + 1, D, device=dev, dtype=_F32)
+            L.call('vqa_causal_conv_bwd', L.dt(x), dy, dy.stride(0), dy.stride(1), dlast, x, x.stride(0),
+                   x.stride(1), weight, bias, state, lengths, B, T, D, taps, ctx.silu, dx, dw, db, dstate, part)
+        else:
+            dw.zero_()
+            if db is not None:
+                db.zero_()
+            if dstate is not None:
+                dstate.zero_() if dlast is None else dstate.copy_(dlast)
         return dx, dw, db, None, dstate, None, None
 
 
@@ -262,6 +251,9 @@ def causal_conv(x, weight, bias=None, activation='silu', state=None, lengths=Non
     [D, taps], bias float32 [D].  state [B, taps - 1, D] (x's type): the rows before the first (None: zeros).  Returns y,
     or with return_state (y, state after each sequence's last token)."""
     _first(x, 3, '[B, L, D]')
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return causal_conv(x, weight, bias, activation, state, lengths, return_state)
     B, T, D = x.shape
     taps = _taps(weight, D)
     weight, bias = _param('weight', weight, (D, taps), x), _param('bias', bias, (D,), x)
@@ -274,8 +266,7 @@ def causal_conv(x, weight, bias=None, activation='silu', state=None, lengths=Non
     if _tracked(x, weight, bias, state):
         y, last = _CausalConv.apply(x, weight, bias, silu, state, lengths, return_state)
     else:
-        with _device_of(x):
-            y, last = _conv_fwd(x, weight, bias, silu, state, lengths, return_state)
+        y, last = _conv_fwd(x, weight, bias, silu, state, lengths, return_state)
     return (y, last) if return_state else y
 
 
@@ -283,6 +274,9 @@ def causal_conv_step(x, state, weight, bias=None, activation='silu'):
     """causal_conv for ONE new token per sequence: x [B, D]; state [B, taps - 1, D] (x's type; rows may be strided) is
     shifted in place.  Returns y [B, D].  Forward only."""
     _first(x, 2, '[B, D]')
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return causal_conv_step(x, state, weight, bias, activation)
     B, D = x.shape
     taps = _taps(weight, D)
     weight, bias = _param('weight', weight, (D, taps), x), _param('bias', bias, (D,), x)
@@ -297,13 +291,12 @@ def causal_conv_step(x, state, weight, bias=None, activation='silu'):
             B == 1 or s0 >= (taps - 2) * s1 + D or (s0 >= D and s1 >= (B - 1) * s0 + D)):
         _fail(f'state has strides {state.stride()}: it is updated in place, so rows must be contiguous and apart')
     x = _unit(x)
-    if L._PROFILE is None and L._REC is None and torch._C._cuda_getDevice() == x.get_device():
+    if L._PROFILE is None and L._REC is None:
         L.check(L.lib().vqa_causal_conv_token(
             L._raw_stream(), L.dt(x), x.data_ptr(), x.stride(0), state.data_ptr(), s0, s1, weight.data_ptr(),
             None if bias is None else bias.data_ptr(), B, D, taps, silu, y.data_ptr()), 'vqa_causal_conv_token')
     else:
-        with _device_of(x):
-            L.call('vqa_causal_conv_token', L.dt(x), x, x.stride(0), state, s0, s1, weight, bias, B, D, taps, silu, y)
+        L.call('vqa_causal_conv_token', L.dt(x), x, x.stride(0), state, s0, s1, weight, bias, B, D, taps, silu, y)
     _touched(state)
     return y
 
@@ -348,8 +341,7 @@ def _scan_fwd(x, dt, a, b, c, skip, gate, dt_bias, softplus, state, lengths, wan
 class _SelectiveScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, dt, a, b, c, skip, gate, dt_bias, softplus, state, lengths, want_last):
-        with _device_of(x):
-            y, last, keep = _scan_fwd(x, dt, a, b, c, skip, gate, dt_bias, softplus, state, lengths, want_last, True)
+        y, last, keep = _scan_fwd(x, dt, a, b, c, skip, gate, dt_bias, softplus, state, lengths, want_last, True)
         ctx.save_for_backward(x, dt, a, b, c, skip, gate, dt_bias, state, lengths, keep)
         ctx.softplus = softplus
         ctx.set_materialize_grads(False)
@@ -362,25 +354,24 @@ class _SelectiveScan(torch.autograd.Function):
         G, N, dev, code = b.shape[2], b.shape[3], x.device, L.dt(x)
         f32 = lambda *s: torch.empty(*s, device=dev, dtype=_F32)       # noqa: E731
         rows = lambda *s: torch.empty(*s, device=dev, dtype=x.dtype)            # noqa: E731
-        with _device_of(x):
-            dlast = None if dlast is None else dlast.contiguous()
-            dx, ddt, dgate = rows(B, T, D), rows(B, T, D), rows(B, T, D) if gate is not None else None
-            db, dc, da = rows(B, T, G, N), rows(B, T, G, N), f32(D, N)
-            dskip, dbias = f32(D) if skip is not None else None, f32(D) if dt_bias is not None else None
-            dstate = f32(B, D, N) if state is not None else None
-            if not dx.numel():
-                for g in (da, dskip, dbias):
-                    if g is not None:
-                        g.zero_()
-                if dstate is not None:
-                    dstate.zero_() if dlast is None else dstate.copy_(dlast)
-            else:
-                dy = torch.zeros(B, T, D, device=dev, dtype=x.dtype) if dy is None else _near(dy)
-                ws = _floats(_scan_bytes(code, B, T, D, N, G)[2], dev)
-                L.call('vqa_scan_bwd', code, dy, dy.stride(0), dy.stride(1), dlast, x, x.stride(0), x.stride(1), dt,
-                       dt.stride(0), dt.stride(1), gate, *_strides(gate), a, b, b.stride(0), b.stride(1), c,
-                       c.stride(0), c.stride(1), skip, dt_bias, ctx.softplus, state, lengths, B, T, D, N, G, keep, dx, ddt,
-                       dgate, da, db, dc, dskip, dbias, dstate, ws)
+        dlast = None if dlast is None else dlast.contiguous()
+        dx, ddt, dgate = rows(B, T, D), rows(B, T, D), rows(B, T, D) if gate is not None else None
+        db, dc, da = rows(B, T, G, N), rows(B, T, G, N), f32(D, N)
+        dskip, dbias = f32(D) if skip is not None else None, f32(D) if dt_bias is not None else None
+        dstate = f32(B, D, N) if state is not None else None
+        if not dx.numel():
+            for g in (da, dskip, dbias):
+                if g is not None:
+                    g.zero_()
+            if dstate is not None:
+                dstate.zero_() if dlast is None else dstate.copy_(dlast)
+        else:
+            dy = torch.zeros(B, T, D, device=dev, dtype=x.dtype) if dy is None else _near(dy)
+            ws = _floats(_scan_bytes(code, B, T, D, N, G)[2], dev)
+            L.call('vqa_scan_bwd', code, dy, dy.stride(0), dy.stride(1), dlast, x, x.stride(0), x.stride(1), dt,
+                   dt.stride(0), dt.stride(1), gate, *_strides(gate), a, b, b.stride(0), b.stride(1), c,
+                   c.stride(0), c.stride(1), skip, dt_bias, ctx.softplus, state, lengths, B, T, D, N, G, keep, dx, ddt,
+                   dgate, da, db, dc, dskip, dbias, dstate, ws)
         return dx, ddt, da, db, dc, dskip, dgate, dbias, None, dstate, None, None
 
 
@@ -422,14 +413,16 @@ def selective_scan(x, dt, a, b, c, skip=None, gate=None, dt_bias=None, softplus=
     [D, N]; skip, dt_bias float32 [D]; state float32 [B, D, N] (None: zeros).  gate, skip, dt_bias may be None.
     Returns y, or with return_state (y, state after each sequence's last token)."""
     _first(x, 3, '[B, L, D]')
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return selective_scan(x, dt, a, b, c, skip, gate, dt_bias, softplus, state, lengths, return_state)
     args = x, dt, a, b, c, skip, gate, dt_bias = _scan_args(x, dt, a, b, c, skip, gate, dt_bias)
     state = _param('state', state, (x.shape[0], *a.shape), x)
     lengths = _lengths(lengths, x)
     if _tracked(*args, state):
         y, last = _SelectiveScan.apply(*args, int(softplus), state, lengths, return_state)
     else:
-        with _device_of(x):
-            y, last, _ = _scan_fwd(*args, int(softplus), state, lengths, return_state, False)
+        y, last, _ = _scan_fwd(*args, int(softplus), state, lengths, return_state, False)
     return (y, last) if return_state else y
 
 
@@ -437,6 +430,9 @@ def selective_scan_step(x, state, dt, a, b, c, skip=None, gate=None, dt_bias=Non
     """selective_scan for ONE new token per sequence: x, dt, gate [B, D]; b, c [B, N] or [B, G, N]; state float32
     [B, D, N] is updated in place (its batch axis may be strided).  Returns y [B, D].  Forward only."""
     _first(x, 2, '[B, D]')
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return selective_scan_step(x, state, dt, a, b, c, skip, gate, dt_bias, softplus)
     x, dt, a, b, c, skip, gate, dt_bias = _scan_args(x, dt, a, b, c, skip, gate, dt_bias)
     B, D = x.shape
     G, N = b.shape[1:]
@@ -449,7 +445,7 @@ def selective_scan_step(x, state, dt, a, b, c, skip=None, gate=None, dt_bias=Non
     if (state.stride(2) != 1 and N > 1) or (state.stride(1) != N and D > 1) or (B > 1 and state.stride(0) < D * N):
         _fail(f'state has strides {state.stride()}: it is updated in place, so [D, N] must be contiguous and apart')
     sg = 0 if gate is None else gate.stride(0)
-    if L._PROFILE is None and L._REC is None and torch._C._cuda_getDevice() == x.get_device():
+    if L._PROFILE is None and L._REC is None:
         # (one token's latency is host time: pointers are taken here, 3 us less than by L.call)
         L.check(L.lib().vqa_scan_token(
             L._raw_stream(), L.dt(x), x.data_ptr(), x.stride(0), state.data_ptr(), state.stride(0), dt.data_ptr(),
@@ -457,8 +453,7 @@ def selective_scan_step(x, state, dt, a, b, c, skip=None, gate=None, dt_bias=Non
             c.data_ptr(), c.stride(0), None if skip is None else skip.data_ptr(),
             None if dt_bias is None else dt_bias.data_ptr(), softplus, B, D, N, G, y.data_ptr()), 'vqa_scan_token')
     else:
-        with _device_of(x):
-            L.call('vqa_scan_token', L.dt(x), x, x.stride(0), state, state.stride(0), dt, dt.stride(0), gate, sg, a, b,
-                   b.stride(0), c, c.stride(0), skip, dt_bias, softplus, B, D, N, G, y)
+        L.call('vqa_scan_token', L.dt(x), x, x.stride(0), state, state.stride(0), dt, dt.stride(0), gate, sg, a, b,
+               b.stride(0), c, c.stride(0), skip, dt_bias, softplus, B, D, N, G, y)
     _touched(state)
     return y
