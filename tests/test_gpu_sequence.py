@@ -65,8 +65,9 @@ def test_layer_norm(rows, width, dtype):
     # rounded a few times, while their sum may cancel altogether (two values a row: xh = +-1, the sum is 0 but for eps),
     # so dx's rounding is counted at the terms' size.  max|xh| <= sqrt(width); mean(g xh) <= max|g|.
     rstd = float(1 / torch.sqrt(xr.detach().var(-1, unbiased=False) + 1e-5).max())
-    terms = rstd * float((dy.double() * wr).abs().max()) * float(((xr - xr.mean(-1, keepdim=True)).abs().amax(-1) /
-                                                                  xr.std(-1, unbiased=False)).max())
+    xd = xr.detach()
+    terms = rstd * float((dy.double() * wr.detach()).abs().max()) * float(
+        ((xd - xd.mean(-1, keepdim=True)).abs().amax(-1) / xd.std(-1, unbiased=False)).max())
     R.close('dx', got['x'], want['x'], 64, scale=terms)
     R.close('dw', got['w'], want['w'], 64 + rows)
     R.close('db', got['b'], want['b'], 64 + rows)
@@ -509,6 +510,54 @@ def test_same_bits_every_time_and_on_another_stream():
     torch.cuda.current_stream().wait_stream(side)
     for u, v in zip(first, second):
         assert torch.equal(u, v)
+
+
+def test_two_streams_at_once():
+    """Two calls in flight on two streams (states and workspaces of their own), several times over."""
+    sets = []
+    for k in (1, 2):
+        leaves, dy, _ = _scan_case(2, 300, 96, 16, 1, 'bf16', seed=70 + k)
+        ins = {q: v[0].detach() for q, v in leaves.items()}
+        sets.append((ins, S().selective_scan(*(ins[q] for q in SCAN[:8]), state=ins['state'], return_state=True)))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                ins = sets[i][0]
+                outs[i].append(S().selective_scan(*(ins[q] for q in SCAN[:8]), state=ins['state'], return_state=True))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for y, last in outs[i]:
+            assert torch.equal(y, sets[i][1][0]) and torch.equal(last, sets[i][1][1])
+
+
+def test_strides_past_32_bits():
+    """Sequences 2^31 and more elements apart, rows 2^26 apart: the same as contiguous copies of them."""
+    s = S()
+    far = (1 << 31) + 24
+    buf = torch.zeros(far + 8192, device='cuda', dtype=torch.bfloat16)
+    x = buf.as_strided((2, 20, 64), (far, 64, 1), 16)
+    x.copy_(torch.randn(2, 20, 64, generator=_gen(80)))
+    near = x.contiguous()
+    w = torch.randn(64, 4, generator=_gen(81)).cuda()
+    assert torch.equal(s.layer_norm(x[:, 3]), s.layer_norm(near[:, 3]))
+    assert torch.equal(s.causal_conv(x, w), s.causal_conv(near, w))
+    a, b = -torch.rand(64, 8, device='cuda'), torch.randn(2, 20, 8, generator=_gen(82)).cuda().bfloat16()
+    assert torch.equal(s.selective_scan(x, x, a, b, b, gate=x), s.selective_scan(near, near, a, b, b, gate=near))
+    cs = buf.as_strided((2, 3, 64), (far, 64, 1), 4096)
+    cs.copy_(near[:, :3])
+    c2 = cs.contiguous()
+    assert torch.equal(s.causal_conv_step(x[:, 4], cs, w), s.causal_conv_step(near[:, 4], c2, w)) and torch.equal(cs, c2)
+    hbuf = buf.view(torch.float32)
+    h = hbuf.as_strided((2, 64, 8), ((1 << 30) + 8, 8, 1), 64)
+    h2 = h.contiguous()
+    assert torch.equal(s.selective_scan_step(x[:, 4], h, x[:, 5], a, b[:, 0], b[:, 1]),
+                       s.selective_scan_step(near[:, 4], h2, near[:, 5], a, b[:, 0], b[:, 1])) and torch.equal(h, h2)
+    rows = buf.as_strided((1, 9, 64), (64, 1 << 26, 1), 8)
+    assert torch.equal(s.selective_scan(rows, rows, a, b[:1, :9], b[:1, :9]),
+                       s.selective_scan(rows.contiguous(), rows.contiguous(), a, b[:1, :9], b[:1, :9]))
 
 
 def test_captured_graphs_replay():
