@@ -66,4 +66,4 @@ def test_scan_workspaces_hold_what_the_kernels_write():
         assert all(s % 16 == 0 for s in (fwd, keep)) and fwd >= 0
         if fwd:
             segments = fwd // (4 * B * padded * (states + 1))
-            assert fwd == 4 * B * padded * (states + 1) * segments and 1 < segments <= max(1, T // 64)
+            assert fwd == 4 * B * padded * (states + 1) * segments and 1 < segments <= max(1, T // 16)

@@ -18,6 +18,7 @@
 // product of decays is exp(a sum dt)), a small one chains them, and the full pass starts every segment from its true
 // state.  The backward does the same from the other end.  For the backward the forward keeps h before every tile but the first.
 // States in workspaces lie as [..][channel, a group's padded to per_pad][NP], NP = 8, 16, 32 or 64 >= N.
+#include <algorithm>
 #include "seq.h"
 
 namespace {
@@ -883,18 +884,22 @@ int np_of(int N) { return N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 int fwd_channels(int N) { return N <= 16 ? 64 : N <= 32 ? 32 : 16; }
 int bwd_channels(int N) { return N <= 16 ? 32 * BW : 16 * BW; }
 
-// Segments: none while the waves of whole sequences keep the chip's 1024 SIMDs busy; else enough for some 4096 waves, each
-// of 8 tiles at least.
+// Segments cost a second pass over the tokens, so there are none while whole sequences make 640 waves (of 512 tokens x 2048
+// channels, forward: 768 waves 180 us and 220 in segments; 512 waves 181 us and 168).  Below that, enough for 4096 waves with
+// eight tiles each at least (2048 to 8192 waves are the same within 3 %), or for 1024 waves with two tiles each, whichever is
+// more (3 x 577 x 600, 30 waves whole, training: 145 us with eight tiles each, 101 with four, 82 with two).
 void plan(Args& A) {
     A.per = A.D / A.G;
     A.fblk = (A.per + fwd_channels(A.N) - 1) / fwd_channels(A.N);
     A.bblk = (A.per + bwd_channels(A.N) - 1) / bwd_channels(A.N);
     A.per_pad = A.bblk * bwd_channels(A.N);
     const long waves = (long)A.B * A.G * A.fblk;
-    long s = waves >= 1024 ? 1 : 4096 / waves;
-    const long most = A.L / (8 * TT);
-    if (s > most) s = most;
-    if (s < 1) s = 1;
+    long s = 1;
+    if (waves < 640) {
+        s = std::min(4096 / waves, (long)A.L / (8 * TT));
+        s = std::max(s, std::min(1024 / waves, (long)A.L / (2 * TT)));
+        s = std::max(s, 1L);
+    }
     long len = (A.L + s - 1) / s;
     len = (len + TT - 1) / TT * TT;
     A.seg_len = (int)len;
