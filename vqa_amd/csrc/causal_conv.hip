@@ -6,7 +6,7 @@
 // All of it is bound by HBM, the backward nearly as much by its 35 operations per element: a thread owns four channels and
 // walks down a chunk of rows with the filter's window in registers, so a row is loaded once per chunk, plus W - 1 rows at its
 // border.  The backward recomputes pre_t from x (nothing is saved) and carries the window of g the same way.
-// Measured at 8 x 4096 x 2048 bf16, 4 taps, silu: forward 56 us = 4.8 TB/s, backward 94 us = 4.3 TB/s (a large copy: 5.1).
+// Measured at 8 x 4096 x 2048 bf16, 4 taps, silu: forward 56 us = 4.8 TB/s, backward 87 us = 4.6 TB/s (a large copy: 5.1).
 #include "seq.h"
 
 namespace {
@@ -295,7 +295,8 @@ struct Fwd {
 
 // The backward's grid: lx lanes x V channels across, the rest of a workgroup's 256 threads down the chunks of rows.  Chunks as
 // long as 100k threads allow (every chunk computes W - 1 rows of its neighbour's g again and steps in and out of the
-// body's unrolled rows): at 8 x 4096 x 2048 bf16 94 us with 128 rows, 105 with 64, 116 with 32; 64 x 256 x 1024 takes 32 us
+// body's unrolled rows; while border rows were still loaded one by one, 8 x 4096 x 2048 bf16 took 94 us with 128 rows, 105 with
+// 64, 116 with 32); 64 x 256 x 1024 takes 32 us
 // where chunks shrink to keep 65k or 100k threads, 44 us where 32k are let through.
 struct Grid { int lx, gx, gy, chunk; };
 Grid bwd_grid(int B, int L, int D, int V) {

@@ -228,9 +228,9 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_bwd(const T* __res
 }
 
 // Lanes per row and elements per lane.  A wave holds up to 2048 columns, 32 a lane, where its registers allow two waves a
-// SIMD: the forward, and the backward of 16-bit rows without a tail (65536 x 2048 bf16: 160 us, with 256 lanes a row
-// 194; forward 102 and 122).  Else (`wide`) those rows take 256 lanes (backward, 16000 x 1999 bf16: 47 us and 52 with one wave;
-// 16000 x 1600 f32: 55 and 65).
+// SIMD: 16-bit rows in the forward, and in the backward where they have no tail (65536 x 2048 bf16: forward 104 us, backward
+// 163; with 256 lanes a row 120 and 166).  Else (`wide`) those rows take 256 lanes (backward, 16000 x 1999 bf16: 44 us, 49 with
+// one wave; 16000 x 1600 f32: 50 and 59).
 struct Shape { int team, e; };
 Shape shape_of(int width, bool wide) {
     if (width <= 512) return {64, 8};
@@ -248,11 +248,15 @@ int bwd_groups(long rows, int team) {
 }
 
 template <typename T, int V, bool TAIL, typename F> int by_shape(int width, F f) {
-    const Shape s = shape_of(width - width % V, F::wide(sizeof(T), TAIL));
+    constexpr bool wide = F::wide(sizeof(T), TAIL);
+    const Shape s = shape_of(width - width % V, wide);
     if (s.team == 64 && s.e == 8) return f.template operator()<T, V, 64, 8 / V, TAIL>();
     if (s.team == 64 && s.e == 16) return f.template operator()<T, V, 64, 16 / V, TAIL>();
-    if (s.team == 64) return f.template operator()<T, V, 64, 32 / V, TAIL>();
-    if (s.team == 256 && s.e == 8) return f.template operator()<T, V, 256, 8 / V, TAIL>();
+    if constexpr (wide) {
+        if (s.team == 256 && s.e == 8) return f.template operator()<T, V, 256, 8 / V, TAIL>();
+    } else {
+        if (s.team == 64) return f.template operator()<T, V, 64, 32 / V, TAIL>();
+    }
     if (s.team == 256) return f.template operator()<T, V, 256, 16 / V, TAIL>();
     return f.template operator()<T, V, 512, 16 / V, TAIL>();
 }
@@ -268,7 +272,7 @@ template <typename F> int by_type(int dtype, int width, F f) {
 }
 
 struct Fwd {
-    static bool wide(int bytes, bool) { return bytes == 4; }
+    static constexpr bool wide(int bytes, bool) { return bytes == 4; }
     hipStream_t st; const void* x; long ldx; const float *w, *b; long rows; int width; float eps; void* y; float *mean, *rstd;
     template <typename T, int V, int TEAM, int NV, bool TAIL> int operator()() const {
         const long grid = TEAM == 64 ? (rows + 3) / 4 : rows;
@@ -279,7 +283,7 @@ struct Fwd {
     }
 };
 struct Bwd {
-    static bool wide(int bytes, bool tail) { return bytes == 4 || tail; }
+    static constexpr bool wide(int bytes, bool tail) { return bytes == 4 || tail; }
     hipStream_t st; const void* dy; long lddy; const void* x; long ldx; const float *w, *mean, *rstd; long rows; int width;
     void* dx; float *dw, *db, *part;
     template <typename T, int V, int TEAM, int NV, bool TAIL> int operator()() const {
