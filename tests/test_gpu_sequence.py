@@ -106,7 +106,7 @@ def test_layer_norm_of_strided_rows(width, dtype):
     y, yr = S().layer_norm(x), R.norm(xr, None, None)
     y.sum().backward()                                       # dy with strides 0
     # xhat sums to 0 over a row, so the exact gradient of the sum is 0: what is left is rounding of terms of size rstd
-    assert float(x.grad.abs().max()) <= 64 * 2.0 ** -24 * float(1 / xr.std(1, unbiased=False).min())
+    assert float(x.grad.abs().max()) <= 64 * 2.0 ** -24 * float(1 / xr.detach().std(1, unbiased=False).min())
 
 
 def test_layer_norm_extremes():
@@ -363,6 +363,19 @@ def test_selective_scan_strided_and_shared(dtype, D):
                                 torch.ones_like(y))
     assert float((gb.double() - gf.double().sum(0, keepdim=True)).abs().max()) <= 4 * torch.finfo(t).eps * float(
         gf.double().abs().sum(0).max())
+
+
+def test_softplus_over_its_range():
+    """dt alone: one token from the zero state with x = b = c = 1, so y = dt = softplus(raw), relative to its own value over
+    the whole range of an f32 exponential (a chain of some 16 roundings)."""
+    raw = torch.cat([torch.linspace(-80, 40, 4001), torch.tensor([0.0, -0.0, 1e-30, -1e-30, 88.0, 200.0])])
+    D = raw.numel()
+    x, one = torch.ones(1, 1, D, device='cuda'), torch.ones(1, 1, 1, device='cuda')
+    y = S().selective_scan(x, raw.cuda().view(1, 1, D), -torch.ones(D, 1, device='cuda'), one, one)
+    want = torch.nn.functional.softplus(raw.double(), threshold=1e9)
+    # exp(-|raw|) is off by raw's rounding times log2 e: |raw| 2^-24 relative on the small side
+    tol = (16 + raw.double().abs().clamp(max=80) * 2) * 2.0 ** -24 * want
+    assert ((y.cpu().view(-1).double() - want).abs() <= tol).all()
 
 
 def test_selective_scan_of_nothing():

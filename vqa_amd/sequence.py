@@ -174,7 +174,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
             return layer_norm(x, weight, bias, eps)
     if x.dim() < 1 or not 1 <= x.shape[-1] <= 8192:
         _fail(f'x has shape {tuple(x.shape)}: a last axis of 1 to 8192 is wanted')
-    weight, bias = _param('weight', weight, x.shape[-1:], x), _param('bias', bias, x.shape[-1:], x)
+    width = (x.shape[-1],)
+    weight, bias = _param('weight', weight, width, x), _param('bias', bias, width, x)
     if _tracked(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, eps)
     return _norm_fwd(x, weight, bias, eps, False)[0]
