@@ -427,6 +427,29 @@ def selective_scan(x, dt, a, b, c, skip=None, gate=None, dt_bias=None, softplus=
     return (y, last) if return_state else y
 
 
+def _ready(x, dt, a, b, c, skip, gate, dt_bias):
+    """(G, N) where every argument of a step is already as its kernel takes it - the usual case, found by a third of
+    _scan_args' host time.  None: _scan_args says what is wrong, or makes copies."""
+    t, g, rows, shared = x.dtype, x.get_device(), x.shape, b.shape
+    k = len(shared)
+    N = shared[-1] if k else 0
+    G = shared[1] if k == 3 else 1
+    D = rows[1]
+    if (k == 2 or k == 3) and shared[0] == rows[0] and 1 <= N <= 64 and G > 0 and D % G == 0 \
+            and dt.dtype is t and dt.get_device() == g and dt.shape == rows and dt.stride(1) == 1 and x.stride(1) == 1 \
+            and b.dtype is t and b.get_device() == g and b.stride(-1) == 1 and (G == 1 or b.stride(1) == N) \
+            and c.dtype is t and c.get_device() == g and c.shape == shared and c.stride(-1) == 1 \
+            and (G == 1 or c.stride(1) == N) and a.dtype is _F32 and a.get_device() == g and a.shape == (D, N) \
+            and a.is_contiguous() \
+            and (gate is None or (gate.dtype is t and gate.get_device() == g and gate.shape == rows
+                                  and gate.stride(1) == 1)):
+        for p in (skip, dt_bias):
+            if p is not None and not (p.dtype is _F32 and p.get_device() == g and p.shape == (D,) and p.is_contiguous()):
+                return None
+        return G, N
+    return None
+
+
 def selective_scan_step(x, state, dt, a, b, c, skip=None, gate=None, dt_bias=None, softplus=True):
     """selective_scan for ONE new token per sequence: x, dt, gate [B, D]; b, c [B, N] or [B, G, N]; state float32
     [B, D, N] is updated in place (its batch axis may be strided).  Returns y [B, D].  Forward only."""
@@ -434,27 +457,31 @@ def selective_scan_step(x, state, dt, a, b, c, skip=None, gate=None, dt_bias=Non
     if _elsewhere(x):
         with torch.cuda.device(x.device):
             return selective_scan_step(x, state, dt, a, b, c, skip, gate, dt_bias, softplus)
-    x, dt, a, b, c, skip, gate, dt_bias = _scan_args(x, dt, a, b, c, skip, gate, dt_bias)
     B, D = x.shape
-    G, N = b.shape[1:]
-    if state.dtype != torch.float32 or state.device != x.device or state.shape != (B, D, N):
+    ready = _ready(x, dt, a, b, c, skip, gate, dt_bias)
+    if ready is None:
+        x, dt, a, b, c, skip, gate, dt_bias = _scan_args(x, dt, a, b, c, skip, gate, dt_bias)
+        ready = b.shape[1:]
+    G, N = ready
+    if state.dtype is not _F32 or state.get_device() != x.get_device() or state.shape != (B, D, N):
         _fail(f'state is {state.dtype} {tuple(state.shape)} on {state.device}: float32 {(B, D, N)} on {x.device} is wanted')
     _no_tracking('selective_scan_step', x, state, dt, a, b, c, skip, gate, dt_bias)
     y = torch.empty(B, D, device=x.device, dtype=x.dtype)
     if not y.numel():
         return y
-    if (state.stride(2) != 1 and N > 1) or (state.stride(1) != N and D > 1) or (B > 1 and state.stride(0) < D * N):
+    s0, s1, s2 = state.stride()
+    if (s2 != 1 and N > 1) or (s1 != N and D > 1) or (B > 1 and s0 < D * N):
         _fail(f'state has strides {state.stride()}: it is updated in place, so [D, N] must be contiguous and apart')
     sg = 0 if gate is None else gate.stride(0)
     if L._PROFILE is None and L._REC is None:
         # (one token's latency is host time: pointers are taken here, 3 us less than by L.call)
         L.check(L.lib().vqa_scan_token(
-            L._raw_stream(), L.dt(x), x.data_ptr(), x.stride(0), state.data_ptr(), state.stride(0), dt.data_ptr(),
+            L._raw_stream(), L.dt(x), x.data_ptr(), x.stride(0), state.data_ptr(), s0, dt.data_ptr(),
             dt.stride(0), None if gate is None else gate.data_ptr(), sg, a.data_ptr(), b.data_ptr(), b.stride(0),
             c.data_ptr(), c.stride(0), None if skip is None else skip.data_ptr(),
             None if dt_bias is None else dt_bias.data_ptr(), softplus, B, D, N, G, y.data_ptr()), 'vqa_scan_token')
     else:
-        L.call('vqa_scan_token', L.dt(x), x, x.stride(0), state, state.stride(0), dt, dt.stride(0), gate, sg, a, b,
+        L.call('vqa_scan_token', L.dt(x), x, x.stride(0), state, s0, dt, dt.stride(0), gate, sg, a, b,
                b.stride(0), c, c.stride(0), skip, dt_bias, softplus, B, D, N, G, y)
     _touched(state)
     return y
