@@ -313,9 +313,11 @@ def test_selective_scan_options(without, softplus, carry):
     _scan_check(leaves, dy, dlast, None, softplus)
 
 
-def test_selective_scan_many_sequences_in_one_wave():
-    """More batch rows than waves are wanted for: a wave takes several, its parameter sums run on."""
-    B, T, D, N = 300, 3, 1024, 16
+@pytest.mark.parametrize('N', [16, 8, 20])
+def test_selective_scan_many_sequences_in_one_wave(N):
+    """More batch rows than waves are wanted for: a wave takes several, its parameter sums run on; and fewer, where a wave
+    takes half the channels: the same bits."""
+    B, T, D = 300, 3, 1024
     leaves, dy, _ = _scan_case(B, T, D, N, 1, 'f32', seed=3, carry=False)
     G = {k: v[0] for k, v in leaves.items()}
     y = S().selective_scan(*(G[k] for k in SCAN[:8]))

@@ -37,6 +37,7 @@ struct Args {
     int softplus, B, L, D, N, G;
     int per, per_pad, fblk, bblk;          // channels of a group, padded; forward waves, backward workgroups across it
     int segs, seg_len, bgroups;            // segments, tokens of one, batch groups of the backward
+    bool narrow;                           // forward waves of half the channels
     void* y; float* last;
     float *keep, *seg_h, *seg_dt;          // h before the tiles; per segment: state, then the true incoming one; sum dt
     void *dx, *ddt, *dgate; float *part_bc, *part_p, *dstate;
@@ -147,12 +148,15 @@ template <typename T, int CH, int NS, int VE> struct Wave {
     __device__ __forceinline__ bool staged(int k, int v, int t0, int te) const {
         return t0 + trow(k) < te && c0 + tcol(k) + v < cend;
     }
-    // (a tile's base is uniform; 8 rows of any tensor span less than 2^31 bytes: the host sees to it)
+    // A tile's base is uniform; 8 rows of any tensor span less than 2^31 bytes: the host sees to it.  there = false gives a
+    // range of 0 bytes instead of a branch around the accesses: the hardware counts loads and stores in one order, and
+    // behind a branch that may skip stores the compiler waits for them where it needs the loads before them (the forward of
+    // 32 x 512 x 2048 keeping its states: 288 us with the branches, 238 without).
     __device__ __forceinline__ unsigned place(int k, int row, int t0, int te) const {
         return t0 + trow(k) < te && c0 + tcol(k) < cend ? (trow(k) * row + tcol(k)) * (unsigned)sizeof(T) : BUF_OUT;
     }
-    __device__ __forceinline__ void fetch(const Rows& R, int b, int t0, int te, Raw<T, VE> (&v)[NV]) const {
-        const auto rs = buffer_of(static_cast<const T*>(R.p) + b * R.batch + t0 * R.row + c0, BUF_BYTES);
+    __device__ __forceinline__ void fetch(const Rows& R, int b, int t0, int te, Raw<T, VE> (&v)[NV], bool there = true) const {
+        const auto rs = buffer_of(static_cast<const T*>(R.p) + b * R.batch + t0 * R.row + c0, there ? BUF_BYTES : 0);
 #pragma unroll
         for (int k = 0; k < NV; ++k) v[k] = buf_load<T, VE>(rs, place(k, (int)R.row, t0, te));
     }
@@ -222,8 +226,8 @@ template <typename T, int CH, int NS, int VE> struct Wave {
                 for (int q = 0; q < SV; ++q) h[i][j + q] = f.get(q);
             }
     }
-    __device__ __forceinline__ void store_own(float* p, const float (&h)[CH][NS]) const {
-        const auto rs = buffer_of(p, BUF_BYTES);
+    __device__ __forceinline__ void store_own(float* p, const float (&h)[CH][NS], bool there = true) const {
+        const auto rs = buffer_of(p, there ? BUF_BYTES : 0);
 #pragma unroll
         for (int i = 0; i < CH; ++i)
 #pragma unroll
@@ -326,14 +330,7 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
         }
     };
     fetch(ts);
-    for (int t0 = ts; t0 < te; t0 += TT) {
-        if (t0 >= len) {                                   // nothing left of this sequence: zero rows
-            if (!FULL) break;
-#pragma unroll
-            for (int k = 0; k < W::NV; ++k) x[k].zero();
-            w.put(A.y, b, A.L, A.D, t0, te, x);
-            continue;
-        }
+    for (int t0 = ts; t0 < live; t0 += TT) {
 #pragma unroll
         for (int k = 0; k < W::NV; ++k) { x[k] = xn[k]; d[k] = dn[k]; }
         lds_order();                                       // (the last tile's reads are done)
@@ -352,10 +349,9 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
             if (FULL) s_c[k * 64 + w.lane] = shared_value<T>(cn[k]);
         }
         lds_order();
-        if (FULL && A.gate.p) w.fetch(A.gate, b, t0, live, z);
-        if (t0 + TT < te) fetch(t0 + TT);
-        if (FULL && A.keep && t0 > 0)
-            w.store_own(A.keep + (((long)b * kept_tiles(A.L) + t0 / TT - 1) * chans + w.p0) * W::NP, h);
+        if (FULL) w.fetch(A.gate, b, t0, live, z, A.gate.p != nullptr);
+        fetch(t0 + TT);                                    // (past the end: zeros)
+        if (FULL) w.store_own(A.keep + (((long)b * kept_tiles(A.L) + t0 / TT - 1) * chans + w.p0) * W::NP, h, A.keep && t0 > 0);
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
             float dt[CH], dtx[CH], bv[NS], cv[NS], y[CH];
@@ -397,6 +393,11 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
         }
     }
     if (FULL) {
+        for (int t0 = live > ts ? ts + (live - ts + TT - 1) / TT * TT : ts; t0 < te; t0 += TT) {     // past the end: zero rows
+#pragma unroll
+            for (int k = 0; k < W::NV; ++k) x[k].zero();
+            w.put(A.y, b, A.L, A.D, t0, te, x);
+        }
         if (A.last && seg == A.segs - 1) w.store_public(A.last, b, A.D, A.N, h);
     } else {
         w.store_own(A.seg_h + at_seg * W::NP, h);
@@ -903,6 +904,10 @@ void plan(Args& A) {
     len = (len + TT - 1) / TT * TT;
     A.seg_len = (int)len;
     A.segs = (int)((A.L + len - 1) / len);
+    // whole sequences in few waves: half the channels a wave, twice the waves (32 x 512 x 2048: 168 us, 190 without; at 4096
+    // waves no difference)
+    A.narrow = A.segs == 1 && waves < 4096 && A.N <= 32;
+    if (A.narrow) A.fblk = (A.per + fwd_channels(A.N) / 2 - 1) / (fwd_channels(A.N) / 2);
     // the backward's sums over tokens leave a workgroup once: as few workgroups as still fill the chip
     const long g = 1024 / ((long)A.G * A.bblk * A.segs);
     A.bgroups = (int)(g < 1 ? 1 : g > A.B ? A.B : g);
@@ -949,6 +954,12 @@ template <typename T, int NS, int CH, int VE, int BCH, int BVE> int launch(bool 
         rc = bwd ? chain<4 * NS, true>(A, st) : chain<4 * NS, false>(A, st);
         if (rc != VQA_OK) return rc;
     }
+    if constexpr (CH > 1)
+        if (!bwd && A.narrow) {
+            scan_fwd<T, CH / 2, NS, (VE < CH ? VE : CH), true><<<waves, 64, 0, st>>>(A);
+            CHECK_LAUNCH();
+            return VQA_OK;
+        }
     if (bwd) scan_bwd<T, BCH, NS, BVE><<<(unsigned)((long)A.bblk * A.G * A.segs * A.bgroups), 64 * BW, 0, st>>>(A);
     else scan_fwd<T, CH, NS, VE, true><<<waves, 64, 0, st>>>(A);
     CHECK_LAUNCH();
