@@ -884,18 +884,19 @@ int np_of(int N) { return N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 int fwd_channels(int N) { return N <= 16 ? 64 : N <= 32 ? 32 : 16; }
 int bwd_channels(int N) { return N <= 16 ? 32 * BW : 16 * BW; }
 
-// Segments cost a second pass over the tokens, so there are none while whole sequences make 640 waves (of 512 tokens x 2048
-// channels, forward: 768 waves 180 us and 220 in segments; 512 waves 181 us and 168).  Below that, enough for 4096 waves with
-// eight tiles each at least (2048 to 8192 waves are the same within 3 %), or for 1024 waves with two tiles each, whichever is
-// more (3 x 577 x 600, 30 waves whole, training: 145 us with eight tiles each, 101 with four, 82 with two).
-void plan(Args& A) {
+// Segments cost a second pass over the tokens, so there are none while whole sequences make enough waves (counted in the
+// forward's 64 channels): 400 in the forward (B x 512 x 2048: 512 waves 122 us and 162 in segments, 384 118 and 124, 256 115
+// and 90), 640 in the backward (768 waves 446 us and 472, 512 335 and 316).  Below that, enough for 4096 waves with eight tiles
+// each at least (2048 to 8192 waves are the same within 3 %), or for 1024 waves with two tiles each, whichever is more
+// (3 x 577 x 600, 30 waves whole, training: 145 us with eight tiles each, 101 with four, 82 with two).
+void plan(Args& A, bool bwd) {
     A.per = A.D / A.G;
     A.fblk = (A.per + fwd_channels(A.N) - 1) / fwd_channels(A.N);
     A.bblk = (A.per + bwd_channels(A.N) - 1) / bwd_channels(A.N);
     A.per_pad = A.bblk * bwd_channels(A.N);
     const long waves = (long)A.B * A.G * A.fblk;
     long s = 1;
-    if (waves < 640) {
+    if (waves < (bwd ? 640 : 400)) {
         s = std::min(4096 / waves, (long)A.L / (8 * TT));
         s = std::max(s, std::min(1024 / waves, (long)A.L / (2 * TT)));
         s = std::max(s, 1L);
@@ -984,8 +985,9 @@ extern "C" int vqa_scan_ws_bytes(int dtype, int B, int L, int D, int N, int G, l
     if (bad_shape(dtype, B, L, D, N, G) || !sizes) return VQA_ERR_ARG;
     Args A = {};
     A.B = B; A.L = L; A.D = D; A.N = N; A.G = G;
-    plan(A);
+    plan(A, false);
     sizes[0] = 4 * seg_floats(A);
+    plan(A, true);
     sizes[1] = 4L * B * kept_tiles(L) * G * A.per_pad * np_of(N);
     sizes[2] = 4 * (seg_floats(A) + part_p_floats(A) + part_bc_floats(A));
     return VQA_OK;
@@ -1003,7 +1005,7 @@ extern "C" int vqa_scan_fwd(void* stream, int dtype, const void* x, long x_batch
     A.b = {b, b_batch, b_row}; A.c = {c, c_batch, c_row};
     A.a = a; A.skip = skip; A.dt_bias = dt_bias; A.state = state; A.lengths = lengths; A.softplus = softplus;
     A.B = B; A.L = L; A.D = D; A.N = N; A.G = G; A.y = y; A.last = last; A.keep = keep;
-    plan(A);
+    plan(A, false);
     if ((A.segs > 1 && !ws) || !aligned16(ws) || !aligned16(keep) || far_rows(A)) return VQA_ERR_ARG;
     A.seg_h = ws;
     A.seg_dt = ws ? seg_dt_of(A, ws) : nullptr;
@@ -1030,7 +1032,7 @@ extern "C" int vqa_scan_bwd(void* stream, int dtype, const void* dy, long dy_bat
     A.B = B; A.L = L; A.D = D; A.N = N; A.G = G; A.keep = const_cast<float*>(keep);
     A.dx = dx; A.ddt = ddt; A.dgate = dgate; A.dstate = dstate;
     if (far_rows(A)) return VQA_ERR_ARG;
-    plan(A);
+    plan(A, true);
     A.seg_h = ws;
     A.seg_dt = seg_dt_of(A, ws);
     A.part_p = ws + seg_floats(A);
