@@ -674,6 +674,26 @@ def test_inference_mode():
         assert z.shape == (2, 16) and s.layer_norm(x).shape == x.shape
 
 
+def test_one_row_at_any_stride():
+    """A sequence of one token whose row stride says nothing: torch calls it contiguous at any stride."""
+    s = S()
+    buf = torch.randn(2, 64, generator=_gen(90)).cuda().bfloat16()
+    far = lambda t: t.as_strided((2, 1, t.shape[1]), (t.shape[1], 1 << 40, 1))       # noqa: E731
+    near = lambda t: t.clone().view(2, 1, -1)      # noqa: E731
+    w, a, g = torch.randn(64, 4, generator=_gen(91)).cuda(), -torch.rand(64, 8, device='cuda'), buf[:, :8].contiguous()
+    got, want = [], []
+    for view, out in ((far, got), (near, want)):
+        x = buf.clone().requires_grad_(True)
+        b = g.clone().requires_grad_(True)
+        u = view(x) if view is far else x.view(2, 1, 64)
+        v = view(b) if view is far else b.view(2, 1, 8)
+        y = s.selective_scan(u, u, a, v, v, gate=u)
+        out += [y, s.causal_conv(u, w), s.layer_norm(u)]
+        dy = view(torch.ones(2, 64, device='cuda', dtype=torch.bfloat16))
+        out += torch.autograd.grad(y, [x, b], dy)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 def test_refusals():
     s = S()
     from vqa_amd._lib import VqaHipError

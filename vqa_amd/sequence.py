@@ -84,7 +84,9 @@ def _unit(x):
 
 def _near(x):
     """... and rows whose distance the scan's kernels can take (8 rows within 2 GiB)"""
-    return x if x.stride(-1) == 1 and (x.dim() == 2 or x.stride(1) < 1 << 26) else x.contiguous()
+    if x.dim() == 2 or x.stride(1) < 1 << 26:
+        return _unit(x)
+    return x.clone(memory_format=torch.contiguous_format)      # (contiguous() keeps the stride of an axis of one row)
 
 
 def _touched(state):
@@ -385,8 +387,9 @@ def _shared(name, b, lead, x):
     if b.dim() == k + 1:
         b = b.unsqueeze(k)
     G, N = b.shape[k:]
-    near = b.stride(-1) == 1 and (G == 1 or b.stride(-2) == N) and (k == 1 or b.stride(1) < 1 << 26)
-    return b if near else b.contiguous()
+    if k == 2 and b.stride(1) >= 1 << 26:
+        return b.clone(memory_format=torch.contiguous_format)  # (as in _near)
+    return b if b.stride(-1) == 1 and (G == 1 or b.stride(-2) == N) else b.contiguous()
 
 
 def _scan_args(x, dt, a, b, c, skip, gate, dt_bias):
