@@ -51,6 +51,21 @@ def test_entry_points_refuse_bad_arguments():
                                   scan(G=3), scan(y=None), scan(B=0)))
 
 
+def test_entry_points_refuse_grids_past_32_bits():
+    """Shapes whose launch would have 2^32 threads or more, within every other limit: refused, nothing is launched."""
+    from vqa_amd import _lib as L
+    lib = L.lib()
+    conv = lambda B, T, D: lib.vqa_causal_conv_fwd(None, 0, P, T * D, D, P, None, None, None, B, T, D, 4, 1, P, None)   # noqa: E731
+    assert conv(1000000000, 1, 20) == 1 and conv(1, 1, 25000001) == 1
+    assert lib.vqa_causal_conv_token(None, 0, P, 7, P, 21, 7, P, None, 700000000, 7, 4, 1, P) == 1
+    token = lambda B, D, N: lib.vqa_scan_token(None, 0, P, D, P, D * N, P, D, None, 0, P, P, N, P, N, None, None, 1,    # noqa: E731
+                                               B, D, N, 1, P)
+    assert token(13000000, 17, 64) == 1
+    sizes = (ctypes.c_long * 3)()
+    assert lib.vqa_scan_ws_bytes(0, 1, 1, 5000000, 64, 1, ctypes.addressof(sizes)) == 1
+    assert lib.vqa_scan_ws_bytes(0, 1, 1, 5000000, 16, 1, ctypes.addressof(sizes)) == 0
+
+
 def test_scan_workspaces_hold_what_the_kernels_write():
     """The forward's segments, the kept states and the backward's partial sums, from the sizes alone."""
     from vqa_amd import _lib as L

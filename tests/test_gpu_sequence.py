@@ -694,6 +694,43 @@ def test_one_row_at_any_stride():
     assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
+def test_layer_norm_of_more_rows_than_a_launch_takes():
+    """Rows past 2^22 and (one wave a row) past 2^32 threads: each as it is by itself."""
+    s = S()
+    rows = (1 << 26) + 5
+    x = torch.empty(rows, 2, device='cuda', dtype=torch.bfloat16).normal_(generator=torch.Generator('cuda').manual_seed(92))
+    w, b = torch.tensor([0.5, -2.0], device='cuda'), torch.tensor([0.25, 1.0], device='cuda')
+    y = s.layer_norm(x, w, b)
+    for r in (0, (1 << 22) - 3, 5 * (1 << 22) - 7, rows - 9):
+        assert torch.equal(y[r:r + 9], s.layer_norm(x[r:r + 9].clone(), w, b))
+    x = x[:(1 << 22) + 7].clone().requires_grad_(True)
+    dy = torch.ones_like(x)
+    dy[:, 1] = 0.5
+    dx, = torch.autograd.grad(s.layer_norm(x, w, b), x, dy)
+    part = x.detach()[-20:].clone().requires_grad_(True)
+    want, = torch.autograd.grad(s.layer_norm(part, w, b), part, dy[-20:].clone())
+    assert torch.equal(dx[-20:], want)
+
+
+def test_selective_scan_gradients_of_many_shared_rows():
+    """More values of db and dc than one pass of the grid that joins them: sequences as they are in halves of the batch
+    (neither is cut into segments)."""
+    s = S()
+    B, T, D, N = 2048, 72, 2, 64
+    x = torch.randn(B, T, D, generator=_gen(93)).cuda()
+    a = -torch.rand(D, N, generator=_gen(94)).cuda()
+    b, c = (torch.randn(B, T, N, generator=_gen(95 + i)).cuda() for i in range(2))
+    lens = torch.randint(0, T + 1, (B,), generator=_gen(97), dtype=torch.int32).cuda()
+
+    def grads(lo, hi):
+        bb, cc = b[lo:hi].clone().requires_grad_(True), c[lo:hi].clone().requires_grad_(True)
+        y = s.selective_scan(x[lo:hi], x[lo:hi], a, bb, cc, lengths=lens[lo:hi])
+        return torch.autograd.grad(y, [bb, cc], torch.ones_like(y))
+    whole, first, second = grads(0, B), grads(0, B // 2), grads(B // 2, B)
+    for t in range(2):
+        assert torch.equal(whole[t][:B // 2], first[t]) and torch.equal(whole[t][B // 2:], second[t])
+
+
 def test_refusals():
     s = S()
     from vqa_amd._lib import VqaHipError

@@ -268,8 +268,9 @@ template <typename F> int by_type(int dtype, bool vec, int taps, int silu, F f) 
 }
 
 bool bad_shape(int dtype, int B, long L, int D, int taps) {
-    return !vqa_dtype_ok(dtype) || B < 1 || L < 1 || D < 1 || taps < 2 || taps > 4 ||
-           (double)B * L > 1e9 || (double)B * L * D > 4e11;
+    return !vqa_dtype_ok(dtype) || B < 1 || L < 1 || D < 1 || taps < 2 || taps > 4 || D > 25000000 ||
+           (double)B * L > 1e9 || (double)B * L * D > 4e11 ||
+           (double)B * ((L + 31) / 32) * (D < 4 ? D : (D + 3) / 4) > 4e9;       // (a grid has fewer than 2^32 threads)
 }
 
 int fwd_chunk(int B, int L, int nv) {
@@ -370,7 +371,8 @@ extern "C" int vqa_causal_conv_bwd(void* stream, int dtype, const void* dy, long
 extern "C" int vqa_causal_conv_token(void* stream, int dtype, const void* x, long x_batch, void* state, long state_batch,
                                      long state_row, const float* weight, const float* bias, int B, int D, int taps,
                                      int silu, void* y) {
-    if (bad_shape(dtype, B, 1, D, taps) || !x || !state || !weight || !y) return VQA_ERR_ARG;
+    if (bad_shape(dtype, B, 1, D, taps) || (D % 4 != 0 && (double)B * D > 4e9) || !x || !state || !weight || !y)
+        return VQA_ERR_ARG;
     return by_type(dtype, D % 4 == 0, taps, silu,            // (in place: no two threads may take the same channel)
                    Token{static_cast<hipStream_t>(stream), x, x_batch, state, state_batch, state_row, weight, bias, B, D, y});
 }

@@ -6,6 +6,7 @@
 // sums - and the result is written from there.  The backward's workgroups walk over rows and keep their share of dw / db
 // in registers; one partial row per workgroup is written and summed in a fixed order (no atomics: the same bits every
 // time).
+#include <algorithm>
 #include "seq.h"
 
 namespace {
@@ -240,6 +241,7 @@ Shape shape_of(int width, bool wide) {
     return {512, 16};
 }
 constexpr int MAX_WIDTH = 8192;
+constexpr long MAX_ROWS = 1 << 22;                         // of one launch: a grid has fewer than 2^32 threads
 
 int bwd_groups(long rows, int team) {
     const long per = team == 64 ? 4 : 1;
@@ -275,10 +277,13 @@ struct Fwd {
     static constexpr bool wide(int bytes, bool) { return bytes == 4; }
     hipStream_t st; const void* x; long ldx; const float *w, *b; long rows; int width; float eps; void* y; float *mean, *rstd;
     template <typename T, int V, int TEAM, int NV, bool TAIL> int operator()() const {
-        const long grid = TEAM == 64 ? (rows + 3) / 4 : rows;
-        ln_fwd<T, V, TEAM, NV, TAIL><<<(unsigned)grid, TEAM == 64 ? 256 : TEAM, 0, st>>>(
-            static_cast<const T*>(x), ldx, w, b, rows, width, eps, static_cast<T*>(y), mean, rstd);
-        CHECK_LAUNCH();
+        for (long r = 0; r < rows; r += MAX_ROWS) {
+            const long n = std::min(rows - r, MAX_ROWS), grid = TEAM == 64 ? (n + 3) / 4 : n;
+            ln_fwd<T, V, TEAM, NV, TAIL><<<(unsigned)grid, TEAM == 64 ? 256 : TEAM, 0, st>>>(
+                static_cast<const T*>(x) + r * ldx, ldx, w, b, n, width, eps, static_cast<T*>(y) + r * width,
+                mean ? mean + r : nullptr, rstd ? rstd + r : nullptr);
+            CHECK_LAUNCH();
+        }
         return VQA_OK;
     }
 };

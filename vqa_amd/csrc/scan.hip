@@ -804,15 +804,16 @@ __global__ __launch_bounds__(1024) void scan_params(const float* __restrict__ pa
 template <typename T>
 __global__ __launch_bounds__(256) void scan_shared(const float* __restrict__ part, const int* __restrict__ lengths, int B,
                                                    int L, int G, int N, int nblk, T* __restrict__ db, T* __restrict__ dc) {
-    const long n = (long)B * L * G * 2 * N, id = (long)blockIdx.x * 256 + threadIdx.x;
-    if (id >= n) return;
-    const long tok = id / (2 * N * G);
-    float s = 0.f;
-    if (!lengths || (int)(tok % L) < lengths[tok / L])
-        for (int k = 0; k < nblk; ++k) s += part[k * n + id];
-    const long row = id / (2 * N);
-    const int e = (int)(id % (2 * N));
-    (e < N ? db[row * N + e] : dc[row * N + e - N]) = from_f32<T>(s);
+    const long n = (long)B * L * G * 2 * N;
+    for (long id = (long)blockIdx.x * 256 + threadIdx.x; id < n; id += (long)gridDim.x * 256) {
+        const long tok = id / (2 * N * G);
+        float s = 0.f;
+        if (!lengths || (int)(tok % L) < lengths[tok / L])
+            for (int k = 0; k < nblk; ++k) s += part[k * n + id];
+        const long row = id / (2 * N);
+        const int e = (int)(id % (2 * N));
+        (e < N ? db[row * N + e] : dc[row * N + e - N]) = from_f32<T>(s);
+    }
 }
 
 // One token: a lane takes four states of a channel, LN lanes a channel, 256 / LN channels of one sequence a workgroup.  Bound
@@ -917,7 +918,7 @@ void plan(Args& A, bool bwd) {
 bool bad_shape(int dtype, int B, int L, int D, int N, int G) {
     return !vqa_dtype_ok(dtype) || B < 1 || L < 1 || L > 0x3fffffff || D < 1 || N < 1 || N > 64 || G < 1 || D % G != 0 ||
            (double)B * L > 1e9 || (double)B * L * D > 4e11 || (double)B * D > 1e9 || (double)B * L * G * N > 1e11 ||
-           (double)G * (D / G + 128) * B > 2e9;
+           (double)G * (D / G + 128) * B > 2e9 || (double)G * (D / G + 128) * (np_of(N) + 2) > 2.5e8;
 }
 // (buffer accesses of up to 16 bytes want their addresses on 4 bytes)
 bool on4(const void* p, long stride, int e) { return ((uintptr_t)p & 3) == 0 && stride * e % 4 == 0; }
@@ -1050,7 +1051,7 @@ extern "C" int vqa_scan_bwd(void* stream, int dtype, const void* dy, long dy_bat
     else if (np == 32) scan_params<32><<<pg, 1024, 0, st>>>(A.part_p, rows, A.per, A.per_pad, N, G, da, dskip, ddt_bias);
     else scan_params<64><<<pg, 1024, 0, st>>>(A.part_p, rows, A.per, A.per_pad, N, G, da, dskip, ddt_bias);
     CHECK_LAUNCH();
-    const unsigned sg = (unsigned)(((long)B * L * G * 2 * N + 255) / 256);
+    const unsigned sg = (unsigned)std::min(((long)B * L * G * 2 * N + 255) / 256, 65536L);
     if (dtype == VQA_F32)
         scan_shared<float><<<sg, 256, 0, st>>>(A.part_bc, lengths, B, L, G, N, A.bblk, static_cast<float*>(db), static_cast<float*>(dc));
     else if (dtype == VQA_BF16)
@@ -1085,7 +1086,8 @@ extern "C" int vqa_scan_token(void* stream, int dtype, const void* x, long x_bat
                               const void* dt, long dt_batch, const void* gate, long gate_batch, const float* a,
                               const void* b, long b_batch, const void* c, long c_batch, const float* skip,
                               const float* dt_bias, int softplus, int B, int D, int N, int G, void* y) {
-    if (bad_shape(dtype, B, 1, D, N, G) || D > 100000000 || !x || !state || !dt || !a || !b || !c || !y) return VQA_ERR_ARG;
+    // (at most 16 lanes a channel, 256 threads a workgroup, and a grid has fewer than 2^32 threads)
+    if (bad_shape(dtype, B, 1, D, N, G) || (double)B * ((D + 15) / 16) > 1.6e7 || !x || !state || !dt || !a || !b || !c || !y) return VQA_ERR_ARG;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const Rows rx = {x, x_batch, 0}, rd = {dt, dt_batch, 0}, rg = {gate, gate_batch, 0}, rb = {b, b_batch, 0}, rc = {c, c_batch, 0};
     if (dtype == VQA_F32) return token<float>(st, rx, state, state_batch, rd, rg, rb, rc, a, skip, dt_bias, softplus, B, D, N, G, y);
