@@ -800,19 +800,27 @@ __global__ __launch_bounds__(1024) void scan_params(const float* __restrict__ pa
     } else if (dbias) dbias[c] = t;
 }
 
-// db and dc: the channel blocks' shares in a fixed order; rows past a sequence's length are 0
+// db and dc: the channel blocks' shares in a fixed order; rows past a sequence's length are 0.  Each share is read once;
+// eight in flight a thread and 32-bit divisions: 4 x 2048 x 2048 5.8 us (17 MB), 9.7 with a load at a time and 64 bits
 template <typename T>
 __global__ __launch_bounds__(256) void scan_shared(const float* __restrict__ part, const int* __restrict__ lengths, int B,
                                                    int L, int G, int N, int nblk, T* __restrict__ db, T* __restrict__ dc) {
     const long n = (long)B * L * G * 2 * N;
-    for (long id = (long)blockIdx.x * 256 + threadIdx.x; id < n; id += (long)gridDim.x * 256) {
-        const long tok = id / (2 * N * G);
+    const int w = G * 2 * N;                               // values a token
+    for (long id0 = (long)blockIdx.x * 256; id0 < n; id0 += (long)gridDim.x * 256) {
+        const long id = id0 + threadIdx.x;
+        if (id >= n) return;
+        // (the divisions of 64 bits are the workgroup's, a thread's are of 32)
+        const long tok0 = id0 / w, seq0 = tok0 / L;
+        const unsigned r = (unsigned)(id0 - tok0 * w) + threadIdx.x, t = (unsigned)(tok0 - seq0 * L) + r / w;
         float s = 0.f;
-        if (!lengths || (int)(tok % L) < lengths[tok / L])
+        if (!lengths || (int)(t % (unsigned)L) < lengths[seq0 + t / (unsigned)L]) {
+#pragma unroll 8
             for (int k = 0; k < nblk; ++k) s += part[k * n + id];
-        const long row = id / (2 * N);
-        const int e = (int)(id % (2 * N));
-        (e < N ? db[row * N + e] : dc[row * N + e - N]) = from_f32<T>(s);
+        }
+        const unsigned v = r % w, g = v / (2u * N), e = v % (2u * N);
+        const long row = (tok0 + r / w) * G + g;
+        (e < (unsigned)N ? db[row * N + e] : dc[row * N + e - N]) = from_f32<T>(s);
     }
 }
 
