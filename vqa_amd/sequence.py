@@ -15,7 +15,8 @@ taken between 0 and L.  `state` continues a sequence and `return_state` returns 
 through both.  Everything runs on torch's current stream of the tensors' device; workspaces are torch allocations of the
 call, so captured graphs share nothing.  A backward that is to be captured into a graph needs leaves that no live eager
 graph uses (torch ties a leaf's gradient accumulation to the stream of its first use); the *_step functions are forward
-only.  Errors of use raise VqaHipError (a RuntimeError) before anything is launched.
+only, and the state they update shares no memory with their other arguments.  Errors of use raise VqaHipError (a
+RuntimeError) before anything is launched.
 """
 import ctypes
 from functools import lru_cache
