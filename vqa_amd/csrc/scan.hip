@@ -41,6 +41,7 @@ struct Args {
     void* y; float* last;
     float *keep, *seg_h, *seg_dt;          // h before the tiles; per segment: state, then the true incoming one; sum dt
     void *dx, *ddt, *dgate; float *part_bc, *part_p, *dstate;
+    void *db, *dc; float *da, *dskip, *dbias; int params;      // the join's outputs, its workgroups for the parameters
 };
 
 // The wave's own LDS traffic in program order: the hardware keeps it, this keeps the compiler from moving it.
@@ -770,9 +771,8 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
 
 // part_p's rows summed in a fixed order (16 row lanes x 64 columns) and put in their public places.
 template <int NP>
-__global__ __launch_bounds__(1024) void scan_params(const float* __restrict__ part, int rows, int per, int per_pad, int N,
-                                                    int G, float* __restrict__ da, float* __restrict__ dskip,
-                                                    float* __restrict__ dbias) {
+__device__ __forceinline__ void sum_params(const float* __restrict__ part, int rows, int per, int per_pad, int N, int G,
+                                           float* __restrict__ da, float* __restrict__ dskip, float* __restrict__ dbias) {
     const long chans = (long)G * per_pad, cols = chans * (NP + 2), col = (long)blockIdx.x * 64 + (threadIdx.x & 63);
     const int lr = threadIdx.x >> 6;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -800,14 +800,14 @@ __global__ __launch_bounds__(1024) void scan_params(const float* __restrict__ pa
     } else if (dbias) dbias[c] = t;
 }
 
-// db and dc: the channel blocks' shares in a fixed order; rows past a sequence's length are 0.  Each share is read once;
-// eight in flight a thread and 32-bit divisions: 4 x 2048 x 2048 5.8 us (17 MB), 9.7 with a load at a time and 64 bits
+// db and dc: the channel blocks' shares in a fixed order; rows past a sequence's length are 0.  Each share is read once, eight
+// in flight a thread.  Workgroup `block` of `blocks`.
 template <typename T>
-__global__ __launch_bounds__(256) void scan_shared(const float* __restrict__ part, const int* __restrict__ lengths, int B,
-                                                   int L, int G, int N, int nblk, T* __restrict__ db, T* __restrict__ dc) {
+__device__ __forceinline__ void sum_shared(const float* __restrict__ part, const int* __restrict__ lengths, int B, int L, int G,
+                                           int N, int nblk, T* __restrict__ db, T* __restrict__ dc, int block, int blocks) {
     const long n = (long)B * L * G * 2 * N;
     const int w = G * 2 * N;                               // values a token
-    for (long id0 = (long)blockIdx.x * 256; id0 < n; id0 += (long)gridDim.x * 256) {
+    for (long id0 = (long)block * 1024; id0 < n; id0 += (long)blocks * 1024) {
         const long id = id0 + threadIdx.x;
         if (id >= n) return;
         // (the divisions of 64 bits are the workgroup's, a thread's are of 32)
@@ -822,6 +822,17 @@ __global__ __launch_bounds__(256) void scan_shared(const float* __restrict__ par
         const long row = (tok0 + r / w) * G + g;
         (e < (unsigned)N ? db[row * N + e] : dc[row * N + e - N]) = from_f32<T>(s);
     }
+}
+
+// Both in one launch, the first A.params workgroups for the parameters: each is a few microseconds of waiting for its loads
+// (4 x 2048 x 2048 9.9 us, 5.8 + 5.7 in two launches; 256 x 14 x 2048 7.3, 4.2 + 5.4).
+template <typename T, int NP> __global__ __launch_bounds__(1024) void scan_join(Args A) {
+    const int block = blockIdx.x;
+    if (block < A.params)
+        sum_params<NP>(A.part_p, A.bgroups * A.segs, A.per, A.per_pad, A.N, A.G, A.da, A.dskip, A.dbias);
+    else
+        sum_shared<T>(A.part_bc, A.lengths, A.B, A.L, A.G, A.N, A.bblk, static_cast<T*>(A.db), static_cast<T*>(A.dc),
+                      block - A.params, (int)gridDim.x - A.params);
 }
 
 // One token: a lane takes four states of a channel, LN lanes a channel, 256 / LN channels of one sequence a workgroup.  Bound
@@ -926,7 +937,7 @@ void plan(Args& A, bool bwd) {
 bool bad_shape(int dtype, int B, int L, int D, int N, int G) {
     return !vqa_dtype_ok(dtype) || B < 1 || L < 1 || L > 0x3fffffff || D < 1 || N < 1 || N > 64 || G < 1 || D % G != 0 ||
            (double)B * L > 1e9 || (double)B * L * D > 4e11 || (double)B * D > 1e9 || (double)B * L * G * N > 1e11 ||
-           (double)G * (D / G + 128) * B > 2e9 || (double)G * (D / G + 128) * (np_of(N) + 2) > 2.5e8;
+           (double)G * (D / G + 128) * B > 2e9 || (double)G * (D / G + 128) * (np_of(N) + 2) > 2.4e8;
 }
 // (buffer accesses of up to 16 bytes want their addresses on 4 bytes)
 bool on4(const void* p, long stride, int e) { return ((uintptr_t)p & 3) == 0 && stride * e % 4 == 0; }
@@ -970,8 +981,15 @@ template <typename T, int NS, int CH, int VE, int BCH, int BVE> int launch(bool 
             CHECK_LAUNCH();
             return VQA_OK;
         }
-    if (bwd) scan_bwd<T, BCH, NS, BVE><<<(unsigned)((long)A.bblk * A.G * A.segs * A.bgroups), 64 * BW, 0, st>>>(A);
-    else scan_fwd<T, CH, NS, VE, true><<<waves, 64, 0, st>>>(A);
+    if (!bwd) {
+        scan_fwd<T, CH, NS, VE, true><<<waves, 64, 0, st>>>(A);
+        CHECK_LAUNCH();
+        return VQA_OK;
+    }
+    scan_bwd<T, BCH, NS, BVE><<<(unsigned)((long)A.bblk * A.G * A.segs * A.bgroups), 64 * BW, 0, st>>>(A);
+    CHECK_LAUNCH();
+    const long shared = std::min(((long)A.B * A.L * A.G * 2 * A.N + 1023) / 1024, 16384L);
+    scan_join<T, 4 * NS><<<(unsigned)(A.params + shared), 1024, 0, st>>>(A);
     CHECK_LAUNCH();
     return VQA_OK;
 }
@@ -1046,28 +1064,12 @@ extern "C" int vqa_scan_bwd(void* stream, int dtype, const void* dy, long dy_bat
     A.seg_dt = seg_dt_of(A, ws);
     A.part_p = ws + seg_floats(A);
     A.part_bc = A.part_p + part_p_floats(A);
+    A.params = (int)(((long)G * A.per_pad * (np_of(N) + 2) + 63) / 64);
+    A.da = da; A.db = db; A.dc = dc; A.dskip = dskip; A.dbias = ddt_bias;
     const int e = vqa_elem_bytes(dtype);
     const bool vec = A.per % (16 / e) == 0 && rows_vec(A.x, e) && rows_vec(A.dt, e) && rows_vec(A.gate, e) &&
                      rows_vec(A.dy, e) && on4(dx, D, e) && on4(ddt, D, e) && on4(dgate, D, e);
-    const hipStream_t st = static_cast<hipStream_t>(stream);
-    const int rc = by_type(true, dtype, vec, A, st);
-    if (rc != VQA_OK) return rc;
-    const int rows = A.bgroups * A.segs, np = np_of(N);
-    const unsigned pg = (unsigned)(((long)G * A.per_pad * (np + 2) + 63) / 64);
-    if (np == 8) scan_params<8><<<pg, 1024, 0, st>>>(A.part_p, rows, A.per, A.per_pad, N, G, da, dskip, ddt_bias);
-    else if (np == 16) scan_params<16><<<pg, 1024, 0, st>>>(A.part_p, rows, A.per, A.per_pad, N, G, da, dskip, ddt_bias);
-    else if (np == 32) scan_params<32><<<pg, 1024, 0, st>>>(A.part_p, rows, A.per, A.per_pad, N, G, da, dskip, ddt_bias);
-    else scan_params<64><<<pg, 1024, 0, st>>>(A.part_p, rows, A.per, A.per_pad, N, G, da, dskip, ddt_bias);
-    CHECK_LAUNCH();
-    const unsigned sg = (unsigned)std::min(((long)B * L * G * 2 * N + 255) / 256, 65536L);
-    if (dtype == VQA_F32)
-        scan_shared<float><<<sg, 256, 0, st>>>(A.part_bc, lengths, B, L, G, N, A.bblk, static_cast<float*>(db), static_cast<float*>(dc));
-    else if (dtype == VQA_BF16)
-        scan_shared<bf16><<<sg, 256, 0, st>>>(A.part_bc, lengths, B, L, G, N, A.bblk, static_cast<bf16*>(db), static_cast<bf16*>(dc));
-    else
-        scan_shared<_Float16><<<sg, 256, 0, st>>>(A.part_bc, lengths, B, L, G, N, A.bblk, static_cast<_Float16*>(db), static_cast<_Float16*>(dc));
-    CHECK_LAUNCH();
-    return VQA_OK;
+    return by_type(true, dtype, vec, A, static_cast<hipStream_t>(stream));
 }
 
 namespace {
