@@ -82,3 +82,17 @@ def test_scan_workspaces_hold_what_the_kernels_write():
         if fwd:
             segments = fwd // (4 * B * padded * (states + 1))
             assert fwd == 4 * B * padded * (states + 1) * segments and 1 < segments <= max(1, T // 16)
+
+
+def test_selective_scan_gradients_without_channels():
+    """No channel, so nothing is launched; b and c still have values, and their gradients are 0 (memory is handed out here
+    that held other values before)."""
+    from vqa_amd.sequence import _SelectiveScan
+    for _ in range(4):
+        b, c = (torch.randn(2, 3, 2, 4, requires_grad=True) for _ in range(2))
+        x, a = torch.zeros(2, 3, 0), torch.zeros(0, 4, requires_grad=True)
+        y, _ = _SelectiveScan.apply(x, x, a, b, c, None, None, None, 1, None, None, False)
+        junk = [torch.full((2, 3, 2, 4), float('nan')) for _ in range(4)]
+        del junk
+        db, dc, da = torch.autograd.grad(y, [b, c, a], torch.zeros_like(y))
+        assert not db.any() and not dc.any() and da.shape == (0, 4)

@@ -770,3 +770,15 @@ def test_refusals():
         with pytest.raises(VqaHipError):
             f()
             pytest.fail(f'call {i} was not refused')
+
+
+def test_selective_scan_without_channels():
+    s = S()
+    b, c = (torch.randn(2, 3, 4, device='cuda', requires_grad=True) for _ in range(2))
+    x, a, h = torch.zeros(2, 3, 0, device='cuda'), torch.zeros(0, 4, device='cuda'), torch.zeros(2, 0, 4, device='cuda')
+    y, last = s.selective_scan(x, x, a, b, c, state=h, return_state=True)
+    assert y.shape == (2, 3, 0) and last.shape == (2, 0, 4)
+    junk = [torch.full((2, 3, 1, 4), float('nan'), device='cuda') for _ in range(8)]
+    del junk
+    db, dc = torch.autograd.grad(y, [b, c], torch.zeros_like(y))
+    assert not db.any() and not dc.any()

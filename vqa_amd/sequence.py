@@ -364,7 +364,7 @@ class _SelectiveScan(torch.autograd.Function):
         dskip, dbias = f32(D) if skip is not None else None, f32(D) if dt_bias is not None else None
         dstate = f32(B, D, N) if state is not None else None
         if not dx.numel():
-            for g in (da, dskip, dbias):
+            for g in (da, db, dc, dskip, dbias):           # (without channels, db and dc still have values)
                 if g is not None:
                     g.zero_()
             if dstate is not None:
