@@ -96,3 +96,77 @@ def test_selective_scan_gradients_without_channels():
         del junk
         db, dc, da = torch.autograd.grad(y, [b, c, a], torch.zeros_like(y))
         assert not db.any() and not dc.any() and da.shape == (0, 4)
+
+
+def _calls(x, w, wc, state, a, b, h, b1):
+    """Every entry point, on x [2, 3, 8]."""
+    from vqa_amd import sequence as S
+    return [lambda x=x, w=w: S.layer_norm(x, w), lambda x=x, wc=wc: S.causal_conv(x, wc),
+            lambda x=x, wc=wc: S.causal_conv_step(x[:, 0], state, wc),
+            lambda x=x, a=a: S.selective_scan(x, x, a, b, b), lambda x=x, a=a: S.selective_scan_step(x[:, 0], h, x[:, 0], a, b1, b1)]
+
+
+def _operands():
+    g = torch.Generator().manual_seed(1)
+    return [torch.randn(*s, generator=g) for s in ((2, 3, 8), (8,), (8, 4), (2, 3, 8), (8, 4), (2, 3, 4), (2, 8, 4), (2, 4))]
+
+
+@pytest.mark.parametrize('which', range(8))
+def test_inputs_with_a_tangent_are_refused(which):
+    """A tangent that a call would drop: in each argument, also where nothing requires a gradient."""
+    import torch.autograd.forward_ad as fw
+    from vqa_amd._lib import VqaHipError
+    args = _operands()
+    takers = {0: range(5), 1: (0,), 2: (1, 2), 3: (2,), 4: (3, 4), 5: (3,), 6: (4,), 7: (4,)}[which]
+    with fw.dual_level():
+        args[which] = fw.make_dual(args[which], torch.ones_like(args[which]))
+        for i in takers:
+            with pytest.raises(VqaHipError, match='tangent'):
+                _calls(*args)[i]()
+        with fw._set_fwd_grad_enabled(False):              # (nothing is followed: refused for another reason)
+            for f in _calls(*args):
+                with pytest.raises(VqaHipError, match='GPU'):
+                    f()
+    with fw.dual_level():                                  # (a level alone is no tangent)
+        for f in _calls(*_operands()):
+            with pytest.raises(VqaHipError, match='GPU'):
+                f()
+
+
+def test_gradients_with_a_tangent_are_refused():
+    """... and in the gradient that comes into a backward, as in a forward derivative of a backward pass."""
+    import torch.autograd.forward_ad as fw
+    from vqa_amd import sequence as S
+    from vqa_amd._lib import VqaHipError
+    x = torch.zeros(0, 8, requires_grad=True)              # (no row: nothing is launched)
+    y = S._LayerNorm.apply(x, None, None, 1e-5)
+    assert torch.autograd.grad(y, x, torch.zeros(0, 8), retain_graph=True)[0].shape == (0, 8)
+    with fw.dual_level():
+        with pytest.raises(VqaHipError, match='tangent'):
+            torch.autograd.grad(y, x, fw.make_dual(torch.zeros(0, 8), torch.zeros(0, 8)))
+
+
+@pytest.mark.parametrize('how', ['jit', 'make_fx', 'pre_dispatch', 'fake', 'export'])
+def test_recording_is_refused(how):
+    """A recorded program would hold an allocation that nothing fills; with and without a gradient."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from vqa_amd._lib import VqaHipError
+    args = _operands()
+
+    def one(i, grad):
+        def f(x):
+            with torch.set_grad_enabled(grad):
+                return _calls(x, *args[1:])[i]()
+
+        class Call(torch.nn.Module):
+            def forward(self, x):
+                return f(x)
+        x = args[0].clone().requires_grad_(grad)
+        with pytest.raises(VqaHipError, match='recorded'):
+            {'jit': lambda: torch.jit.trace(f, (x,)), 'make_fx': lambda: make_fx(f)(x),
+             'pre_dispatch': lambda: make_fx(f, pre_dispatch=True)(x),
+             'fake': lambda: make_fx(f, tracing_mode='fake')(x),
+             'export': lambda: torch.export.export(Call(), (x,), strict=False)}[how]()
+    for i in range(5):
+        one(i, False)
+        one(i, True)

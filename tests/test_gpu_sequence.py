@@ -782,3 +782,39 @@ def test_selective_scan_without_channels():
     del junk
     db, dc = torch.autograd.grad(y, [b, c], torch.zeros_like(y))
     assert not db.any() and not dc.any()
+
+
+def test_tangents_and_recorders_are_refused():
+    """Nothing that follows or records operators one by one gets an answer that it could not see."""
+    import torch.autograd.forward_ad as fw
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from vqa_amd._lib import VqaHipError
+    s = S()
+    x, w, wc = (torch.randn(*n, device='cuda') for n in ((2, 4, 8), (8,), (8, 4)))
+    a, b, h, cs = -torch.ones(8, 4, device='cuda'), torch.randn(2, 4, 4, device='cuda'), torch.zeros(2, 8, 4, device='cuda'), \
+        torch.zeros(2, 3, 8, device='cuda')
+    calls = [lambda x: s.layer_norm(x, w), lambda x: s.causal_conv(x, wc), lambda x: s.selective_scan(x, x, a, b, b),
+             lambda x: s.causal_conv_step(x[:, 0], cs, wc), lambda x: s.selective_scan_step(x[:, 0], h, x[:, 0], a, b[:, 0], b[:, 1])]
+    for f in calls:
+        want = f(x)
+        with fw.dual_level():
+            with pytest.raises(VqaHipError, match='tangent'):
+                f(fw.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(VqaHipError, match='recorded'):
+            torch.jit.trace(f, (x,))
+        with pytest.raises(VqaHipError, match='recorded'):
+            make_fx(f)(x)
+        cs.zero_(), h.zero_()
+        with fw.dual_level():
+            assert torch.equal(f(x), want)                 # (no tangent among the inputs)
+        cs.zero_(), h.zero_()
+    for f in calls[:3]:
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (x,), (x,))
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(f)(x[None])
+    z = x.clone().requires_grad_(True)
+    y = s.layer_norm(z)
+    with fw.dual_level():
+        with pytest.raises(VqaHipError, match='tangent'):
+            torch.autograd.grad(y, z, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))

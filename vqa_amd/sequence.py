@@ -15,13 +15,15 @@ taken between 0 and L.  `state` continues a sequence and `return_state` returns 
 through both.  Everything runs on torch's current stream of the tensors' device; workspaces are torch allocations of the
 call, so captured graphs share nothing.  A backward that is to be captured into a graph needs leaves that no live eager
 graph uses (torch ties a leaf's gradient accumulation to the stream of its first use); the *_step functions are forward
-only, and the state they update shares no memory with their other arguments.  Errors of use raise VqaHipError (a
+only, and the state they update shares no memory with their other arguments.  There are no forward-mode derivatives, and
+torch.jit.trace, make_fx and torch.export cannot record these calls.  Errors of use raise VqaHipError (a
 RuntimeError) before anything is launched.
 """
 import ctypes
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -39,6 +41,24 @@ def _elsewhere(x):
 
 def _fail(what):
     raise L.VqaHipError(what)
+
+
+_tracing = torch._C._is_tracing
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+_key_included, _PRE_DISPATCH = torch._C._dispatch_tls_is_dispatch_key_included, torch._C.DispatchKey.PreDispatch
+
+
+def _seen(*tensors):
+    """The kernels run behind torch's back: what follows or records a computation operator by operator (forward-mode
+    derivatives, torch.jit.trace, make_fx and torch.export) would see an empty allocation in place of a result.  Refused,
+    in 0.3 us."""
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                _fail('an input carries a tangent: the sequence operators have no forward-mode derivative')
+    if _tracing() or _key_included(_PRE_DISPATCH) or (
+            _dispatch_modes() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None):
+        _fail('the sequence operators cannot be recorded by torch.jit.trace, make_fx or torch.export')
 
 
 def _first(x, dims, what):
@@ -113,7 +133,11 @@ def _backward(f):
     """The backward of these operators, which has no derivative of its own: asked for one (create_graph) its results are
     marked so.  (once_differentiable alone costs every ordinary backward a few microseconds.)"""
     marked = once_differentiable(f)
-    return staticmethod(lambda ctx, *grads: marked(ctx, *grads) if torch.is_grad_enabled() else f(ctx, *grads))
+
+    def backward(ctx, *grads):
+        _seen(*grads)
+        return marked(ctx, *grads) if torch.is_grad_enabled() else f(ctx, *grads)
+    return staticmethod(backward)
 
 
 # ---------------------------------------------------------------------------------------------------------- layer norm
@@ -171,6 +195,7 @@ def _norm_parts(rows, width):
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis (biased variance), statistics in float32.
     x [..., C] with C <= 8192; weight, bias float32 [C] or None."""
+    _seen(x, weight, bias)
     _first(x, None, '')
     if _elsewhere(x):
         with torch.cuda.device(x.device):
@@ -254,6 +279,7 @@ def causal_conv(x, weight, bias=None, activation='silu', state=None, lengths=Non
     y_t = act(bias + sum_k weight[:, k] x_{t - taps + 1 + k}), act = silu or (activation=None) nothing; weight float32
     [D, taps], bias float32 [D].  state [B, taps - 1, D] (x's type): the rows before the first (None: zeros).  Returns y,
     or with return_state (y, state after each sequence's last token)."""
+    _seen(x, weight, bias, state)
     _first(x, 3, '[B, L, D]')
     if _elsewhere(x):
         with torch.cuda.device(x.device):
@@ -277,6 +303,7 @@ def causal_conv(x, weight, bias=None, activation='silu', state=None, lengths=Non
 def causal_conv_step(x, state, weight, bias=None, activation='silu'):
     """causal_conv for ONE new token per sequence: x [B, D]; state [B, taps - 1, D] (x's type; rows may be strided) is
     shifted in place.  Returns y [B, D].  Forward only."""
+    _seen(x, state, weight, bias)
     _first(x, 2, '[B, D]')
     if _elsewhere(x):
         with torch.cuda.device(x.device):
@@ -417,6 +444,7 @@ def selective_scan(x, dt, a, b, c, skip=None, gate=None, dt_bias=None, softplus=
     dt, gate [B, L, D]; b, c [B, L, N], or [B, L, G, N] where each of G groups of D / G channels has its own; a float32
     [D, N]; skip, dt_bias float32 [D]; state float32 [B, D, N] (None: zeros).  gate, skip, dt_bias may be None.
     Returns y, or with return_state (y, state after each sequence's last token)."""
+    _seen(x, dt, a, b, c, skip, gate, dt_bias, state)
     _first(x, 3, '[B, L, D]')
     if _elsewhere(x):
         with torch.cuda.device(x.device):
@@ -457,6 +485,7 @@ def _ready(x, dt, a, b, c, skip, gate, dt_bias):
 def selective_scan_step(x, state, dt, a, b, c, skip=None, gate=None, dt_bias=None, softplus=True):
     """selective_scan for ONE new token per sequence: x, dt, gate [B, D]; b, c [B, N] or [B, G, N]; state float32
     [B, D, N] is updated in place (its batch axis may be strided).  Returns y [B, D].  Forward only."""
+    _seen(x, state, dt, a, b, c, skip, gate, dt_bias)
     _first(x, 2, '[B, D]')
     if _elsewhere(x):
         with torch.cuda.device(x.device):
