@@ -170,3 +170,15 @@ def test_recording_is_refused(how):
     for i in range(5):
         one(i, False)
         one(i, True)
+
+
+def test_compiled_callers_reach_the_checks():
+    """torch.compile leaves its graph at these calls: on the CPU it ends at the same refusal as without it."""
+    from vqa_amd._lib import VqaHipError
+    args = _operands()
+    for i in range(5):
+        def f(x, i=i):
+            return _calls(x, *args[1:])[i]()
+        torch._dynamo.reset()
+        with pytest.raises(VqaHipError, match='GPU'):
+            torch.compile(f, backend='eager')(args[0])

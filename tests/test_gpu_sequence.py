@@ -818,3 +818,26 @@ def test_tangents_and_recorders_are_refused():
     with fw.dual_level():
         with pytest.raises(VqaHipError, match='tangent'):
             torch.autograd.grad(y, z, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+@pytest.mark.parametrize('backend', ['eager', 'aot_eager'])
+def test_compiled_callers(backend):
+    """torch.compile around a caller: the same bits, values and gradients."""
+    s = S()
+    x, w, wc = (torch.randn(*n, device='cuda') for n in ((2, 4, 8), (8,), (8, 4)))
+    a, b, h, cs = -torch.ones(8, 4, device='cuda'), torch.randn(2, 4, 4, device='cuda'), torch.zeros(2, 8, 4, device='cuda'), \
+        torch.zeros(2, 3, 8, device='cuda')
+    calls = [lambda x: 2 * s.layer_norm(x, w), lambda x: 2 * s.causal_conv(x, wc), lambda x: 2 * s.selective_scan(x, x, a, b, b),
+             lambda x: 2 * s.causal_conv_step(x[:, 0], cs, wc),
+             lambda x: 2 * s.selective_scan_step(x[:, 0], h, x[:, 0], a, b[:, 0], b[:, 1])]
+    for i, f in enumerate(calls):
+        outs = []
+        for g in (f, torch.compile(f, backend=backend)):
+            cs.zero_(), h.zero_()
+            outs.append([g(x), cs.clone(), h.clone()])
+            if i < 3:
+                leaf = x.clone().requires_grad_(True)
+                outs[-1] += torch.autograd.grad(g(leaf), leaf, x)
+        torch._dynamo.reset()
+        for p, q in zip(*outs):
+            assert torch.equal(p, q), i

@@ -43,6 +43,7 @@ def _fail(what):
     raise L.VqaHipError(what)
 
 
+_compiling = torch.compiler.is_dynamo_compiling
 _tracing = torch._C._is_tracing
 _dispatch_modes = torch._C._len_torch_dispatch_stack
 _key_included, _PRE_DISPATCH = torch._C._dispatch_tls_is_dispatch_key_included, torch._C.DispatchKey.PreDispatch
@@ -51,11 +52,13 @@ _key_included, _PRE_DISPATCH = torch._C._dispatch_tls_is_dispatch_key_included, 
 def _seen(*tensors):
     """The kernels run behind torch's back: what follows or records a computation operator by operator (forward-mode
     derivatives, torch.jit.trace, make_fx and torch.export) would see an empty allocation in place of a result.  Refused,
-    in 0.3 us."""
+    in 0.4 us."""
     if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
         for t in tensors:
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 _fail('an input carries a tangent: the sequence operators have no forward-mode derivative')
+    if _compiling():                                       # (torch.compile leaves its graph for a call of the library)
+        return
     if _tracing() or _key_included(_PRE_DISPATCH) or (
             _dispatch_modes() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None):
         _fail('the sequence operators cannot be recorded by torch.jit.trace, make_fx or torch.export')
