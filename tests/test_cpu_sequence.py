@@ -182,3 +182,41 @@ def test_compiled_callers_reach_the_checks():
         torch._dynamo.reset()
         with pytest.raises(VqaHipError, match='GPU'):
             torch.compile(f, backend='eager')(args[0])
+
+
+class _Wrapper(torch.Tensor):
+    """A tensor of another class without memory of its own, as distributed and quantized tensors are."""
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device, strides=inner.stride())
+
+    @classmethod
+    def __torch_dispatch__(cls, f, types, args=(), kwargs=None):
+        raise NotImplementedError(str(f))
+
+
+def test_tensors_without_storage_are_refused():
+    """The address of such a tensor is 0, which the entry points take for an argument that was left out."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from vqa_amd import sequence as S
+    from vqa_amd._lib import VqaHipError
+    x, w, wc, state, a, b, h, b1 = _operands()
+    t = x[:, 0]
+
+    class Kept(torch.Tensor):                              # a class with ordinary memory is taken
+        pass
+    for make in (_Wrapper, FakeTensorMode().from_tensor):
+        for f in (lambda: S.layer_norm(make(x)), lambda: S.layer_norm(x, make(w)), lambda: S.layer_norm(x, None, make(w)),
+                  lambda: S.causal_conv(x, wc, make(w)), lambda: S.causal_conv(x, wc, state=make(state)),
+                  lambda: S.causal_conv(x, wc, lengths=make(torch.ones(2, dtype=torch.int32))),
+                  lambda: S.causal_conv_step(t, state, wc, make(w)),
+                  lambda: S.selective_scan(x, x, a, b, b, make(w)), lambda: S.selective_scan(x, x, a, b, b, gate=make(x)),
+                  lambda: S.selective_scan(x, x, a, b, b, state=make(h)),
+                  lambda: S.selective_scan_step(t, h, t, a, b1, b1, gate=make(t)),
+                  lambda: S.selective_scan_step(t, h, t, a, b1, b1, dt_bias=make(w))):
+            with pytest.raises(VqaHipError, match='no storage'):
+                f()
+    with pytest.raises(VqaHipError, match='list was given'):
+        S.causal_conv(x, wc, lengths=[1, 2])
+    with pytest.raises(VqaHipError, match='GPU'):
+        S.layer_norm(x.as_subclass(Kept), torch.nn.Parameter(w))

@@ -47,21 +47,34 @@ _compiling = torch.compiler.is_dynamo_compiling
 _tracing = torch._C._is_tracing
 _dispatch_modes = torch._C._len_torch_dispatch_stack
 _key_included, _PRE_DISPATCH = torch._C._dispatch_tls_is_dispatch_key_included, torch._C.DispatchKey.PreDispatch
+_PLAIN = {torch.Tensor, torch.nn.Parameter, type(None)}
+
+
+def _stored(args):
+    """Every argument of another class is a tensor with memory of its own: a wrapper's address is 0, which an entry point
+    takes for an argument that was left out."""
+    for t in args:
+        if type(t) not in _PLAIN:
+            if not isinstance(t, torch.Tensor):
+                _fail(f'a {type(t).__name__} was given where a tensor is wanted')
+            if t.layout is not torch.strided or t.numel() and not t.data_ptr():
+                _fail(f'a {type(t).__name__} has no storage that a kernel could read')
 
 
 def _seen(*tensors):
     """The kernels run behind torch's back: what follows or records a computation operator by operator (forward-mode
     derivatives, torch.jit.trace, make_fx and torch.export) would see an empty allocation in place of a result.  Refused,
-    in 0.4 us."""
+    in 0.5 us with the look at the arguments' types."""
+    if not _compiling():                                   # (torch.compile leaves its graph for a call of the library)
+        if _tracing() or _key_included(_PRE_DISPATCH) or (
+                _dispatch_modes() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None):
+            _fail('the sequence operators cannot be recorded by torch.jit.trace, make_fx or torch.export')
+        if not _PLAIN.issuperset(map(type, tensors)):
+            _stored(tensors)
     if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
         for t in tensors:
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 _fail('an input carries a tangent: the sequence operators have no forward-mode derivative')
-    if _compiling():                                       # (torch.compile leaves its graph for a call of the library)
-        return
-    if _tracing() or _key_included(_PRE_DISPATCH) or (
-            _dispatch_modes() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None):
-        _fail('the sequence operators cannot be recorded by torch.jit.trace, make_fx or torch.export')
 
 
 def _first(x, dims, what):
@@ -282,7 +295,7 @@ def causal_conv(x, weight, bias=None, activation='silu', state=None, lengths=Non
     y_t = act(bias + sum_k weight[:, k] x_{t - taps + 1 + k}), act = silu or (activation=None) nothing; weight float32
     [D, taps], bias float32 [D].  state [B, taps - 1, D] (x's type): the rows before the first (None: zeros).  Returns y,
     or with return_state (y, state after each sequence's last token)."""
-    _seen(x, weight, bias, state)
+    _seen(x, weight, bias, state, lengths)
     _first(x, 3, '[B, L, D]')
     if _elsewhere(x):
         with torch.cuda.device(x.device):
@@ -447,7 +460,7 @@ def selective_scan(x, dt, a, b, c, skip=None, gate=None, dt_bias=None, softplus=
     dt, gate [B, L, D]; b, c [B, L, N], or [B, L, G, N] where each of G groups of D / G channels has its own; a float32
     [D, N]; skip, dt_bias float32 [D]; state float32 [B, D, N] (None: zeros).  gate, skip, dt_bias may be None.
     Returns y, or with return_state (y, state after each sequence's last token)."""
-    _seen(x, dt, a, b, c, skip, gate, dt_bias, state)
+    _seen(x, dt, a, b, c, skip, gate, dt_bias, state, lengths)
     _first(x, 3, '[B, L, D]')
     if _elsewhere(x):
         with torch.cuda.device(x.device):
