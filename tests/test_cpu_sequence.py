@@ -220,3 +220,17 @@ def test_tensors_without_storage_are_refused():
         S.causal_conv(x, wc, lengths=[1, 2])
     with pytest.raises(VqaHipError, match='GPU'):
         S.layer_norm(x.as_subclass(Kept), torch.nn.Parameter(w))
+
+
+def test_eps_is_a_number():
+    """A tensor would go to the library as its address; other numbers are converted."""
+    import numpy as np
+    from vqa_amd import sequence as S
+    from vqa_amd._lib import VqaHipError
+    x = torch.zeros(2, 8)
+    for eps in (torch.tensor(1e-5), torch.tensor(1e-5, requires_grad=True), None, 'small', [1e-5]):
+        with pytest.raises(VqaHipError, match='eps'):
+            S.layer_norm(x, eps=eps)
+    for eps in (1e-5, 0, 1, np.float32(1e-5), np.float64(1e-5)):
+        with pytest.raises(VqaHipError, match='GPU'):
+            S.layer_norm(x, eps=eps)

@@ -841,3 +841,20 @@ def test_compiled_callers(backend):
         torch._dynamo.reset()
         for p, q in zip(*outs):
             assert torch.equal(p, q), i
+
+
+def test_scalar_arguments():
+    """Numbers and truth values of numpy as Python's; an eps in a tensor is refused, not taken by its address."""
+    import numpy as np
+    from vqa_amd._lib import VqaHipError
+    s = S()
+    x, w = torch.randn(3, 8, device='cuda'), torch.ones(8, device='cuda')
+    with pytest.raises(VqaHipError, match='eps'):
+        s.layer_norm(x, w, eps=torch.tensor(1e-5, device='cuda'))
+    assert torch.equal(s.layer_norm(x, w, eps=np.float32(0.5)), s.layer_norm(x, w, eps=0.5))
+    assert torch.equal(s.layer_norm(x, w, eps=1), s.layer_norm(x, w, eps=1.0))
+    a, b = -torch.ones(8, 4, device='cuda'), torch.randn(3, 4, device='cuda')
+    for flag in (True, False):
+        h = [torch.ones(3, 8, 4, device='cuda') for _ in range(2)]
+        assert torch.equal(s.selective_scan_step(x, h[0], x, a, b, b, softplus=np.bool_(flag)),
+                           s.selective_scan_step(x, h[1], x, a, b, b, softplus=flag)) and torch.equal(*h)

@@ -106,6 +106,16 @@ def _param(name, p, shape, x):
     return p if p.is_contiguous() else p.contiguous()
 
 
+def _number(name, v):
+    """A Python number (a tensor would go to the library as its address)"""
+    if isinstance(v, torch.Tensor):
+        _fail(f'{name} is a tensor: a number is wanted')
+    try:
+        return float(v)
+    except (TypeError, ValueError):
+        _fail(f'{name} is {v!r}: a number is wanted')
+
+
 def _lengths(lengths, x):
     if lengths is None:
         return None
@@ -212,6 +222,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis (biased variance), statistics in float32.
     x [..., C] with C <= 8192; weight, bias float32 [C] or None."""
     _seen(x, weight, bias)
+    if type(eps) is not float:
+        eps = _number('eps', eps)
     _first(x, None, '')
     if _elsewhere(x):
         with torch.cuda.device(x.device):
@@ -521,7 +533,7 @@ def selective_scan_step(x, state, dt, a, b, c, skip=None, gate=None, dt_bias=Non
     s0, s1, s2 = state.stride()
     if (s2 != 1 and N > 1) or (s1 != N and D > 1) or (B > 1 and s0 < D * N):
         _fail(f'state has strides {state.stride()}: it is updated in place, so [D, N] must be contiguous and apart')
-    sg = 0 if gate is None else gate.stride(0)
+    sg, softplus = 0 if gate is None else gate.stride(0), int(softplus)
     if L._PROFILE is None and L._REC is None:
         # (one token's latency is host time: pointers are taken here, 3 us less than by L.call)
         L.check(L.lib().vqa_scan_token(
