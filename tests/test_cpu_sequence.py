@@ -234,3 +234,21 @@ def test_eps_is_a_number():
     for eps in (1e-5, 0, 1, np.float32(1e-5), np.float64(1e-5)):
         with pytest.raises(VqaHipError, match='GPU'):
             S.layer_norm(x, eps=eps)
+
+
+def test_axes_past_31_bits_are_refused():
+    """A size of 2^32 + 1 would reach the library as 1: the first row would be answered, the others left as allocated."""
+    import types
+
+    from vqa_amd import sequence as S
+    from vqa_amd._lib import VqaHipError
+
+    def rows(*shape):                                      # what _first looks at of a GPU tensor
+        t = torch.zeros(1, dtype=torch.bfloat16).expand(shape)
+        return types.SimpleNamespace(is_cuda=True, dtype=t.dtype, shape=t.shape, dim=t.dim, numel=t.numel)
+    far = (1 << 32) + 1
+    for shape in ((far, 1, 1), (1, far, 1), (1, 1, far), (1 << 31, 2, 1)):
+        with pytest.raises(VqaHipError, match='below 2'):
+            S._first(rows(*shape), 3, '[B, L, D]')
+    for shape in ((1 << 20, 1 << 12, 1), (far, 0, 1), ((1 << 31) - 1, 2, 1)):
+        S._first(rows(*shape), 3, '[B, L, D]')

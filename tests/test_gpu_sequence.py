@@ -858,3 +858,22 @@ def test_scalar_arguments():
         h = [torch.ones(3, 8, 4, device='cuda') for _ in range(2)]
         assert torch.equal(s.selective_scan_step(x, h[0], x, a, b, b, softplus=np.bool_(flag)),
                            s.selective_scan_step(x, h[1], x, a, b, b, softplus=flag)) and torch.equal(*h)
+
+
+def test_axes_past_31_bits_are_refused():
+    """(one value, expanded: no memory behind it)"""
+    from vqa_amd._lib import VqaHipError
+    s, far = S(), (1 << 32) + 1
+    one = torch.ones(1, device='cuda', dtype=torch.bfloat16)
+    w, a = torch.ones(1, 4, device='cuda'), -torch.ones(1, 1, device='cuda')
+    for shape in ((far, 1, 1), (1, far, 1)):
+        x = one.expand(shape)
+        for f in (lambda: s.layer_norm(x), lambda: s.causal_conv(x, w), lambda: s.selective_scan(x, x, a, x, x)):
+            with pytest.raises(VqaHipError):
+                f()
+    x = one.expand(far, 1)
+    h = torch.zeros(1, 1, 1, device='cuda')
+    for f in (lambda: s.causal_conv_step(x, one.expand(far, 3, 1), w),
+              lambda: s.selective_scan_step(x, h.expand(far, 1, 1), x, a, x, x)):
+        with pytest.raises(VqaHipError):
+            f()

@@ -85,6 +85,8 @@ def _first(x, dims, what):
         _fail(f'x must be float32, bfloat16 or float16, not {x.dtype}')
     if dims is not None and x.dim() != dims:
         _fail(f'x has shape {tuple(x.shape)}: {what} is wanted')
+    if x.numel() > 0x7fffffff and max(x.shape) > 0x7fffffff:    # (the entry points take sizes of 32 bits)
+        _fail(f'x has shape {tuple(x.shape)}: axes below 2^31 are wanted')
 
 
 def _rows(name, t, shape, x):
