@@ -252,3 +252,18 @@ def test_axes_past_31_bits_are_refused():
             S._first(rows(*shape), 3, '[B, L, D]')
     for shape in ((1 << 20, 1 << 12, 1), (far, 0, 1), ((1 << 31) - 1, 2, 1)):
         S._first(rows(*shape), 3, '[B, L, D]')
+
+
+def test_scan_refuses_grids_past_32_bits():
+    """64 threads for every 64, 32 or 16 channels of a group (up to 16, 32, 64 states), within every other limit."""
+    from vqa_amd import _lib as L
+    lib = L.lib()
+    sizes = (ctypes.c_long * 3)()
+    ok = lambda B, D, N, G=1: lib.vqa_scan_ws_bytes(1, B, 1, D, N, G, ctypes.addressof(sizes)) == 0      # noqa: E731
+    for B, D, N, G in ((7751937, 129, 64, 1), (6896551, 145, 64, 1), (3448275, 290, 64, 2), (6211180, 161, 33, 1)):
+        assert B * G * -(-(D // G) // 16) * 64 >= 1 << 32 and not ok(B, D, N, G)
+        rc = lib.vqa_scan_fwd(None, 1, P, D, D, P, D, D, None, 0, 0, P, P, G * N, G * N, P, G * N, G * N, None, None, 1, None,
+                              None, B, 1, D, N, G, P, None, None, P)
+        assert rc == 1
+    # the same widths with fewer rows, and more channels a wave, stay
+    assert ok(7000000, 129, 64) and ok(7751937, 129, 32) and ok(7751937, 129, 16)

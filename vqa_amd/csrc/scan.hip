@@ -937,7 +937,9 @@ void plan(Args& A, bool bwd) {
 bool bad_shape(int dtype, int B, int L, int D, int N, int G) {
     return !vqa_dtype_ok(dtype) || B < 1 || L < 1 || L > 0x3fffffff || D < 1 || N < 1 || N > 64 || G < 1 || D % G != 0 ||
            (double)B * L > 1e9 || (double)B * L * D > 4e11 || (double)B * D > 1e9 || (double)B * L * G * N > 1e11 ||
-           (double)G * (D / G + 128) * B > 2e9 || (double)G * (D / G + 128) * (np_of(N) + 2) > 2.4e8;
+           (double)G * (D / G + 128) * B > 2e9 || (double)G * (D / G + 128) * (np_of(N) + 2) > 2.4e8 ||
+           // (a grid has fewer than 2^32 threads: the forward's waves.  Segments and half waves are for few of them.)
+           (double)B * G * ((D / G + fwd_channels(N) - 1) / fwd_channels(N)) * 64 > 4.29e9;
 }
 // (buffer accesses of up to 16 bytes want their addresses on 4 bytes)
 bool on4(const void* p, long stride, int e) { return ((uintptr_t)p & 3) == 0 && stride * e % 4 == 0; }
