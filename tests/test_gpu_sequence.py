@@ -877,3 +877,99 @@ def test_axes_past_31_bits_are_refused():
               lambda: s.selective_scan_step(x, h.expand(far, 1, 1), x, a, x, x)):
         with pytest.raises(VqaHipError):
             f()
+
+
+def _same_kind(name, got, want, roundings):
+    """Where the definition (64 bits) gives a number, got is near it; where it gives an infinity, that infinity; where it
+    gives no number, anything."""
+    g, w = got.detach().double().cpu(), want.detach()
+    inf = w.isinf()
+    assert torch.equal(g[inf], w[inf]), f'{name}: {g[inf][:8]} for {w[inf][:8]}'
+    ok = w.isfinite()
+    assert ok.any(), name
+    R.close(name, got.detach().cpu()[ok], w[ok], roundings)
+
+
+@pytest.mark.parametrize('B,T,D,N,dtype', [(2, 19, 40, 5, 'f32'), (2, 19, 40, 16, 'f32'), (1, 21, 65, 12, 'bf16'),
+                                           (2, 300, 40, 20, 'f32'), (1, 300, 72, 33, 'f32'), (1, 2100, 8, 3, 'f32'),
+                                           (70, 17, 2048, 12, 'bf16')])
+def test_selective_scan_of_infinite_values(B, T, D, N, dtype):
+    """One infinite x, where the states' terms have one sign: an infinite state and y from there on, and nothing else; one
+    infinite dy: an infinite gradient of what came before."""
+    leaves, dy, dlast = _scan_case(B, T, D, N, 1, dtype, seed=40)
+    at, ch, late = (0, T // 3, 3), 5, 2 * T // 3
+    for k in ('x', 'b', 'c', 'skip', 'state'):
+        for v in leaves[k]:
+            v.data.abs_().clamp_(min=0.125)
+    dy, dlast = dy.abs() + 0.125, dlast.abs() + 0.125
+    n = 128 + 8 * T
+    if B == 70:                                            # (many sequences: the first is compared)
+        leaves = {k: (g, c[:1] if k in ('x', 'dt', 'b', 'c', 'gate', 'state') else c) for k, (g, c) in leaves.items()}
+    G, C = ({k: v[i].detach().clone() for k, v in leaves.items()} for i in (0, 1))
+
+    def go(x_inf, dy_inf):
+        outs = []
+        for v, f, d, dl in ((G, None, dy.cuda(), dlast.cuda()), (C, R.scan, dy.double(), dlast.double())):
+            v = {k: t.clone() for k, t in v.items()}
+            d = d[:len(v['x'])].clone()
+            if x_inf:
+                v['x'][at] = float('inf')
+            if dy_inf:
+                d[0, late, ch] = float('inf')
+                v['gate'][0, late, ch] = 1.0
+            v = {k: t.requires_grad_(True) for k, t in v.items()}
+            if f is None:
+                y, last = S().selective_scan(*(v[k] for k in SCAN[:8]), state=v['state'], return_state=True)
+            else:
+                y, last = R.scan(*(v[k] for k in SCAN[:8]), True, v['state'], None)
+            outs.append((y, last, _grads([y, last], [d, dl[:len(d)]], v)))
+        return outs
+    (y, last, _), (yr, lastr, _) = go(True, False)
+    assert yr[0, T // 3:, 3].isinf().all() and lastr[0, 3].isinf().all()
+    _same_kind('y', y[:len(yr)], yr, n)
+    _same_kind('last', last[:len(yr)], lastr, n)
+    (_, _, g), (_, _, w) = go(False, True)
+    assert w['x'][0, :late + 1, ch].isinf().all()
+    for k in ('x', 'dt', 'gate', 'state', 'b'):
+        _same_kind('d' + k, g[k][:len(yr)], w[k], 2 * n + (D if k == 'b' else 0))
+    if B < 70:
+        _same_kind('da', g['a'], w['a'], 2 * n + B * T)
+
+
+@pytest.mark.parametrize('N', [3, 5, 12, 16, 33])
+def test_selective_scan_step_of_infinite_values(N):
+    g = _gen(41)
+    B, D = 2, 24
+    rn = lambda *s: torch.rand(*s, generator=g) + 0.125                          # noqa: E731
+    x, dt, gate, b, c, h, a, skip = rn(B, D), rn(B, D), rn(B, D), rn(B, 1, N), rn(B, 1, N), rn(B, D, N), -rn(D, N), rn(D)
+    x[1, 7], dt[0, 2] = float('inf'), float('inf')
+    state = h.cuda()
+    y = S().selective_scan_step(*(v.cuda() if v is not state else v for v in (x, state, dt, a, b, c, skip, gate)))
+    yr, hr = R.scan(*(v.double()[:, None] for v in (x, dt)), a.double(), b.double()[:, None], c.double()[:, None],
+                    skip.double(), gate.double()[:, None], None, True, h.double(), None)
+    assert yr[1, 0, 7].isinf() and yr[0, 0, 2].isinf()
+    _same_kind('y', y, yr[:, 0], 256)
+    _same_kind('state', state, hr, 256)
+
+
+@pytest.mark.parametrize('N', [16, 5])
+def test_selective_scan_infinite_states_pass_segments(N):
+    """A segment's decay underflows to 0 where no token's does: an infinite state, and an infinite adjoint, pass it as they
+    pass its tokens, and finite ones are forgotten."""
+    g = _gen(42)
+    B, T, D = 1, 400, 24
+    rn = lambda *s: torch.rand(*s, generator=g) + 0.125                          # noqa: E731
+    v = dict(x=rn(B, T, D), dt=rn(B, T, D), a=-10 * rn(D, N), b=rn(B, T, 1, N), c=rn(B, T, 1, N), skip=rn(D))
+    v['x'][0, 20, 3] = float('inf')
+    dy = rn(B, T, D)
+    dy[0, 390, 5] = float('inf')
+    dev = {k: t.cuda().requires_grad_(True) for k, t in v.items()}
+    ref = {k: t.double().requires_grad_(True) for k, t in v.items()}
+    y, last = S().selective_scan(*(dev[k] for k in SCAN[:6]), return_state=True)
+    yr, lastr = R.scan(*(ref[k] for k in SCAN[:6]), None, None, True, None, None)
+    assert yr[0, 20:, 3].isinf().all() and lastr[0, 3].isinf().all()
+    _same_kind('y', y, yr, 128 + 8 * T)
+    _same_kind('last', last, lastr, 128 + 8 * T)
+    (dx,), (dxr,) = torch.autograd.grad(y, [dev['x']], dy.cuda()), torch.autograd.grad(yr, [ref['x']], dy.double())
+    assert dxr[0, :391, 5].isinf().all()
+    _same_kind('dx', dx, dxr, 2 * (128 + 8 * T))

@@ -176,7 +176,8 @@ template <typename T, int CH, int NS, int VE> struct Wave {
 #pragma unroll
             for (int j = 0; j < NS; ++j) {
                 const int n = r * NS + j;
-                a2[i][j] = channel(i) < cend && n < A.N ? A.a[(long)channel(i) * A.N + n] * LOG2E : 0.f;
+                // (past the end not 0, whose product with an infinite dt is NaN: any finite dt gives a finite decay)
+                a2[i][j] = channel(i) < cend && n < A.N ? A.a[(long)channel(i) * A.N + n] * LOG2E : -1.2e-38f;
             }
     }
     // a state in its public layout [B][D][N].  (The lane is hidden from the compiler: these run once a sequence, and their
@@ -293,8 +294,37 @@ __device__ __forceinline__ void stage_steps(const W& w, const R (&d)[NV], const 
     }
 }
 
+// The states past N, where N is not NP (PAD), have b = c = 0, and 0 times an infinite dt x or dcore would make NaN of a sum over
+// states that is infinite.  In the forward a tile with such a value takes a second form of its loop, in which those states are
+// kept at 0 (16383 tokens x 2048, N = 12, bf16: 147 us, 159 with a select or a mask per state in every tile, 145 without).  The
+// backward has no registers for two forms and keeps their h and G at 0 by masks of bits (4 x 2048 x 2048, N = 12: 253 us; two
+// forms 270, selects, whose conditions take scalar registers, 258, without 240).
+struct Masked { static constexpr bool on = true; };
+struct Plain { static constexpr bool on = false; };
+__device__ __forceinline__ bool any_infinite(float largest) { return __any(largest == __builtin_inff()); }
+template <bool PAD, int NS> struct Real {
+    unsigned bits[NS];
+    __device__ __forceinline__ Real(int r, int N) {
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+            bits[j] = r * NS + j < N ? ~0u : 0u;
+            if (PAD) asm volatile("" : "+v"(bits[j]));     // (a value, not a condition to the compiler)
+        }
+    }
+    __device__ __forceinline__ float operator()(int j, float v) const {
+        return PAD ? __uint_as_float(__float_as_uint(v) & bits[j]) : v;
+    }
+    // (what the first pass over a segment, which has no masks, left in their places of the workspace is not taken over)
+    template <int CH> __device__ __forceinline__ void clear(float (&h)[CH][NS]) const {
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+#pragma unroll
+            for (int j = 0; j < NS; ++j) h[i][j] = (*this)(j, h[i][j]);
+    }
+};
+
 // FULL: the forward.  Otherwise the first pass over a segment: its end state from 0, and sum dt.
-template <typename T, int CH, int NS, int VE, bool FULL>
+template <typename T, int CH, int NS, int VE, bool FULL, bool PAD = false>
 __global__ __launch_bounds__(64) void scan_fwd(Args A) {
     typedef Wave<T, CH, NS, VE> W;
     constexpr int NBC = TT * W::NP / 64;
@@ -316,8 +346,10 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
         for (int j = 0; j < NS; ++j) h[i][j] = 0.f;
     }
     if (FULL) {
-        if (A.segs > 1) w.load_own(A.seg_h + at_seg * W::NP, h);
-        else w.load_public(A.state, b, A.D, A.N, h);
+        if (A.segs > 1) {
+            w.load_own(A.seg_h + at_seg * W::NP, h);
+            Real<PAD, NS>(w.r, A.N).clear(h);
+        } else w.load_public(A.state, b, A.D, A.N, h);
     }
     Raw<T, VE> x[W::NV], d[W::NV], z[W::NV], xn[W::NV], dn[W::NV];
     unsigned bn[NBC], cn[NBC];
@@ -335,14 +367,16 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
 #pragma unroll
         for (int k = 0; k < W::NV; ++k) { x[k] = xn[k]; d[k] = dn[k]; }
         lds_order();                                       // (the last tile's reads are done)
-        float step[W::NV][VE];
+        float step[W::NV][VE], largest = 0.f;
         stage_steps<false>(w, d, s_bias, A.softplus, t0, live, step, step);
 #pragma unroll
         for (int k = 0; k < W::NV; ++k)
 #pragma unroll
             for (int v = 0; v < VE; ++v) {
+                const float dtx = step[k][v] * x[k].get(v);
+                if (PAD) largest = fmaxf(largest, fabsf(dtx));
                 s_dt[w.tat(k) + v] = step[k][v];
-                s_dtx[w.tat(k) + v] = step[k][v] * x[k].get(v);
+                s_dtx[w.tat(k) + v] = dtx;
             }
 #pragma unroll
         for (int k = 0; k < NBC; ++k) {
@@ -353,25 +387,30 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
         if (FULL) w.fetch(A.gate, b, t0, live, z, A.gate.p != nullptr);
         fetch(t0 + TT);                                    // (past the end: zeros)
         if (FULL) w.store_own(A.keep + (((long)b * kept_tiles(A.L) + t0 / TT - 1) * chans + w.p0) * W::NP, h, A.keep && t0 > 0);
+        auto tokens = [&](auto form) {
 #pragma unroll
-        for (int t = 0; t < TT; ++t) {
-            float dt[CH], dtx[CH], bv[NS], cv[NS], y[CH];
-            lds_read<CH>(s_dt + t * W::WC + w.cl * CH, dt);
-            lds_read<CH>(s_dtx + t * W::WC + w.cl * CH, dtx);
-            lds_read<NS>(s_b + t * W::NP + w.r * NS, bv);
-            if (FULL) lds_read<NS>(s_c + t * W::NP + w.r * NS, cv);
+            for (int t = 0; t < TT; ++t) {
+                float dt[CH], dtx[CH], bv[NS], cv[NS], y[CH];
+                lds_read<CH>(s_dt + t * W::WC + w.cl * CH, dt);
+                lds_read<CH>(s_dtx + t * W::WC + w.cl * CH, dtx);
+                lds_read<NS>(s_b + t * W::NP + w.r * NS, bv);
+                if (FULL) lds_read<NS>(s_c + t * W::NP + w.r * NS, cv);
 #pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                y[i] = 0.f;
-                if (!FULL) sum_dt[i] += dt[i];
+                for (int i = 0; i < CH; ++i) {
+                    y[i] = 0.f;
+                    if (!FULL) sum_dt[i] += dt[i];
 #pragma unroll
-                for (int j = 0; j < NS; ++j) {
-                    h[i][j] = __builtin_amdgcn_exp2f(dt[i] * a2[i][j]) * h[i][j] + dtx[i] * bv[j];
-                    if (FULL) y[i] += h[i][j] * cv[j];
+                    for (int j = 0; j < NS; ++j) {
+                        // (which product is rounded before the sum is not left to the compiler: its choice differed between forms)
+                        h[i][j] = __builtin_fmaf(dtx[i], bv[j], __builtin_amdgcn_exp2f(dt[i] * a2[i][j]) * h[i][j]);
+                        if (decltype(form)::on && w.r * NS + j >= A.N) h[i][j] = 0.f;
+                        if (FULL) y[i] += h[i][j] * cv[j];
+                    }
                 }
+                if (FULL) s_y[t * W::WC + w.cl * CH + own_channel<CH>(w.r)] = sum_states<CH>(y);
             }
-            if (FULL) s_y[t * W::WC + w.cl * CH + own_channel<CH>(w.r)] = sum_states<CH>(y);
-        }
+        };
+        if (PAD && any_infinite(largest)) tokens(Masked()); else tokens(Plain());
         if (FULL) {
             lds_order();
 #pragma unroll
@@ -438,7 +477,9 @@ template <int NP, bool REV> __global__ __launch_bounds__(256) void scan_chain(Ar
             const int s = REV ? A.segs - 1 - s0 - u : s0 + u;
             if (s >= 0 && s < A.segs) {
                 q[s * chans * NP] = h;
-                h = __builtin_amdgcn_exp2f(d[u] * a) * h + e[u];
+                // (a segment's whole decay may underflow where no token's does, and an infinite state stays infinite)
+                const float decay = __builtin_amdgcn_exp2f(d[u] * a);
+                h = __builtin_fmaf(decay < 0x1p-149f ? 0x1p-149f : decay, h, e[u]);
             }
         }
     }
@@ -532,7 +573,7 @@ __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
 // The BW waves of a workgroup take neighbouring channels, share b and c in LDS and join their sums db, dc over channels
 // there: part_bc[workgroup of the group][B][L][G][2][N].  A workgroup takes the sequences of its batch group one after the
 // other, so that its sums over tokens leave once: part_p[(batch group, segment)]{da [channel][NP], dskip, ddt_bias}.
-template <typename T, int CH, int NS, int VE>
+template <typename T, int CH, int NS, int VE, bool PAD>
 __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A) {
     typedef Wave<T, CH, NS, VE> W;
     constexpr int TILE = TT * W::WC, SH = TT * W::NP, NBC = (2 * SH + 64 * BW - 1) / (64 * BW), 
@@ -548,6 +589,7 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
     const float *s_b = s_bc, *s_c = s_bc + SH;
     const long chans = (long)A.G * A.per_pad;
     const int ts = seg * A.seg_len, tend = min(A.L, ts + A.seg_len);
+    const Real<PAD, NS> real(w.r, A.N);
     float a2[CH][NS], g[CH][NS], da[CH][NS], sum_skip[W::NV][VE], sum_bias[W::NV][VE];
     w.lane_a(A, a2);
     w.stage_param(A.dt_bias, s_bias);
@@ -600,8 +642,10 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
             w.put(A.ddt, b, A.L, A.D, t0, tend, x);
             if (A.gate.p) w.put(A.dgate, b, A.L, A.D, t0, tend, x);
         }
-        if (A.segs > 1) w.load_own(A.seg_h + (((long)b * A.segs + seg) * chans + w.p0) * W::NP, g);
-        else w.load_public(A.dlast, b, A.D, A.N, g);
+        if (A.segs > 1) {
+            w.load_own(A.seg_h + (((long)b * A.segs + seg) * chans + w.p0) * W::NP, g);
+            real.clear(g);
+        } else w.load_public(A.dlast, b, A.D, A.N, g);
         for (int t0 = t_last; t0 >= ts; t0 -= TT) {
             Raw<T, VE> x[W::NV], d[W::NV], z[W::NV], gy[W::NV];
             float hist[TT][CH][NS], h[CH][NS], kd[KD > 0 ? KD : 1][CH][NS];
@@ -660,7 +704,7 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
                             hist[t][i][j] = h[i][j];
                             const float decay = __builtin_amdgcn_exp2f(dt[i] * a2[i][j]);
                             if (t >= TT - KD) kd[t >= TT - KD ? t - (TT - KD) : 0][i][j] = decay;
-                            h[i][j] = decay * h[i][j] + dtx[i] * bv[j];
+                            h[i][j] = real(j, __builtin_fmaf(decay, h[i][j], dtx[i] * bv[j]));
                             y[i] += h[i][j] * cv[j];
                             sc[j] += h[i][j] * dc[i];
                         }
@@ -668,7 +712,7 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
                     s_y[t * W::WC + w.cl * CH + own_channel<CH>(w.r)] = sum_states<CH>(y);
                     put_sums<NS>(s_dc + t * W::NP, sc, w.r, w.cl);
                 }
-                lds_order();                               // (and the decays are formed again, not held in registers)
+                lds_order();                           // (and the decays are formed again, not held in registers)
 #pragma unroll
                 for (int t = TT - 1; t >= 0; --t) {
                     float dt[CH], dtx[CH], dc[CH], bv[NS], cv[NS], gb[CH], ta[CH], sb[NS];
@@ -684,7 +728,7 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
                         gb[i] = ta[i] = 0.f;
 #pragma unroll
                         for (int j = 0; j < NS; ++j) {
-                            const float G = g[i][j] + dc[i] * cv[j];
+                            const float G = real(j, g[i][j] + dc[i] * cv[j]);
                             gb[i] += G * bv[j];
                             sb[j] += G * dtx[i];
                             g[i][j] = G * (t >= TT - KD ? kd[t >= TT - KD ? t - (TT - KD) : 0][i][j]
@@ -880,7 +924,8 @@ __global__ __launch_bounds__(256) void scan_token(Rows x, float* __restrict__ st
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        h.v[k] = exp_f(step * av.v[k]) * h.v[k] + step * xv * bv.get(k);
+        // (a state past N stays 0 whatever dt and x are)
+        h.v[k] = n0 + k < N ? exp_f(step * av.v[k]) * h.v[k] + step * xv * bv.get(k) : 0.f;
         s += h.v[k] * cv.get(k);
     }
     if constexpr (VEC) {
@@ -967,7 +1012,7 @@ template <int NP, bool REV> int chain(const Args& A, hipStream_t st) {
 }
 
 // CH, VE: the forward's channels a lane and elements a load; BCH, BVE: the backward's
-template <typename T, int NS, int CH, int VE, int BCH, int BVE> int launch(bool bwd, const Args& A, hipStream_t st) {
+template <typename T, int NS, int CH, int VE, int BCH, int BVE, bool PAD> int launch(bool bwd, const Args& A, hipStream_t st) {
     const unsigned waves = (unsigned)((long)A.fblk * A.G * A.segs * A.B);
     int rc = VQA_OK;
     if (A.segs > 1) {
@@ -979,28 +1024,31 @@ template <typename T, int NS, int CH, int VE, int BCH, int BVE> int launch(bool 
     }
     if constexpr (CH > 1)
         if (!bwd && A.narrow) {
-            scan_fwd<T, CH / 2, NS, (VE < CH ? VE : CH), true><<<waves, 64, 0, st>>>(A);
+            scan_fwd<T, CH / 2, NS, (VE < CH ? VE : CH), true, PAD><<<waves, 64, 0, st>>>(A);
             CHECK_LAUNCH();
             return VQA_OK;
         }
     if (!bwd) {
-        scan_fwd<T, CH, NS, VE, true><<<waves, 64, 0, st>>>(A);
+        scan_fwd<T, CH, NS, VE, true, PAD><<<waves, 64, 0, st>>>(A);
         CHECK_LAUNCH();
         return VQA_OK;
     }
-    scan_bwd<T, BCH, NS, BVE><<<(unsigned)((long)A.bblk * A.G * A.segs * A.bgroups), 64 * BW, 0, st>>>(A);
+    scan_bwd<T, BCH, NS, BVE, PAD><<<(unsigned)((long)A.bblk * A.G * A.segs * A.bgroups), 64 * BW, 0, st>>>(A);
     CHECK_LAUNCH();
     const long shared = std::min(((long)A.B * A.L * A.G * 2 * A.N + 1023) / 1024, 16384L);
     scan_join<T, 4 * NS><<<(unsigned)(A.params + shared), 1024, 0, st>>>(A);
     CHECK_LAUNCH();
     return VQA_OK;
 }
-template <typename T> int by_states(bool bwd, bool vec, const Args& A, hipStream_t st) {
+template <typename T, bool PAD> int by_states(bool bwd, bool vec, const Args& A, hipStream_t st) {
     constexpr int V = 16 / sizeof(T);
-    if (A.N <= 8) return vec ? launch<T, 2, 4, V, 2, 4>(bwd, A, st) : launch<T, 2, 4, 1, 2, 1>(bwd, A, st);
-    if (A.N <= 16) return vec ? launch<T, 4, 4, V, 2, 4>(bwd, A, st) : launch<T, 4, 4, 1, 2, 1>(bwd, A, st);
-    if (A.N <= 32) return vec ? launch<T, 8, 2, 4, 1, 2>(bwd, A, st) : launch<T, 8, 2, 1, 1, 1>(bwd, A, st);
-    return vec ? launch<T, 16, 1, 2, 1, 2>(bwd, A, st) : launch<T, 16, 1, 1, 1, 1>(bwd, A, st);
+    if (A.N <= 8) return vec ? launch<T, 2, 4, V, 2, 4, PAD>(bwd, A, st) : launch<T, 2, 4, 1, 2, 1, PAD>(bwd, A, st);
+    if (A.N <= 16) return vec ? launch<T, 4, 4, V, 2, 4, PAD>(bwd, A, st) : launch<T, 4, 4, 1, 2, 1, PAD>(bwd, A, st);
+    if (A.N <= 32) return vec ? launch<T, 8, 2, 4, 1, 2, PAD>(bwd, A, st) : launch<T, 8, 2, 1, 1, 1, PAD>(bwd, A, st);
+    return vec ? launch<T, 16, 1, 2, 1, 2, PAD>(bwd, A, st) : launch<T, 16, 1, 1, 1, 1, PAD>(bwd, A, st);
+}
+template <typename T> int by_states(bool bwd, bool vec, const Args& A, hipStream_t st) {
+    return A.N == np_of(A.N) ? by_states<T, false>(bwd, vec, A, st) : by_states<T, true>(bwd, vec, A, st);
 }
 int by_type(bool bwd, int dtype, bool vec, const Args& A, hipStream_t st) {
     if (dtype == VQA_F32) return by_states<float>(bwd, vec, A, st);
