@@ -973,3 +973,35 @@ def test_selective_scan_infinite_states_pass_segments(N):
     (dx,), (dxr,) = torch.autograd.grad(y, [dev['x']], dy.cuda()), torch.autograd.grad(yr, [ref['x']], dy.double())
     assert dxr[0, :391, 5].isinf().all()
     _same_kind('dx', dx, dxr, 2 * (128 + 8 * T))
+
+
+@pytest.mark.parametrize('N,D', [(16, 64), (5, 33)])
+def test_absent_parameters_meet_no_infinity(N, D):
+    """skip=None is no skip, not a skip of 0: an infinite x or dy keeps its sign."""
+    g = _gen(43)
+    B, T = 2, 19
+    rn = lambda *s: torch.rand(*s, generator=g) + 0.125                          # noqa: E731
+    v = dict(x=rn(B, T, D), dt=rn(B, T, D), a=-rn(D, N), b=rn(B, T, 1, N), c=rn(B, T, 1, N), gate=rn(B, T, D))
+    dy = rn(B, T, D)
+    dy[1, 9, 2], v['gate'][1, 9, 2] = float('inf'), 1.0
+    dev = {k: t.cuda().requires_grad_(True) for k, t in v.items()}
+    ref = {k: t.double().requires_grad_(True) for k, t in v.items()}
+    y, _ = S().selective_scan(*(dev[k] for k in SCAN[:5]), gate=dev['gate'], return_state=True)
+    yr, _ = R.scan(*(ref[k] for k in SCAN[:5]), None, ref['gate'], None, True, None, None)
+    got, want = _grads([y], [dy.cuda()], dev), _grads([yr], [dy.double()], ref)
+    assert want['x'][1, :10, 2].isinf().all()
+    for k in ('x', 'gate', 'dt'):
+        _same_kind('d' + k, got[k], want[k], 2 * (128 + 8 * T))
+    x = v['x'].clone()
+    x[0, 4, 1] = float('inf')
+    args = {k: v[k] for k in SCAN[1:5]}
+    y = S().selective_scan(x.cuda(), *(t.cuda() for t in args.values()), gate=v['gate'].cuda())
+    yr, _ = R.scan(x.double(), *(t.double() for t in args.values()), None, v['gate'].double(), None, True, None, None)
+    assert yr[0, 4:, 1].isinf().all()
+    _same_kind('y', y, yr, 128 + 8 * T)
+    h = torch.zeros(B, D, N, device='cuda')
+    one = S().selective_scan_step(x[:, 4].cuda(), h, *(args[k][:, 4].cuda() if k != 'a' else args[k].cuda() for k in args),
+                                  gate=v['gate'][:, 4].cuda())
+    yr, _ = R.scan(*(t.double()[:, 4:5] if k != 'a' else t.double() for k, t in dict(x=x, **args).items()), None,
+                   v['gate'].double()[:, 4:5], None, True, None, None)
+    _same_kind('step', one, yr[:, 0], 256)

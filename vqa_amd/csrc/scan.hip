@@ -28,13 +28,14 @@ constexpr int TT = 8;                      // tokens of a tile
 constexpr int BW = 4;                      // waves of a backward workgroup
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
+enum { SOFTPLUS = 1, SKIP = 2 };
 struct Rows { const void* p; long batch, row; };          // [B][L][...], element strides; the last axis is contiguous
 
 struct Args {
     Rows x, dt, gate, b, c, dy;
     const float *a, *skip, *dt_bias, *state, *dlast;
     const int* lengths;
-    int softplus, B, L, D, N, G;
+    int flags, B, L, D, N, G;              // flags: SOFTPLUS, SKIP (there is one)
     int per, per_pad, fblk, bblk;          // channels of a group, padded; forward waves, backward workgroups across it
     int segs, seg_len, bgroups;            // segments, tokens of one, batch groups of the backward
     bool narrow;                           // forward waves of half the channels
@@ -368,7 +369,7 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
         for (int k = 0; k < W::NV; ++k) { x[k] = xn[k]; d[k] = dn[k]; }
         lds_order();                                       // (the last tile's reads are done)
         float step[W::NV][VE], largest = 0.f;
-        stage_steps<false>(w, d, s_bias, A.softplus, t0, live, step, step);
+        stage_steps<false>(w, d, s_bias, A.flags & SOFTPLUS, t0, live, step, step);
 #pragma unroll
         for (int k = 0; k < W::NV; ++k)
 #pragma unroll
@@ -416,7 +417,13 @@ __global__ __launch_bounds__(64) void scan_fwd(Args A) {
 #pragma unroll
             for (int k = 0; k < W::NV; ++k)
 #pragma unroll
-                for (int v = 0; v < VE; ++v) step[k][v] = s_y[w.tat(k) + v] + s_skip[w.tcol(k) + v] * x[k].get(v);
+                for (int v = 0; v < VE; ++v) step[k][v] = s_y[w.tat(k) + v];
+            if (A.flags & SKIP) {                          // (not 0 times an x that may be infinite)
+#pragma unroll
+                for (int k = 0; k < W::NV; ++k)
+#pragma unroll
+                    for (int v = 0; v < VE; ++v) step[k][v] += s_skip[w.tcol(k) + v] * x[k].get(v);
+            }
             if (A.gate.p) {
 #pragma unroll
                 for (int k = 0; k < W::NV; ++k)
@@ -519,7 +526,7 @@ __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
     for (; te > ts && t0 >= ts; t0 -= TT) {
         lds_order();
         float step[W::NV][VE], dcore[W::NV][VE];
-        stage_steps<false>(w, dn, s_bias, A.softplus, t0, te, step, step);
+        stage_steps<false>(w, dn, s_bias, A.flags & SOFTPLUS, t0, te, step, step);
 #pragma unroll
         for (int k = 0; k < W::NV; ++k)
 #pragma unroll
@@ -590,6 +597,10 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
     const long chans = (long)A.G * A.per_pad;
     const int ts = seg * A.seg_len, tend = min(A.L, ts + A.seg_len);
     const Real<PAD, NS> real(w.r, A.N);
+    // (without a skip its 0 meets no infinity.  A mask in a vector register: a branch here costs 3 % of the kernel)
+    unsigned skip_bits = A.flags & SKIP ? ~0u : 0u;
+    asm volatile("" : "+v"(skip_bits));
+    auto if_skip = [&](float v) { return __uint_as_float(__float_as_uint(v) & skip_bits); };
     float a2[CH][NS], g[CH][NS], da[CH][NS], sum_skip[W::NV][VE], sum_bias[W::NV][VE];
     w.lane_a(A, a2);
     w.stage_param(A.dt_bias, s_bias);
@@ -660,7 +671,7 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
                 if (k * 64 * BW + (int)threadIdx.x < 2 * SH) s_bc[k * 64 * BW + threadIdx.x] = shared_value<T>(sn[k]);
             float step[W::NV][VE], slope[W::NV][VE], sig[W::NV][VE], dcore[W::NV][VE];
             if (live) {
-                stage_steps<true>(w, d, s_bias, A.softplus, t0, te, step, slope);
+                stage_steps<true>(w, d, s_bias, A.flags & SOFTPLUS, t0, te, step, slope);
 #pragma unroll
                 for (int k = 0; k < W::NV; ++k)
 #pragma unroll
@@ -751,7 +762,7 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
                     for (int k = 0; k < W::NV; ++k) {
 #pragma unroll
                         for (int v = 0; v < VE; ++v) {
-                            const float core = s_y[w.tat(k) + v] + s_skip[w.tcol(k) + v] * x[k].get(v);
+                            const float core = s_y[w.tat(k) + v] + s_skip[w.tcol(k) + v] * if_skip(x[k].get(v));
                             z[k].set(v, gy[k].get(v) * core * sig[k][v] * (1.f + z[k].get(v) * (1.f - sig[k][v])));
                         }
                         if (t0 + TT > te && t0 + w.trow(k) >= te) z[k].zero();
@@ -769,7 +780,7 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
                         sum_bias[k][v] += dr;
                         sum_skip[k][v] += past ? 0.f : dcore[k][v] * xv;
                         d[k].set(v, dr);
-                        x[k].set(v, step[k][v] * gb + s_skip[w.tcol(k) + v] * dcore[k][v]);
+                        x[k].set(v, __builtin_fmaf(step[k][v], gb, s_skip[w.tcol(k) + v] * if_skip(dcore[k][v])));
                     }
                     if (past) x[k].zero();
                 }
@@ -938,7 +949,7 @@ __global__ __launch_bounds__(256) void scan_token(Rows x, float* __restrict__ st
 #pragma unroll
     for (int o = 1; o < LN; o <<= 1) s += __shfl_xor(s, o);
     if (part == 0) {
-        s += sk * xv;
+        if (skip) s += sk * xv;
         if (gate.p) s *= silu_f(zv);
         y[(long)bi * D + d] = from_f32<T>(s);
     }
@@ -1080,7 +1091,8 @@ extern "C" int vqa_scan_fwd(void* stream, int dtype, const void* x, long x_batch
     Args A = {};
     A.x = {x, x_batch, x_row}; A.dt = {dt, dt_batch, dt_row}; A.gate = {gate, gate_batch, gate_row};
     A.b = {b, b_batch, b_row}; A.c = {c, c_batch, c_row};
-    A.a = a; A.skip = skip; A.dt_bias = dt_bias; A.state = state; A.lengths = lengths; A.softplus = softplus;
+    A.a = a; A.skip = skip; A.dt_bias = dt_bias; A.state = state; A.lengths = lengths;
+    A.flags = (softplus ? SOFTPLUS : 0) | (skip ? SKIP : 0);
     A.B = B; A.L = L; A.D = D; A.N = N; A.G = G; A.y = y; A.last = last; A.keep = keep;
     plan(A, false);
     if ((A.segs > 1 && !ws) || !aligned16(ws) || !aligned16(keep) || far_rows(A)) return VQA_ERR_ARG;
@@ -1105,7 +1117,8 @@ extern "C" int vqa_scan_bwd(void* stream, int dtype, const void* dy, long dy_bat
     A.dy = {dy, dy_batch, dy_row};
     A.x = {x, x_batch, x_row}; A.dt = {dt, dt_batch, dt_row}; A.gate = {gate, gate_batch, gate_row};
     A.b = {b, b_batch, b_row}; A.c = {c, c_batch, c_row};
-    A.a = a; A.skip = skip; A.dt_bias = dt_bias; A.dlast = dlast; A.state = state; A.lengths = lengths; A.softplus = softplus;
+    A.a = a; A.skip = skip; A.dt_bias = dt_bias; A.dlast = dlast; A.state = state; A.lengths = lengths;
+    A.flags = (softplus ? SOFTPLUS : 0) | (skip ? SKIP : 0);
     A.B = B; A.L = L; A.D = D; A.N = N; A.G = G; A.keep = const_cast<float*>(keep);
     A.dx = dx; A.ddt = ddt; A.dgate = dgate; A.dstate = dstate;
     if (far_rows(A)) return VQA_ERR_ARG;
