@@ -1005,3 +1005,14 @@ def test_absent_parameters_meet_no_infinity(N, D):
     yr, _ = R.scan(*(t.double()[:, 4:5] if k != 'a' else t.double() for k, t in dict(x=x, **args).items()), None,
                    v['gate'].double()[:, 4:5], None, True, None, None)
     _same_kind('step', one, yr[:, 0], 256)
+
+
+@pytest.mark.parametrize('B,T,D,N,lengths', [(2, 5, 24, 16, None), (3, 19, 40, 5, [19, 3, 0]), (2, 300, 24, 16, [300, 17]),
+                                             (1, 8, 16, 8, None)])
+def test_selective_scan_of_states_that_are_forgotten(B, T, D, N, lengths):
+    """a = -inf: every token forgets such a state; tokens that a sequence does not have leave it.  Against a = -1e30, where
+    64 bits have the products that 0 times -inf has not."""
+    lens = torch.tensor(lengths, dtype=torch.int32) if lengths is not None else None
+    leaves, dy, dlast = _scan_case(B, T, D, N, 1, 'f32', seed=44)
+    leaves['a'][0].data[:, 1], leaves['a'][1].data[:, 1] = float('-inf'), -1e30
+    _scan_check(leaves, dy, dlast, lens)

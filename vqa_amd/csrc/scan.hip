@@ -65,6 +65,13 @@ __device__ __forceinline__ float softplus_f(float v, float e) {
     return fmaxf(v, 0.f) + 2.f * s * p;
 }
 
+// a log2 e.  -inf, a state that every token forgets, is the lowest number instead: tokens past a sequence's end have dt = 0 and
+// leave it as it is
+__device__ __forceinline__ float exponent_of(float a) {
+    const float e = a * LOG2E;
+    return e < -__FLT_MAX__ ? -__FLT_MAX__ : e;
+}
+
 // v[i]: lane (row r, channel lane) holds its row's share of channel i.  -> the sum over the 4 rows of channel own(r).
 template <int CH> __device__ __forceinline__ int own_channel(int r) { return CH == 4 ? r : CH == 2 ? r >> 1 : 0; }
 __device__ __forceinline__ float swap_add32(float a, float b) {        // lanes 0-31: a over both halves, 32-63: b
@@ -178,7 +185,7 @@ template <typename T, int CH, int NS, int VE> struct Wave {
             for (int j = 0; j < NS; ++j) {
                 const int n = r * NS + j;
                 // (past the end not 0, whose product with an infinite dt is NaN: any finite dt gives a finite decay)
-                a2[i][j] = channel(i) < cend && n < A.N ? A.a[(long)channel(i) * A.N + n] * LOG2E : -1.2e-38f;
+                a2[i][j] = channel(i) < cend && n < A.N ? exponent_of(A.a[(long)channel(i) * A.N + n]) : -1.2e-38f;
             }
     }
     // a state in its public layout [B][D][N].  (The lane is hidden from the compiler: these run once a sequence, and their
@@ -466,7 +473,7 @@ template <int NP, bool REV> __global__ __launch_bounds__(256) void scan_chain(Ar
     const int g = p / A.per_pad, off = p % A.per_pad, c = g * A.per + off;
     if (off >= A.per || n >= A.N) return;
     const float* start = REV ? A.dlast : A.state;
-    const float a = A.a[(long)c * A.N + n] * LOG2E;
+    const float a = exponent_of(A.a[(long)c * A.N + n]);
     float h = start ? start[((long)b * A.D + c) * A.N + n] : 0.f;
     const long first = (long)b * A.segs * chans + p;
     float* q = A.seg_h + first * NP + n;
