@@ -1016,3 +1016,22 @@ def test_selective_scan_of_states_that_are_forgotten(B, T, D, N, lengths):
     leaves, dy, dlast = _scan_case(B, T, D, N, 1, 'f32', seed=44)
     leaves['a'][0].data[:, 1], leaves['a'][1].data[:, 1] = float('-inf'), -1e30
     _scan_check(leaves, dy, dlast, lens)
+
+
+@pytest.mark.parametrize('width,dtype', [(3, 'f32'), (47, 'f32'), (300, 'bf16'), (512, 'f16'), (1051, 'bf16'), (1600, 'f32'),
+                                         (2048, 'bf16'), (5000, 'f16'), (8191, 'bf16')])
+def test_layer_norm_of_infinite_gradients(width, dtype):
+    """One infinite dy, in the first and in the last column: dx by the formula in 64 bits, and no other row touched."""
+    g = _gen(45)
+    x = torch.randn(5, width, generator=g).to(DT[dtype])
+    w = torch.rand(width, generator=g) + 0.5
+    dy = torch.randn(5, width, generator=g).to(DT[dtype])
+    dy[1, -1] = dy[3, 0] = float('inf')
+    leaf = x.cuda().requires_grad_(True)
+    dx, = torch.autograd.grad(S().layer_norm(leaf, w.cuda()), leaf, dy.cuda())
+    xd, gd = x.double(), dy.double() * w.double()
+    rstd = 1 / torch.sqrt(xd.var(-1, unbiased=False, keepdim=True) + 1e-5)
+    xh = (xd - xd.mean(-1, keepdim=True)) * rstd
+    want = rstd * (gd - gd.mean(-1, keepdim=True) - xh * (gd * xh).mean(-1, keepdim=True))
+    assert want[1].isinf().any() or want[3].isinf().any()
+    _same_kind('dx', dx, want, 1024)

@@ -124,8 +124,9 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_bwd(const T* __res
     Raw<T, 1> xt, gt, xnt, gnt;
     float mu = 0.f, rs = 0.f, mun = 0.f, rsn = 0.f;
     // The next row is in flight while this one is worked on.  The loads are straight-line code - a lane past the end loads
-    // the last columns again, which meet weights of 0, and past the last row that row - because behind a branch that may
-    // skip them the compiler waits for the new loads where it needs the old ones.
+    // the last columns again, whose dy it takes as 0, and past the last row that row - because behind a branch that may
+    // skip them the compiler waits for the new loads where it needs the old ones.  (A weight of 0 alone does not do: 0
+    // times an infinite dy would make NaN of a row whose sums are infinite.)
     auto fetch = [&](long at) {
         at = min(at, rows - 1);
 #pragma unroll
@@ -145,8 +146,16 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void ln_bwd(const T* __res
     fetch(row);
     for (; row < rows; row += step) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) { xr[i] = xn[i]; gr[i] = gn[i]; }
-        if (TAIL) { xt = xnt; gt = gnt; }
+        for (int i = 0; i < NV; ++i) {
+            xr[i] = xn[i];
+            gr[i] = gn[i];
+            if ((i * TEAM + lane) * V >= main) gr[i].zero();
+        }
+        if (TAIL) {
+            xt = xnt;
+            gt = gnt;
+            if (!tail) gt.zero();
+        }
         mu = mun;
         rs = rsn;
         fetch(row + step);
