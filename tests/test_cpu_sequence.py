@@ -267,3 +267,15 @@ def test_scan_refuses_grids_past_32_bits():
         assert rc == 1
     # the same widths with fewer rows, and more channels a wave, stay
     assert ok(7000000, 129, 64) and ok(7751937, 129, 32) and ok(7751937, 129, 16)
+
+
+def test_scan_workspaces_of_narrow_groups():
+    """Groups that fill less than a quarter of a workgroup's channels are held as they are."""
+    from vqa_amd import _lib as L
+    sizes = (ctypes.c_long * 3)()
+    for B, T, D, N, G, states in ((64, 4096, 64, 16, 4, 16), (4, 2048, 2048, 16, 2048, 16), (2, 100, 30, 5, 10, 8), (3, 65, 24, 33, 8, 64)):
+        assert L.lib().vqa_scan_ws_bytes(1, B, T, D, N, G, ctypes.addressof(sizes)) == 0
+        fwd, keep, bwd = sizes
+        assert keep == 4 * B * (-(-T // 8) - 1) * D * states
+        assert fwd % 16 == 0 and keep % 16 == 0 and bwd % 4 == 0
+        assert bwd < 2 * (fwd + 4 * B * T * G * 2 * N) + 4 * 2048 * D * (states + 2)

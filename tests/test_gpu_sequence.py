@@ -1035,3 +1035,13 @@ def test_layer_norm_of_infinite_gradients(width, dtype):
     want = rstd * (gd - gd.mean(-1, keepdim=True) - xh * (gd * xh).mean(-1, keepdim=True))
     assert want[1].isinf().any() or want[3].isinf().any()
     _same_kind('dx', dx, want, 1024)
+
+
+@pytest.mark.parametrize('B,T,D,N,G,dtype,lengths', [
+    (2, 100, 64, 16, 4, 'f32', [100, 41]), (2, 20, 30, 5, 10, 'bf16', None), (1, 200, 12, 12, 12, 'f32', [199]),
+    (3, 64, 24, 33, 8, 'f32', None), (2, 50, 40, 8, 8, 'f16', [50, 3]), (300, 9, 62, 16, 2, 'f32', None)])
+def test_selective_scan_narrow_groups(B, T, D, N, G, dtype, lengths):
+    """Groups of a few channels, whose states lie close together in the workspaces; whole and in segments."""
+    lens = torch.tensor(lengths, dtype=torch.int32) if lengths is not None else None
+    leaves, dy, dlast = _scan_case(B, T, D, N, G, dtype, seed=46)
+    _scan_check(leaves, dy, dlast, lens)

@@ -17,7 +17,7 @@
 // With few rows the tokens are cut into segments: a first pass finds each segment's own end state and total decay (the
 // product of decays is exp(a sum dt)), a small one chains them, and the full pass starts every segment from its true
 // state.  The backward does the same from the other end.  For the backward the forward keeps h before every tile but the first.
-// States in workspaces lie as [..][channel, a group's padded to per_pad][NP], NP = 8, 16, 32 or 64 >= N.
+// States in workspaces lie as [..][channel, per_pad of them a group][NP], NP = 8, 16, 32 or 64 >= N.
 #include <algorithm>
 #include "seq.h"
 
@@ -976,7 +976,11 @@ void plan(Args& A, bool bwd) {
     A.per = A.D / A.G;
     A.fblk = (A.per + fwd_channels(A.N) - 1) / fwd_channels(A.N);
     A.bblk = (A.per + bwd_channels(A.N) - 1) / bwd_channels(A.N);
+    // Workspaces hold a group's channels as whole backward workgroups take them, which costs little with one group.  Narrow
+    // groups, of which there may be many, are held as they are (64 x 4096 tokens, 64 channels in 4 groups: the kept states
+    // would take 1.07 GB in place of 134 MB).
     A.per_pad = A.bblk * bwd_channels(A.N);
+    if (A.G > 1 && 4 * A.per < A.per_pad) A.per_pad = A.per;
     const long waves = (long)A.B * A.G * A.fblk;
     long s = 1;
     if (waves < (bwd ? 640 : 400)) {
@@ -1015,11 +1019,13 @@ bool far_rows(const Args& A) {
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Workspaces, in floats: the segments' states and sums of dt (none without segments), the backward's partial sums
+// (each a multiple of 16 bytes)
+long whole(long floats) { return (floats + 3) / 4 * 4; }
 long seg_floats(const Args& A) {
-    return A.segs > 1 ? (long)A.B * A.segs * A.G * A.per_pad * (np_of(A.N) + 1) : 0;
+    return A.segs > 1 ? whole((long)A.B * A.segs * A.G * A.per_pad * (np_of(A.N) + 1)) : 0;
 }
 float* seg_dt_of(const Args& A, float* ws) { return ws + (long)A.B * A.segs * A.G * A.per_pad * np_of(A.N); }
-long part_p_floats(const Args& A) { return (long)A.bgroups * A.segs * A.G * A.per_pad * (np_of(A.N) + 2); }
+long part_p_floats(const Args& A) { return whole((long)A.bgroups * A.segs * A.G * A.per_pad * (np_of(A.N) + 2)); }
 long part_bc_floats(const Args& A) { return (long)A.bblk * A.B * A.L * A.G * 2 * A.N; }
 
 template <int NP, bool REV> int chain(const Args& A, hipStream_t st) {
