@@ -279,3 +279,39 @@ def test_scan_workspaces_of_narrow_groups():
         assert keep == 4 * B * (-(-T // 8) - 1) * D * states
         assert fwd % 16 == 0 and keep % 16 == 0 and bwd % 4 == 0
         assert bwd < 2 * (fwd + 4 * B * T * G * 2 * N) + 4 * 2048 * D * (states + 2)
+
+
+def _scan_plan(B, T, D, N, G, backward):
+    """What the scan's launches write, counted again: (padded states, channels a group takes in a workspace, segments, tokens
+    of one, channel blocks and batch groups of the backward)."""
+    per, states = D // G, 8 if N <= 8 else 16 if N <= 16 else 32 if N <= 32 else 64
+    wave, block = {8: 64, 16: 64, 32: 32, 64: 16}[states], 128 if N <= 16 else 64
+    waves, blocks = B * G * -(-per // wave), -(-per // block)
+    held = per if G > 1 and 4 * per < blocks * block else blocks * block
+    cut = max(min(4096 // waves, T // 64), min(1024 // waves, T // 16), 1) if waves < (640 if backward else 400) else 1
+    tokens = -(-(-(-T // cut)) // 8) * 8
+    segments = -(-T // tokens)
+    return states, held, segments, tokens, blocks, max(1, min(B, 1024 // (G * blocks * segments)))
+
+
+@pytest.mark.parametrize('B,T,D,N,G', [
+    (1, 1, 1, 1, 1), (256, 14, 2048, 16, 1), (1, 16383, 2048, 16, 1), (3, 577, 600, 16, 2), (4, 2048, 2048, 16, 1),
+    (2, 100, 64, 64, 4), (7, 700, 33, 20, 1), (16, 512, 2048, 16, 1), (500, 64, 64, 16, 1), (639, 33, 30, 8, 1),
+    (400, 40, 16, 33, 1), (64, 4096, 64, 16, 4), (4, 333, 30, 5, 10), (2, 100, 31, 64, 31), (640, 200, 64, 12, 1)])
+def test_scan_workspace_sizes(B, T, D, N, G):
+    """Exactly what the kernels write: the segments' states and sums of dt, h before every tile but the first, and the
+    backward's shares of db / dc by channel block and of the parameters' gradients by (batch group, segment)."""
+    from vqa_amd import _lib as L
+    sizes = (ctypes.c_long * 3)()
+    assert L.lib().vqa_scan_ws_bytes(1, B, T, D, N, G, ctypes.addressof(sizes)) == 0
+    whole = lambda floats: -(-floats // 4) * 16                                 # noqa: E731
+    ends = []
+    for backward in (False, True):
+        states, held, segments, tokens, blocks, groups = _scan_plan(B, T, D, N, G, backward)
+        assert tokens % 8 == 0 and (segments - 1) * tokens < T <= segments * tokens
+        ends.append(whole(B * segments * G * held * (states + 1)) if segments > 1 else 0)
+    assert sizes[0] == ends[0]
+    assert sizes[1] == 4 * B * (-(-T // 8) - 1) * G * held * states
+    assert sizes[2] == ends[1] + whole(groups * segments * G * held * (states + 2)) + 4 * blocks * B * T * G * 2 * N
+    if (B, T) in ((500, 64), (400, 40)):                   # (between the two thresholds: only the backward is cut)
+        assert sizes[0] == 0 and ends[1] > 0
