@@ -238,14 +238,14 @@ def test_eps_is_a_number():
 
 def test_axes_past_31_bits_are_refused():
     """A size of 2^32 + 1 would reach the library as 1: the first row would be answered, the others left as allocated."""
-    import types
-
     from vqa_amd import sequence as S
     from vqa_amd._lib import VqaHipError
 
-    def rows(*shape):                                      # what _first looks at of a GPU tensor
-        t = torch.zeros(1, dtype=torch.bfloat16).expand(shape)
-        return types.SimpleNamespace(is_cuda=True, dtype=t.dtype, shape=t.shape, dim=t.dim, numel=t.numel)
+    class Said(torch.Tensor):                              # a CPU tensor that says it is on the GPU
+        is_cuda = True
+
+    def rows(*shape):
+        return torch.zeros(1, dtype=torch.bfloat16).expand(shape).as_subclass(Said)
     far = (1 << 32) + 1
     for shape in ((far, 1, 1), (1, far, 1), (1, 1, far), (1 << 31, 2, 1)):
         with pytest.raises(VqaHipError, match='below 2'):

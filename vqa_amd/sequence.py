@@ -23,6 +23,7 @@ import ctypes
 from functools import lru_cache
 
 import torch
+import torch.fx._symbolic_trace as _fx
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
@@ -33,24 +34,38 @@ _ROW_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 _F32 = torch.float32
 
 
+_device, _grad_enabled, _tracing = torch._C._cuda_getDevice, torch.is_grad_enabled, torch._C._is_tracing
+
+
 def _elsewhere(x):
     """Whether x's device is not the current one (the kernels go to the current device's stream; autograd makes a
     backward's device the current one by itself)."""
-    return torch._C._cuda_getDevice() != x.get_device()
+    return _device() != x.get_device()
 
 
 def _fail(what):
     raise L.VqaHipError(what)
 
 
-_compiling = torch.compiler.is_dynamo_compiling
-_tracing = torch._C._is_tracing
-_dispatch_modes = torch._C._len_torch_dispatch_stack
-_key_included, _PRE_DISPATCH = torch._C._dispatch_tls_is_dispatch_key_included, torch._C.DispatchKey.PreDispatch
+def _followed(*tensors):
+    """The kernels run behind torch's back: what follows or records a computation operator by operator (forward-mode
+    derivatives, torch.jit.trace, make_fx and torch.export) would see an empty allocation in place of a result.  Refused -
+    called only where one of them is at work (a call looks for that and at its arguments' types in 0.3 us).  torch.compile
+    leaves its graph for a call of the library."""
+    if not torch.compiler.is_dynamo_compiling() and (
+            _tracing() or torch._C._dispatch_tls_is_dispatch_key_included(torch._C.DispatchKey.PreDispatch)
+            or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None):
+        _fail('the sequence operators cannot be recorded by torch.jit.trace, make_fx or torch.export')
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                _fail('an input carries a tangent: the sequence operators have no forward-mode derivative')
+
+
 _PLAIN = {torch.Tensor, torch.nn.Parameter, type(None)}
 
 
-def _stored(args):
+def _stored(*args):
     """Every argument of another class is a tensor with memory of its own: a wrapper's address is 0, which an entry point
     takes for an argument that was left out."""
     for t in args:
@@ -61,31 +76,20 @@ def _stored(args):
                 _fail(f'a {type(t).__name__} has no storage that a kernel could read')
 
 
-def _seen(*tensors):
-    """The kernels run behind torch's back: what follows or records a computation operator by operator (forward-mode
-    derivatives, torch.jit.trace, make_fx and torch.export) would see an empty allocation in place of a result.  Refused,
-    in 0.5 us with the look at the arguments' types."""
-    if not _compiling():                                   # (torch.compile leaves its graph for a call of the library)
-        if _tracing() or _key_included(_PRE_DISPATCH) or (
-                _dispatch_modes() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None):
-            _fail('the sequence operators cannot be recorded by torch.jit.trace, make_fx or torch.export')
-        if not _PLAIN.issuperset(map(type, tensors)):
-            _stored(tensors)
-    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
-        for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                _fail('an input carries a tangent: the sequence operators have no forward-mode derivative')
-
-
-def _first(x, dims, what):
-    """The tensor that sets the type and the device: rows on the GPU, of a row type, with this many axes (None: any)."""
+def _first(x, dims, what, *others):
+    """The tensor that sets the type and the device: rows on the GPU, of a row type, with this many axes (None: any).
+    others: the call's other tensors, or None."""
+    if forward_ad._current_level >= 0 or _fx._is_fx_tracing_flag or _tracing():
+        _followed(x, *others)
+    if type(x) not in _PLAIN or not _PLAIN.issuperset(map(type, others)):
+        _stored(x, *others)
     if not x.is_cuda:
         _fail('x must be on the GPU (there is no CPU fallback)')
     if x.dtype not in _ROW_TYPES:
         _fail(f'x must be float32, bfloat16 or float16, not {x.dtype}')
     if dims is not None and x.dim() != dims:
         _fail(f'x has shape {tuple(x.shape)}: {what} is wanted')
-    if x.numel() > 0x7fffffff and max(x.shape) > 0x7fffffff:    # (the entry points take sizes of 32 bits)
+    if x.numel() > 0x7fffffff and max(x.shape) > 0x7fffffff:   # (the entry points take sizes of 32 bits)
         _fail(f'x has shape {tuple(x.shape)}: axes below 2^31 are wanted')
 
 
@@ -145,7 +149,7 @@ def _touched(state):
 
 
 def _tracked(*tensors):
-    if torch.is_grad_enabled():
+    if _grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
@@ -153,8 +157,10 @@ def _tracked(*tensors):
 
 
 def _no_tracking(what, *tensors):
-    if _tracked(*tensors):
-        _fail(f'{what} has no gradient: call it under torch.no_grad()')
+    if _grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                _fail(f'{what} has no gradient: call it under torch.no_grad()')
 
 
 def _backward(f):
@@ -163,8 +169,9 @@ def _backward(f):
     marked = once_differentiable(f)
 
     def backward(ctx, *grads):
-        _seen(*grads)
-        return marked(ctx, *grads) if torch.is_grad_enabled() else f(ctx, *grads)
+        if forward_ad._current_level >= 0 or _fx._is_fx_tracing_flag or _tracing():
+            _followed(*grads)
+        return marked(ctx, *grads) if _grad_enabled() else f(ctx, *grads)
     return staticmethod(backward)
 
 
@@ -223,10 +230,9 @@ def _norm_parts(rows, width):
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis (biased variance), statistics in float32.
     x [..., C] with C <= 8192; weight, bias float32 [C] or None."""
-    _seen(x, weight, bias)
     if type(eps) is not float:
         eps = _number('eps', eps)
-    _first(x, None, '')
+    _first(x, None, '', weight, bias)
     if _elsewhere(x):
         with torch.cuda.device(x.device):
             return layer_norm(x, weight, bias, eps)
@@ -309,8 +315,7 @@ def causal_conv(x, weight, bias=None, activation='silu', state=None, lengths=Non
     y_t = act(bias + sum_k weight[:, k] x_{t - taps + 1 + k}), act = silu or (activation=None) nothing; weight float32
     [D, taps], bias float32 [D].  state [B, taps - 1, D] (x's type): the rows before the first (None: zeros).  Returns y,
     or with return_state (y, state after each sequence's last token)."""
-    _seen(x, weight, bias, state, lengths)
-    _first(x, 3, '[B, L, D]')
+    _first(x, 3, '[B, L, D]', weight, bias, state, lengths)
     if _elsewhere(x):
         with torch.cuda.device(x.device):
             return causal_conv(x, weight, bias, activation, state, lengths, return_state)
@@ -333,8 +338,7 @@ def causal_conv(x, weight, bias=None, activation='silu', state=None, lengths=Non
 def causal_conv_step(x, state, weight, bias=None, activation='silu'):
     """causal_conv for ONE new token per sequence: x [B, D]; state [B, taps - 1, D] (x's type; rows may be strided) is
     shifted in place.  Returns y [B, D].  Forward only."""
-    _seen(x, state, weight, bias)
-    _first(x, 2, '[B, D]')
+    _first(x, 2, '[B, D]', state, weight, bias)
     if _elsewhere(x):
         with torch.cuda.device(x.device):
             return causal_conv_step(x, state, weight, bias, activation)
@@ -474,8 +478,7 @@ def selective_scan(x, dt, a, b, c, skip=None, gate=None, dt_bias=None, softplus=
     dt, gate [B, L, D]; b, c [B, L, N], or [B, L, G, N] where each of G groups of D / G channels has its own; a float32
     [D, N]; skip, dt_bias float32 [D]; state float32 [B, D, N] (None: zeros).  gate, skip, dt_bias may be None.
     Returns y, or with return_state (y, state after each sequence's last token)."""
-    _seen(x, dt, a, b, c, skip, gate, dt_bias, state, lengths)
-    _first(x, 3, '[B, L, D]')
+    _first(x, 3, '[B, L, D]', dt, a, b, c, skip, gate, dt_bias, state, lengths)
     if _elsewhere(x):
         with torch.cuda.device(x.device):
             return selective_scan(x, dt, a, b, c, skip, gate, dt_bias, softplus, state, lengths, return_state)
@@ -515,8 +518,7 @@ def _ready(x, dt, a, b, c, skip, gate, dt_bias):
 def selective_scan_step(x, state, dt, a, b, c, skip=None, gate=None, dt_bias=None, softplus=True):
     """selective_scan for ONE new token per sequence: x, dt, gate [B, D]; b, c [B, N] or [B, G, N]; state float32
     [B, D, N] is updated in place (its batch axis may be strided).  Returns y [B, D].  Forward only."""
-    _seen(x, state, dt, a, b, c, skip, gate, dt_bias)
-    _first(x, 2, '[B, D]')
+    _first(x, 2, '[B, D]', state, dt, a, b, c, skip, gate, dt_bias)
     if _elsewhere(x):
         with torch.cuda.device(x.device):
             return selective_scan_step(x, state, dt, a, b, c, skip, gate, dt_bias, softplus)
