@@ -345,9 +345,11 @@ int vqa_clip_adamax(void* stream, float* p, const float* g, float* m, float* u, 
 /* ---------------------------------------------------------------- sequence operators (vqa_amd/sequence.py)
  * NO COUNTERPART IN THE REFERENCE: a norm, a short convolution and a linear recurrence over tokens, beside its BatchNorm,
  * convolutions and GRU.  dtype 0, 1 or 2 (f16 as well) for the rows; parameters, states of the scan, statistics and every
- * sum are f32.  Strides are in elements, the last axis is contiguous; 16-byte accesses are used where pointers, strides
- * and widths allow them, element accesses elsewhere.  lengths (int32 [B], may be NULL): tokens at or past lengths[b] are
- * padding - zero rows out, zero gradients, no part in any sum or state, whatever they hold. */
+ * sum are f32.  Strides are in elements, the last axis is contiguous.  Layer norm moves 16 bytes a lane and the convolution
+ * four elements, at any alignment (what a width leaves over: single elements, or a last vector that overlaps its neighbour);
+ * the scan up to 16 bytes where a group's channels are a multiple of 16 bytes and pointers and strides of 4, else single
+ * elements.  lengths (int32 [B], may be NULL): tokens at or past lengths[b] are padding - zero rows out, zero gradients, no
+ * part in any sum or state, whatever they hold. */
 
 /* y = (x - mean) rstd weight + bias over the last axis; x [rows] with stride ldx, y contiguous; width <= 8192; weight /
  * bias may be NULL (1 / 0); stats [2][rows] (mean, rstd; may be NULL) is what the backward needs. */

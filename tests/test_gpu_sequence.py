@@ -4,6 +4,7 @@ padded batches, carried states, single tokens, strides, types, streams, graphs, 
 Roundings counted in a tolerance (sequence_ref.close): layer norm and the convolution chain a few operations per value plus
 their sums' partial chains (rows / 16 rows side by side); a scan's state takes 3 roundings a token and its decay's error is
 that of dt (about 16: softplus by exponential, reciprocal and a series of 7 terms) times dt a e^{dt a} <= 1/e."""
+# (softplus now takes a polynomial of degree 4 in place of the series: fewer roundings than the 16 that are counted)
 import pytest
 import torch
 
@@ -1045,3 +1046,28 @@ def test_selective_scan_narrow_groups(B, T, D, N, G, dtype, lengths):
     lens = torch.tensor(lengths, dtype=torch.int32) if lengths is not None else None
     leaves, dy, dlast = _scan_case(B, T, D, N, G, dtype, seed=46)
     _scan_check(leaves, dy, dlast, lens)
+
+
+@pytest.mark.parametrize('T,N,lengths', [(13, 16, None), (21, 5, [17]), (300, 16, None), (40, 33, [33])])
+def test_selective_scan_infinite_last_state(T, N, lengths):
+    """The last token's x is infinite: no token follows, so a's gradient has no infinite state in it."""
+    g = _gen(47)
+    B, D = 1, 24
+    rn = lambda *s: torch.rand(*s, generator=g) + 0.125                          # noqa: E731
+    v = dict(x=rn(B, T, D), dt=rn(B, T, D), a=-rn(D, N), b=rn(B, T, 1, N), c=rn(B, T, 1, N), skip=rn(D))
+    end = T if lengths is None else lengths[0]
+    v['x'][0, end - 1, 3] = float('inf')
+    lens = None if lengths is None else torch.tensor(lengths, dtype=torch.int32)
+    dy, dlast = rn(B, T, D), rn(B, D, N)
+    dev = {k: t.cuda().requires_grad_(True) for k, t in v.items()}
+    ref = {k: t.double().requires_grad_(True) for k, t in v.items()}
+    y, last = S().selective_scan(*(dev[k] for k in SCAN[:6]), lengths=None if lens is None else lens.cuda(), return_state=True)
+    yr, lastr = R.scan(*(ref[k] for k in SCAN[:6]), None, None, True, None, lens)
+    for ends in (1, 2):
+        got = _grads([y, last][:ends], [dy.cuda(), dlast.cuda()], dev)
+        want = torch.autograd.grad([yr, lastr][:ends], list(ref.values()), [dy.double(), dlast.double()][:ends], retain_graph=True)
+        want = dict(zip(ref, want))
+        assert want['a'].isfinite().all()
+        for k in ('a', 'x', 'dt'):
+            _same_kind('d' + k, got[k], want[k], 2 * (128 + 8 * T) + (B * T if k == 'a' else 0))
+        y, last = S().selective_scan(*(dev[k] for k in SCAN[:6]), lengths=None if lens is None else lens.cuda(), return_state=True)

@@ -583,7 +583,8 @@ __global__ __launch_bounds__(64) void scan_bwd_ends(Args A) {
 // registers are why a lane has half the forward's channels: at 16 states a lane they do not fit, and the spills cost more
 // than all the rest (566 us against 88 of the forward at 4 x 2048 tokens x 2048 channels, N = 16, bf16; this form: 231).  What
 // two waves a SIMD leave of 256 registers keeps the decays of a tile's last KD tokens for the way back (five: 251 -> 231 us;
-// with a sixth one wave fits, 308 us); the other tokens' are formed again.  The vector ALU is busy 3/4 of the time.
+// with a sixth one wave fits, 308 us); the other tokens' are formed again.  The scalar registers do not suffice: about 100 of
+// them lie in lanes of vector registers, and every tile reads them back on the vector ALU, which is busy 3/4 of the time.
 // The BW waves of a workgroup take neighbouring channels, share b and c in LDS and join their sums db, dc over channels
 // there: part_bc[workgroup of the group][B][L][G][2][N].  A workgroup takes the sequences of its batch group one after the
 // other, so that its sums over tokens leave once: part_p[(batch group, segment)]{da [channel][NP], dskip, ddt_bias}.
@@ -730,6 +731,17 @@ __global__ __launch_bounds__(64 * BW, CH * NS > 8 ? 1 : 2) void scan_bwd(Args A)
                     s_y[t * W::WC + w.cl * CH + own_channel<CH>(w.r)] = sum_states<CH>(y);
                     put_sums<NS>(s_dc + t * W::NP, sc, w.r, w.cl);
                 }
+                // a token past the end takes no part in da: its dt of 0 times an infinite state would be NaN.  (The empty asm
+                // keeps this a branch over the tokens that are there, not a select for each of their states.)
+#pragma unroll
+                for (int t = 1; t < TT; ++t)
+                    if (t0 + t >= te) {
+                        asm volatile("");
+#pragma unroll
+                        for (int i = 0; i < CH; ++i)
+#pragma unroll
+                            for (int j = 0; j < NS; ++j) hist[t][i][j] = 0.f;
+                    }
                 lds_order();                           // (and the decays are formed again, not held in registers)
 #pragma unroll
                 for (int t = TT - 1; t >= 0; --t) {
@@ -967,9 +979,10 @@ int np_of(int N) { return N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
 int fwd_channels(int N) { return N <= 16 ? 64 : N <= 32 ? 32 : 16; }
 int bwd_channels(int N) { return N <= 16 ? 32 * BW : 16 * BW; }
 
-// Segments cost a second pass over the tokens, so there are none while whole sequences make enough waves (counted in the
-// forward's 64 channels): 400 in the forward (B x 512 x 2048: 512 waves 122 us and 162 in segments, 384 118 and 124, 256 115
-// and 90), 640 in the backward (768 waves 446 us and 472, 512 335 and 316).  Below that, enough for 4096 waves with eight tiles
+// Segments cost a second pass over the tokens, so there are none while whole sequences make enough waves (counted as the
+// forward's: of 64 channels up to 16 states, 32 up to 32, 16 above; the figures are of 16 states): 400 in the forward
+// (B x 512 x 2048: 512 waves 122 us and 162 in segments, 384 118 and 124, 256 115 and 90), 640 in the backward (768 waves 446
+// us and 472, 512 335 and 316).  Below that, enough for 4096 waves with eight tiles
 // each at least (2048 to 8192 waves are the same within 3 %), or for 1024 waves with two tiles each, whichever is more
 // (3 x 577 x 600, 30 waves whole, training: 145 us with eight tiles each, 101 with four, 82 with two).
 void plan(Args& A, bool bwd) {
