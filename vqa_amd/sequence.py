@@ -34,7 +34,8 @@ _ROW_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 _F32 = torch.float32
 
 
-_device, _grad_enabled, _tracing = torch._C._cuda_getDevice, torch.is_grad_enabled, torch._C._is_tracing
+_device, _stream_of = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_grad_enabled, _tracing = torch.is_grad_enabled, torch._C._is_tracing
 
 
 def _elsewhere(x):
@@ -248,9 +249,11 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 # --------------------------------------------------------------------------------------------------- causal convolution
 
 def _silu_flag(activation):
-    if activation not in (None, 'silu'):
+    if activation == 'silu':
+        return 1
+    if activation is not None:
         _fail(f"activation is {activation!r}: 'silu' or None is wanted")
-    return int(activation == 'silu')
+    return 0
 
 
 def _taps(weight, D):
@@ -357,9 +360,11 @@ def causal_conv_step(x, state, weight, bias=None, activation='silu'):
         _fail(f'state has strides {state.stride()}: it is updated in place, so rows must be contiguous and apart')
     x = _unit(x)
     if L._PROFILE is None and L._REC is None:
-        L.check(L.lib().vqa_causal_conv_token(
-            L._raw_stream(), L.dt(x), x.data_ptr(), x.stride(0), state.data_ptr(), s0, s1, weight.data_ptr(),
-            None if bias is None else bias.data_ptr(), B, D, taps, silu, y.data_ptr()), 'vqa_causal_conv_token')
+        rc = L.lib().vqa_causal_conv_token(
+            _stream_of(x.get_device()), L.dt(x), x.data_ptr(), x.stride(0), state.data_ptr(), s0, s1, weight.data_ptr(),
+            None if bias is None else bias.data_ptr(), B, D, taps, silu, y.data_ptr())
+        if rc:
+            L.check(rc, 'vqa_causal_conv_token')
     else:
         L.call('vqa_causal_conv_token', L.dt(x), x, x.stride(0), state, s0, s1, weight, bias, B, D, taps, silu, y)
     _touched(state)
@@ -540,11 +545,13 @@ def selective_scan_step(x, state, dt, a, b, c, skip=None, gate=None, dt_bias=Non
     sg, softplus = 0 if gate is None else gate.stride(0), int(softplus)
     if L._PROFILE is None and L._REC is None:
         # (one token's latency is host time: pointers are taken here, 3 us less than by L.call)
-        L.check(L.lib().vqa_scan_token(
-            L._raw_stream(), L.dt(x), x.data_ptr(), x.stride(0), state.data_ptr(), s0, dt.data_ptr(),
+        rc = L.lib().vqa_scan_token(
+            _stream_of(x.get_device()), L.dt(x), x.data_ptr(), x.stride(0), state.data_ptr(), s0, dt.data_ptr(),
             dt.stride(0), None if gate is None else gate.data_ptr(), sg, a.data_ptr(), b.data_ptr(), b.stride(0),
             c.data_ptr(), c.stride(0), None if skip is None else skip.data_ptr(),
-            None if dt_bias is None else dt_bias.data_ptr(), softplus, B, D, N, G, y.data_ptr()), 'vqa_scan_token')
+            None if dt_bias is None else dt_bias.data_ptr(), softplus, B, D, N, G, y.data_ptr())
+        if rc:
+            L.check(rc, 'vqa_scan_token')
     else:
         L.call('vqa_scan_token', L.dt(x), x, x.stride(0), state, s0, dt, dt.stride(0), gate, sg, a, b,
                b.stride(0), c, c.stride(0), skip, dt_bias, softplus, B, D, N, G, y)
