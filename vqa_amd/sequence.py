@@ -136,6 +136,11 @@ def _unit(x):
     return x if x.stride(-1) == 1 else x.contiguous()
 
 
+def _like(x):
+    """A contiguous tensor of x's kind for a result"""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 def _near(x):
     """... and rows whose distance the scan's kernels can take (8 rows within 2 GiB)"""
     if x.dim() == 2 or x.stride(1) < 1 << 26:
@@ -188,7 +193,7 @@ def _as_matrix(x):
 def _norm_fwd(x, weight, bias, eps, stats):
     x2 = _as_matrix(x)
     rows, width = x2.shape
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = _like(x)
     st = torch.empty(2, rows, device=x.device, dtype=_F32) if stats else None
     if rows:
         L.call('vqa_layer_norm_fwd', L.dt(x), x2, x2.stride(0), weight, bias, rows, width, eps, y, st)
@@ -265,7 +270,7 @@ def _taps(weight, D):
 def _conv_fwd(x, weight, bias, silu, state, lengths, want_last):
     B, T, D = x.shape
     taps = weight.shape[1]
-    y = torch.empty(B, T, D, device=x.device, dtype=x.dtype)
+    y = _like(x)
     last = torch.empty(B, taps - 1, D, device=x.device, dtype=x.dtype) if want_last else None
     if y.numel():
         L.call('vqa_causal_conv_fwd', L.dt(x), x, x.stride(0), x.stride(1), weight, bias, state, lengths, B, T, D, taps,
@@ -393,7 +398,7 @@ def _strides(x):
 def _scan_fwd(x, dt, a, b, c, skip, gate, dt_bias, softplus, state, lengths, want_last, want_keep):
     B, T, D = x.shape
     G, N, dev, code = b.shape[2], b.shape[3], x.device, L.dt(x)
-    y = torch.empty(B, T, D, device=dev, dtype=x.dtype)
+    y = _like(x)
     last = torch.empty(B, D, N, device=dev, dtype=_F32) if want_last else None
     if not y.numel():
         if want_last and last.numel():
